@@ -57,6 +57,32 @@ class LlmdotSampling(C.Structure):
         super().__init__(top_k, top_p, temperature, repeat_penalty, repeat_window, seed)
 
 
+class KvqPool(C.Structure):
+    """llmdot_kvq_pool."""
+    _fields_ = [("format", C.c_int32), ("head_dim", C.c_int32), ("heads_kv", C.c_int32), ("n_pages", C.c_int32),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
+
+
+class KvqBatch(C.Structure):
+    """llmdot_kvq_batch."""
+    _fields_ = [("batch", C.c_int32), ("rows", C.c_int32), ("max_rows", C.c_int32), ("max_pages", C.c_int32),
+                ("row_start", C.c_void_p), ("seq_len", C.c_void_p), ("pages", C.c_void_p)]
+
+
+class KvqAttn(C.Structure):
+    """llmdot_kvq_attn."""
+    _fields_ = [("heads", C.c_int32), ("type", C.c_uint32), ("prefix_len", C.c_int32), ("window", C.c_int32),
+                ("scale", C.c_float), ("softcap", C.c_float), ("prefix_pages", C.c_void_p)]
+
+
+class Verify(C.Structure):
+    """llmdot_verify."""
+    _fields_ = [("batch", C.c_int32), ("drafts", C.c_int32), ("vocab", C.c_int32), ("reserved", C.c_int32),
+                ("p", C.c_void_p), ("q", C.c_void_p), ("ld_p", C.c_int64), ("ld_q", C.c_int64),
+                ("draft", C.c_void_p), ("uniform", C.c_void_p), ("n_draft", C.c_void_p), ("tokens", C.c_void_p),
+                ("accepted", C.c_void_p)]
+
+
 F32P = C.POINTER(C.c_float)
 U8P = C.POINTER(C.c_uint8)
 I32P = C.POINTER(C.c_int32)
@@ -118,6 +144,13 @@ _SIGS = {
     "llmdot_cuda_profile_step": (C.c_int, [C.POINTER(VP), C.c_int, I32P, I32P, C.c_int, F32P, C.POINTER(C.c_int)]),
     "llmdot_cuda_profile_matvec": (C.c_int, [VP, C.c_char_p, C.c_int, C.c_int, F32P, C.POINTER(C.c_uint64)]),
     "llmdot_cuda_argmax_noalloc": (C.c_int, [VP, C.c_int, C.c_int, C.c_int, VP, VP]),
+    "llmdot_cuda_kvq_write": (C.c_int, [C.POINTER(KvqPool), C.POINTER(KvqBatch), VP, VP, C.c_uint32, C.c_int64, C.c_int64, VP]),
+    "llmdot_cuda_kvq_read": (C.c_int, [C.POINTER(KvqPool), C.POINTER(KvqBatch), VP, VP, C.c_uint32, C.c_int64, C.c_int64, VP]),
+    "llmdot_cuda_kvq_attention_workspace": (C.c_int, [C.POINTER(KvqPool), C.POINTER(KvqBatch), C.POINTER(KvqAttn),
+                                                      C.POINTER(C.c_size_t)]),
+    "llmdot_cuda_kvq_attention": (C.c_int, [C.POINTER(KvqPool), C.POINTER(KvqBatch), C.POINTER(KvqAttn), VP, C.c_int64,
+                                            VP, C.c_int64, VP, VP, C.c_size_t, VP]),
+    "llmdot_cuda_verify_draft": (C.c_int, [C.POINTER(Verify), VP]),
     "llmdot_cuda_model_matvec": (C.c_int, [VP, C.c_char_p, F32P, C.c_int, C.c_int, F32P, F32P]),
 }
 

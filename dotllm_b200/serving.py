@@ -1,0 +1,214 @@
+"""Serving operators over the C ABI: an 8-bit paged KV pool (write, read), attention of a batch over
+a shared prefix and its own pages, and the verification of drafted tokens.
+
+Arguments are CUDA tensors; a call runs on the calling thread's current torch stream of their
+device, asynchronously, and returns new tensors (outputs and scratch come from torch's allocator on
+that stream).  Wrong types, shapes, strides or devices raise ``ValueError`` before the call; what
+the library refuses raises ``CudaBackendError``.  There is no other path: without the library or a
+device every call fails.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+
+from . import native
+from .native import check, lib
+
+PAGE = 64
+KVQ_I8, KVQ_E4M3 = 0, 1
+_FORMATS = {torch.int8: KVQ_I8, torch.float8_e4m3fn: KVQ_E4M3}
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 25}
+
+
+def _bad(text: str):
+    raise ValueError(text)
+
+
+def _int32(name: str, t: torch.Tensor, shape: tuple, device) -> int:
+    if t.dtype is not torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
+        _bad(f"{name}: needs a contiguous int32 tensor of shape {shape} on {device}")
+    return t.data_ptr()
+
+
+class KvqPool:
+    """Pages of 8-bit K and V: codes ``[n_pages, heads_kv, 64, head_dim]`` (int8 or float8_e4m3fn) and
+    fp32 scales ``[n_pages, heads_kv, 64]``.  Holds the tensors; many batches share one pool."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        fmt, shape, device = _FORMATS.get(k.dtype), k.shape, k.device
+        if fmt is None or v.dtype is not k.dtype:
+            _bad("KvqPool: codes must be int8 or float8_e4m3fn, K and V alike")
+        if len(shape) != 4 or shape[2] != PAGE or v.shape != shape:
+            _bad("KvqPool: codes must be [n_pages, heads_kv, 64, head_dim], K and V alike")
+        if k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32 or k_scale.shape != shape[:3] \
+                or v_scale.shape != shape[:3]:
+            _bad("KvqPool: scales must be float32 [n_pages, heads_kv, 64]")
+        if not (k.is_cuda and v.device == device and k_scale.device == device and v_scale.device == device):
+            _bad("KvqPool: all tensors must be on one CUDA device")
+        if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
+            _bad("KvqPool: tensors must be contiguous")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.device = device
+        self.n_pages, self.heads_kv, self.head_dim = shape[0], shape[1], shape[3]
+        self._c = native.KvqPool(fmt, shape[3], shape[1], shape[0], k.data_ptr(), v.data_ptr(), k_scale.data_ptr(),
+                                 v_scale.data_ptr())
+
+    @classmethod
+    def empty(cls, n_pages: int, heads_kv: int, head_dim: int, dtype: torch.dtype = torch.int8, device="cuda") -> "KvqPool":
+        """A new pool; its contents are undefined until written."""
+        shape = (n_pages, heads_kv, PAGE, head_dim)
+        return cls(torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device),
+                   torch.empty(shape[:3], dtype=torch.float32, device=device),
+                   torch.empty(shape[:3], dtype=torch.float32, device=device))
+
+
+class KvqBatch:
+    """Sequences over a pool: ``pages[b, i]`` holds positions 64 i .. 64 i + 63 of sequence b,
+    ``seq_len[b]`` is its length, and rows ``row_start[b] .. row_start[b + 1]`` of a call are its last
+    positions.  ``max_rows`` bounds the rows of any one sequence."""
+
+    def __init__(self, row_start: torch.Tensor, seq_len: torch.Tensor, pages: torch.Tensor, max_rows: int):
+        if pages.dim() != 2:
+            _bad("KvqBatch: pages must be [batch, max_pages]")
+        B, most = pages.shape
+        device = pages.device
+        if not pages.is_cuda:
+            _bad("KvqBatch: tensors must be on a CUDA device")
+        if max_rows < 0:
+            _bad("KvqBatch: max_rows is negative")
+        self.row_start, self.seq_len, self.pages, self.device = row_start, seq_len, pages, device
+        self._c = native.KvqBatch(B, 0, max_rows, most, _int32("row_start", row_start, (B + 1,), device),
+                                  _int32("seq_len", seq_len, (B,), device), _int32("pages", pages, (B, most), device))
+
+
+def _rows(name: str, t: torch.Tensor, heads: int, dim: int, device) -> int:
+    """ld of a [rows, heads, dim] tensor whose rows may be strided; its heads and values are dense."""
+    s = t.shape
+    if len(s) != 3 or s[1] != heads or s[2] != dim or t.device != device:
+        _bad(f"{name}: needs [rows, {heads}, {dim}] on {device}")
+    st = t.stride()
+    if st[2] != 1 or (st[1] != dim and heads > 1) or (s[0] > 1 and st[0] < heads * dim):
+        _bad(f"{name}: heads and values of a row must be dense and rows must not overlap")
+    return st[0]
+
+
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+class _On:
+    """The library launches on the current device: make it the tensors' one."""
+
+    def __new__(cls, device):
+        return torch.cuda.device(device)
+
+
+def kvq_write(pool: KvqPool, batch: KvqBatch, k: torch.Tensor, v: torch.Tensor) -> None:
+    """Quantise the rows ``k`` and ``v`` ([rows, heads_kv, head_dim], float32, float16 or bfloat16; rows
+    may be strided) into their positions' slots of the pool."""
+    if k.dtype not in _TYPES or v.dtype is not k.dtype or v.shape != k.shape:
+        _bad("kvq_write: K and V must be float32, float16 or bfloat16, alike")
+    if batch.device != pool.device:
+        _bad("kvq_write: pool and batch are on different devices")
+    ld_k = _rows("k", k, pool.heads_kv, pool.head_dim, pool.device)
+    ld_v = _rows("v", v, pool.heads_kv, pool.head_dim, pool.device)
+    batch._c.rows = k.shape[0]
+    with _On(pool.device):
+        check(lib().llmdot_cuda_kvq_write(pool._c, batch._c, k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], ld_k, ld_v,
+                                          _stream(pool.device)))
+
+
+def kvq_read(pool: KvqPool, batch: KvqBatch, rows: int, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The rows' positions as values: K and V, each [rows, heads_kv, head_dim]."""
+    if dtype not in _TYPES:
+        _bad("kvq_read: dtype must be float32, float16 or bfloat16")
+    if rows < 0 or batch.device != pool.device:
+        _bad("kvq_read: negative rows, or pool and batch on different devices")
+    out = torch.empty((2, rows, pool.heads_kv, pool.head_dim), dtype=dtype, device=pool.device)
+    ld = pool.heads_kv * pool.head_dim
+    batch._c.rows = rows
+    k, v = out[0], out[1]
+    with _On(pool.device):
+        check(lib().llmdot_cuda_kvq_read(pool._c, batch._c, k.data_ptr(), v.data_ptr(), _TYPES[dtype], ld, ld,
+                                         _stream(pool.device)))
+    return k, v
+
+
+def kvq_attention(pool: KvqPool, batch: KvqBatch, q: torch.Tensor, prefix_pages: Optional[torch.Tensor] = None,
+                  prefix_len: int = 0, scale: Optional[float] = None, softcap: float = 0.0, window: int = 0,
+                  return_lse: bool = False):
+    """Attention of the rows ``q`` ([rows, heads, head_dim]; rows may be strided) over the shared prefix
+    (``prefix_len`` positions in the pages ``prefix_pages``) and their sequences' own positions.  Returns the
+    output in q's type, and with ``return_lse`` the log of the exponentials' sum, [rows, heads] fp32.
+    ``scale`` defaults to head_dim ** -0.5."""
+    if q.dtype not in _TYPES or q.dim() != 3:
+        _bad("kvq_attention: q must be float32, float16 or bfloat16 [rows, heads, head_dim]")
+    rows, heads = q.shape[0], q.shape[1]
+    device = pool.device
+    if batch.device != device:
+        _bad("kvq_attention: pool and batch are on different devices")
+    ld = _rows("q", q, heads, pool.head_dim, device)
+    prefix = 0
+    if prefix_len > 0:
+        if prefix_pages is None:
+            _bad("kvq_attention: prefix_len without prefix_pages")
+        if prefix_pages.dim() != 1 or prefix_pages.shape[0] * PAGE < prefix_len:
+            _bad("kvq_attention: prefix_pages holds fewer than prefix_len positions")
+        prefix = _int32("prefix_pages", prefix_pages, tuple(prefix_pages.shape), device)
+    a = native.KvqAttn(heads, _TYPES[q.dtype], prefix_len, window, pool.head_dim ** -0.5 if scale is None else scale, softcap,
+                       prefix)
+    batch._c.rows = rows
+    out = torch.empty((rows, heads, pool.head_dim), dtype=q.dtype, device=device)
+    lse = torch.empty((rows, heads), dtype=torch.float32, device=device) if return_lse else None
+    need = C.c_size_t()
+    check(lib().llmdot_cuda_kvq_attention_workspace(pool._c, batch._c, a, need))
+    work = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    with _On(device):
+        check(lib().llmdot_cuda_kvq_attention(pool._c, batch._c, a, q.data_ptr(), ld, out.data_ptr(), heads * pool.head_dim,
+                                              lse.data_ptr() if return_lse else None, work.data_ptr() if need.value else None,
+                                              need.value, _stream(device)))
+    return (out, lse) if return_lse else out
+
+
+def verify_draft(p: torch.Tensor, q: Optional[torch.Tensor], draft: torch.Tensor, uniform: torch.Tensor,
+                 n_draft: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Verify drafted tokens against the target's probabilities.
+
+    ``p`` [batch, k + 1, vocab] and ``q`` [batch, k, vocab] (None: drafts without probabilities, as from a
+    lookup) are float32; ``draft`` [batch, k] int32; ``uniform`` [batch, k + 1] float32 in [0, 1), the last of a
+    row for the drawn token; ``n_draft`` [batch] int32 counts a sequence's drafts (None: k).  Returns
+    ``tokens`` [batch, k + 1] int32 -- the accepted drafts, the drawn token, then -1 -- and ``accepted`` [batch]."""
+    if p.dtype is not torch.float32 or p.dim() != 3 or not p.is_cuda:
+        _bad("verify_draft: p must be a float32 CUDA tensor [batch, drafts + 1, vocab]")
+    B, k1, V = p.shape
+    device, k = p.device, k1 - 1
+    if k < 0:
+        _bad("verify_draft: p holds no row")
+
+    def ld(name, t, n):
+        st = t.stride()
+        if t.dtype is not torch.float32 or t.shape != (B, n, V) or t.device != device or (V > 1 and st[2] != 1) \
+                or (n > 0 and B > 1 and st[0] != n * st[1]) or (n > 1 and st[1] < V):
+            _bad(f"verify_draft: {name} must be float32 [{B}, {n}, {V}] on {device} with evenly strided rows")
+        return max(st[1], V)
+
+    ld_p = ld("p", p, k1)
+    if q is not None and k == 0:
+        if q.shape != (B, 0, V):
+            _bad(f"verify_draft: q must be [{B}, 0, {V}]")
+        q = None  # no draft, nothing to subtract
+    ld_q = ld("q", q, k) if q is not None else 0
+    if uniform.dtype is not torch.float32 or uniform.shape != (B, k1) or uniform.device != device or not uniform.is_contiguous():
+        _bad(f"verify_draft: uniform must be contiguous float32 [{B}, {k1}] on {device}")
+    tokens = torch.empty((B, k1), dtype=torch.int32, device=device)
+    accepted = torch.empty((B,), dtype=torch.int32, device=device)
+    a = native.Verify(B, k, V, 0, p.data_ptr(), q.data_ptr() if q is not None else None, ld_p, ld_q,
+                      _int32("draft", draft, (B, k), device), uniform.data_ptr(),
+                      _int32("n_draft", n_draft, (B,), device) if n_draft is not None else None, tokens.data_ptr(),
+                      accepted.data_ptr())
+    with _On(device):
+        check(lib().llmdot_cuda_verify_draft(a, _stream(device)))
+    return tokens, accepted

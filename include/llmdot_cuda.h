@@ -381,6 +381,112 @@ LLMDOT_API int llmdot_cuda_profile_step(llmdot_session **sessions, int batch, co
 LLMDOT_API int llmdot_cuda_argmax_noalloc(const float *d_logits, int n, int rows, int ld, int32_t *d_index,
                                           void *stream);
 
+/* ====================================================================================
+ * Serving operators -- device pointers, caller's memory, caller's stream.
+ * No counterpart in the reference (its engine holds one fp32 cache per session).  All pointers
+ * named d_* or held by the structs below are device memory of the current device; the structs
+ * themselves are host memory, read during the call only.  Every call is asynchronous on `stream`
+ * (a cudaStream_t as a plain pointer, NULL = the legacy default stream), allocates nothing, keeps
+ * nothing between calls, and can be captured into a CUDA graph: sequence lengths, row counts and
+ * page lists are read on the device.  Page ids outside the pool and positions outside a page list
+ * are never followed (a write skips them, a read returns zeros, attention does not see them).
+ * ==================================================================================== */
+
+/* Pool of KV pages held in 8 bits: LLMDOT_KV_PAGE positions of one kv head are one contiguous run
+ * of codes, [n_pages][heads_kv][64][head_dim], with one fp32 scale per position and head,
+ * [n_pages][heads_kv][64].  A code stands for code * scale.  head_dim is 64, 96, 128 or 256.  The
+ * code arrays are 16-byte aligned. */
+#define LLMDOT_KV_PAGE 64
+#define LLMDOT_KVQ_I8 0   /* signed 8-bit integers, -127..127 */
+#define LLMDOT_KVQ_E4M3 1 /* 8-bit floating point, 4 exponent bits, 3 mantissa bits, largest 448 */
+typedef struct llmdot_kvq_pool {
+    int32_t format; /* LLMDOT_KVQ_* */
+    int32_t head_dim;
+    int32_t heads_kv;
+    int32_t n_pages;
+    void *k, *v;
+    float *k_scale, *v_scale;
+} llmdot_kvq_pool;
+
+/* A batch of sequences over a pool.  pages[b][i] holds positions 64 i .. 64 i + 63 of sequence b
+ * (max_pages entries each); seq_len[b] is its number of positions.  The call's rows are packed:
+ * rows row_start[b] .. row_start[b + 1] - 1 are the LAST positions of sequence b, in order (a row
+ * that would fall before position 0 is no position).  max_rows bounds the rows of any sequence;
+ * rows beyond it are not computed. */
+typedef struct llmdot_kvq_batch {
+    int32_t batch;
+    int32_t rows; /* row_start[batch] */
+    int32_t max_rows;
+    int32_t max_pages;
+    const int32_t *row_start; /* [batch + 1], row_start[0] = 0 */
+    const int32_t *seq_len;   /* [batch] */
+    const int32_t *pages;     /* [batch][max_pages] */
+} llmdot_kvq_batch;
+
+/* Quantise rows of K and V into their positions' slots.  d_k and d_v hold [rows][heads_kv][head_dim]
+ * values of `type` (LLMDOT_F32, LLMDOT_F16 or LLMDOT_BF16), ld_k / ld_v elements from one row to
+ * the next.  Per row and head, a = max |x|: scale = a / M and code = rne(x * (M * (1 / a))), each
+ * operation rounded to fp32, with M = 127 or 448; a < 1e-30 gives scale 0 and zero codes; a row with
+ * a NaN or an infinity gives a NaN scale and zero codes.  Two rows of one call must not be the same position of the same page. */
+LLMDOT_API int llmdot_cuda_kvq_write(const llmdot_kvq_pool *pool, const llmdot_kvq_batch *batch, const void *d_k,
+                                     const void *d_v, uint32_t type, int64_t ld_k, int64_t ld_v, void *stream);
+/* The rows' positions read back: d_k and d_v receive [rows][heads_kv][head_dim] values
+ * code * scale of `type`, rounded once; rows that are no position receive zeros. */
+LLMDOT_API int llmdot_cuda_kvq_read(const llmdot_kvq_pool *pool, const llmdot_kvq_batch *batch, void *d_k, void *d_v,
+                                    uint32_t type, int64_t ld_k, int64_t ld_v, void *stream);
+
+/* Attention of a batch whose sequences share a prefix.  The prefix is prefix_len positions in the
+ * pages prefix_pages (ceil(prefix_len / 64) of them); sequence b's own positions follow it, so
+ * position j of sequence b is prefix_len + j of the whole.  A row at whole position p sees positions
+ * <= p, and with window > 0 only those > p - window.  Query head h reads kv head h / (heads /
+ * heads_kv).  s = scale * q . k, then softcap * tanh(s / softcap) when softcap > 0; the output is
+ * sum softmax(s) v, in `type`; sums and softmax in fp32.  A row that sees nothing gives zeros and a
+ * log-sum of -infinity. */
+typedef struct llmdot_kvq_attn {
+    int32_t heads; /* a multiple of heads_kv */
+    uint32_t type; /* of q and the output: LLMDOT_F32, LLMDOT_F16 or LLMDOT_BF16 */
+    int32_t prefix_len;
+    int32_t window; /* 0 = none */
+    float scale;
+    float softcap;                /* 0 = none */
+    const int32_t *prefix_pages; /* may be NULL when prefix_len is 0 */
+} llmdot_kvq_attn;
+/* Bytes of scratch that the call below needs (0 is possible); host only, no device needed. */
+LLMDOT_API int llmdot_cuda_kvq_attention_workspace(const llmdot_kvq_pool *pool, const llmdot_kvq_batch *batch,
+                                                   const llmdot_kvq_attn *attn, size_t *bytes);
+/* d_q and d_out: [rows][heads][head_dim], ld_q / ld_out elements from one row to the next.
+ * d_lse (nullable): [rows][heads] fp32, the natural log of sum exp(s).  d_work: work_bytes bytes,
+ * 16-byte aligned, not shared with a call that may run at the same time. */
+LLMDOT_API int llmdot_cuda_kvq_attention(const llmdot_kvq_pool *pool, const llmdot_kvq_batch *batch,
+                                         const llmdot_kvq_attn *attn, const void *d_q, int64_t ld_q, void *d_out,
+                                         int64_t ld_out, float *d_lse, void *d_work, size_t work_bytes, void *stream);
+
+/* Verification of drafted tokens (speculative decoding) from given uniform numbers.  For each
+ * sequence b with n = n_draft[b] drafts x_0 .. x_{n-1}, target probabilities p_i (i = 0..n) and
+ * draft probabilities q_i: draft i is accepted when all before it were and u_i * q_i(x_i) < p_i(x_i)
+ * (a NaN or a token outside the vocabulary is refused).  With a accepted, the next token is drawn
+ * with the uniform number u_drafts (the row's last) from w = clamp(p_a - q_a, 0, 1) if a < n, else
+ * clamp(p_n, 0, 1), a NaN weighing 0:
+ * W_j = floor(w_j * 2^40), T = sum W, t = floor(floor(u * 2^24) * T / 2^24), and the token is the
+ * first j whose running sum of W exceeds t.  The sums are 64-bit integers, so the result does not
+ * depend on the order of summation.  If T = 0 the weights are p_a's alone; if that is 0 too the
+ * token is 0.  q NULL: each q_i is 1 at the drafted token (greedy or looked-up drafts). */
+typedef struct llmdot_verify {
+    int32_t batch;
+    int32_t drafts; /* k: drafted tokens per sequence, 0..64 */
+    int32_t vocab;  /* at most 4194304 */
+    int32_t reserved;
+    const float *p;         /* [batch][drafts + 1][vocab], ld_p floats between rows */
+    const float *q;         /* [batch][drafts][vocab], ld_q floats between rows; nullable */
+    int64_t ld_p, ld_q;
+    const int32_t *draft;   /* [batch][drafts] */
+    const float *uniform;   /* [batch][drafts + 1], in [0, 1) */
+    const int32_t *n_draft; /* [batch], 0..drafts each; NULL = drafts for all */
+    int32_t *tokens;        /* out [batch][drafts + 1]: the accepted drafts, the next token, then -1 */
+    int32_t *accepted;      /* out [batch] */
+} llmdot_verify;
+LLMDOT_API int llmdot_cuda_verify_draft(const llmdot_verify *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,127 @@
+"""Argument checks of the serving operators' C entry points: refused before anything touches a device
+(no GPU needed; nothing is launched)."""
+import ctypes as C
+import subprocess
+
+import pytest
+
+from dotllm_b200 import native
+
+INVALID, UNSUPPORTED = -1, -2
+P = 1 << 12  # a non-null, aligned address that is never followed
+
+
+def pool(**kw):
+    d = dict(format=0, head_dim=64, heads_kv=2, n_pages=4, k=P, v=P, k_scale=P, v_scale=P)
+    d.update(kw)
+    return native.KvqPool(**d)
+
+
+def batch(**kw):
+    d = dict(batch=1, rows=1, max_rows=1, max_pages=1, row_start=P, seq_len=P, pages=P)
+    d.update(kw)
+    return native.KvqBatch(**d)
+
+
+def attn(**kw):
+    d = dict(heads=4, type=1, prefix_len=0, window=0, scale=0.125, softcap=0.0, prefix_pages=None)
+    d.update(kw)
+    return native.KvqAttn(**d)
+
+
+def message():
+    return native.lib().llmdot_cuda_last_error().decode()
+
+
+BAD_POOLS = [(dict(format=2), INVALID), (dict(head_dim=80), UNSUPPORTED), (dict(heads_kv=0), INVALID), (dict(n_pages=-1), INVALID),
+             (dict(k=None), INVALID), (dict(v_scale=None), INVALID), (dict(k=P + 8), INVALID), (dict(k_scale=P + 2), INVALID)]
+BAD_BATCHES = [dict(batch=-1), dict(rows=-1), dict(max_rows=-1), dict(max_pages=-1), dict(max_pages=1 << 25), dict(row_start=None),
+               dict(seq_len=None), dict(pages=None), dict(batch=0)]
+
+
+def test_pool_and_batch_refusals():
+    L = native.lib()
+    need = C.c_size_t()
+    calls = [lambda p, b: L.llmdot_cuda_kvq_write(p, b, P, P, 1, 128, 128, None),
+             lambda p, b: L.llmdot_cuda_kvq_read(p, b, P, P, 1, 128, 128, None),
+             lambda p, b: L.llmdot_cuda_kvq_attention_workspace(p, b, attn(), need),
+             lambda p, b: L.llmdot_cuda_kvq_attention(p, b, attn(), P, 256, P, 256, None, None, 0, None)]
+    for call in calls:
+        assert call(None, batch()) == INVALID and call(pool(), None) == INVALID
+        for kw, status in BAD_POOLS:
+            assert call(pool(**kw), batch()) == status, kw
+            assert message().startswith("kvq_")
+        for kw in BAD_BATCHES:
+            assert call(pool(), batch(**kw)) == INVALID, kw
+
+
+def test_row_refusals():
+    L = native.lib()
+    for call in (L.llmdot_cuda_kvq_write, L.llmdot_cuda_kvq_read):
+        p, b = pool(), batch(rows=3)
+        assert call(p, b, P, P, 12, 128, 128, None) == UNSUPPORTED          # a quantised ggml type
+        assert call(p, b, None, P, 1, 128, 128, None) == INVALID
+        assert call(p, b, P, P, 1, 127, 128, None) == INVALID               # rows overlap
+        assert call(p, b, P + 1, P, 1, 128, 128, None) == INVALID           # not aligned to fp16
+        assert call(p, batch(rows=0), None, None, 1, 0, 0, None) == 0       # nothing to do
+
+
+def test_attention_refusals():
+    L = native.lib()
+    need = C.c_size_t()
+    for kw, status in [(dict(type=8), UNSUPPORTED), (dict(heads=3), INVALID), (dict(heads=0), INVALID), (dict(prefix_len=-1), INVALID),
+                       (dict(prefix_len=64), INVALID), (dict(window=-1), INVALID), (dict(scale=float("nan")), INVALID),
+                       (dict(softcap=-1.0), INVALID), (dict(softcap=float("inf")), INVALID)]:
+        assert L.llmdot_cuda_kvq_attention_workspace(pool(), batch(), attn(**kw), need) == status, kw
+        assert L.llmdot_cuda_kvq_attention(pool(), batch(), attn(**kw), P, 256, P, 256, None, P, 1 << 30, None) == status, kw
+    b = batch(rows=2)
+    assert L.llmdot_cuda_kvq_attention(pool(), b, attn(), None, 256, P, 256, None, P, 1 << 30, None) == INVALID
+    assert L.llmdot_cuda_kvq_attention(pool(), b, attn(), P, 255, P, 256, None, P, 1 << 30, None) == INVALID
+    assert L.llmdot_cuda_kvq_attention(pool(), b, attn(), P + 1, 256, P, 256, None, P, 1 << 30, None) == INVALID
+    assert L.llmdot_cuda_kvq_attention_workspace(pool(), b, attn(), None) == INVALID
+    assert L.llmdot_cuda_kvq_attention(pool(), batch(rows=0), attn(), None, 0, None, 0, None, None, 0, None) == 0
+
+
+def test_verify_refusals():
+    L = native.lib()
+
+    def args(**kw):
+        d = dict(batch=1, drafts=2, vocab=100, p=P, q=P, ld_p=100, ld_q=100, draft=P, uniform=P, n_draft=None, tokens=P, accepted=P)
+        d.update(kw)
+        return native.Verify(**d)
+
+    assert L.llmdot_cuda_verify_draft(None, None) == INVALID
+    for kw, status in [(dict(batch=-1), INVALID), (dict(drafts=-1), INVALID), (dict(vocab=0), INVALID), (dict(drafts=65), UNSUPPORTED),
+                       (dict(vocab=(1 << 22) + 1, ld_p=1 << 23, ld_q=1 << 23), UNSUPPORTED), (dict(p=None), INVALID),
+                       (dict(draft=None), INVALID), (dict(uniform=None), INVALID), (dict(tokens=None), INVALID),
+                       (dict(accepted=None), INVALID), (dict(ld_p=99), INVALID), (dict(ld_q=99), INVALID), (dict(p=P + 2), INVALID)]:
+        assert L.llmdot_cuda_verify_draft(args(**kw), None) == status, kw
+        assert message().startswith("verify_draft")
+    assert L.llmdot_cuda_verify_draft(args(batch=0), None) == 0
+
+
+def test_structs_have_the_headers_layout(tmp_path):
+    names = [("llmdot_kvq_pool", native.KvqPool), ("llmdot_kvq_batch", native.KvqBatch), ("llmdot_kvq_attn", native.KvqAttn),
+             ("llmdot_verify", native.Verify)]
+    body = "".join(f'printf("%zu ", sizeof({n})); ' for n, _ in names)
+    body += "".join(f'printf("%zu ", offsetof({n}, {f[0]})); ' for n, s in names for f in s._fields_)
+    src = tmp_path / "layout.c"
+    src.write_text(f'#include "{native.HEADER}"\n#include <stdio.h>\nint main(void) {{ {body} return 0; }}\n')
+    subprocess.run(["gcc", "-std=c99", str(src), "-o", str(tmp_path / "layout")], check=True)
+    got = list(map(int, subprocess.run([str(tmp_path / "layout")], capture_output=True, text=True).stdout.split()))
+    want = [C.sizeof(s) for _, s in names] + [getattr(s, f[0]).offset for _, s in names for f in s._fields_]
+    assert got == want
+
+
+def test_serving_refuses_host_tensors():
+    import torch
+
+    from dotllm_b200 import serving
+    k = torch.zeros(2, 2, 64, 64, dtype=torch.int8)
+    s = torch.zeros(2, 2, 64)
+    with pytest.raises(ValueError):
+        serving.KvqPool(k, k, s, s)
+    with pytest.raises(ValueError):
+        serving.KvqBatch(torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32), 1)
+    with pytest.raises(ValueError):
+        serving.verify_draft(torch.zeros(1, 1, 8), None, torch.zeros(1, 0, dtype=torch.int32), torch.zeros(1, 1))
