@@ -4,7 +4,8 @@
 // (e4m3), every operation rounded to fp32 by itself, so the codes are a function of the inputs alone.  Bound: HBM (each input value read once, one byte written for it) for long
 // prompts, launch latency for a decode step.  A (row, head) item is held by a group of D / 8 lanes
 // (rounded up to a power of two), eight values per lane: one 16-byte load per lane for 16-bit
-// inputs, one 8-byte store of codes, the maximum by shuffles inside the group.
+// inputs, one 8-byte store of codes, the maximum by shuffles inside the group.  A group takes K and V
+// of two items, so a lane has four loads in flight while the rows' places are looked up.
 #include "kvq.cuh"
 
 namespace llmdot {
@@ -34,52 +35,85 @@ namespace {
 
 // Lanes per (row, head): D / 8, rounded up to a power of two (96 leaves 4 of 16 idle).
 template <int D> constexpr int kvq_lanes() { return D == 64 ? 8 : D == 256 ? 32 : 16; }
-constexpr int KVQ_THREADS = 256;
+constexpr int KVQ_THREADS = 256, KVQ_EACH = 2;
+template <int D> constexpr int kvq_items() { return KVQ_THREADS / kvq_lanes<D>() * KVQ_EACH; }
 
-// blockIdx.y: 0 = K, 1 = V.
+// Where a block's rows lie: for each row of the block's items the pool row of (page, head 0, slot), or -1.
+// One thread per row, so that the chain of dependent loads (row -> sequence -> length, page) is walked
+// once per row and not once per head, and while the values are already on their way.
+template <int D> __device__ __forceinline__ void kvq_find(const llmdot_kvq_pool &pool, const llmdot_kvq_batch &bt, int64_t item0,
+                                                          int64_t (&place)[kvq_items<D>()])
+{
+    const int r = (int)(item0 / pool.heads_kv) + threadIdx.x;
+    if (threadIdx.x < kvq_items<D>() && r < bt.rows) {
+        const int b = kvq_seq_of(bt.row_start, bt.batch, r);
+        place[threadIdx.x] = b < 0 ? -2 : kvq_place(pool, bt, b, bt.seq_len[b] - bt.row_start[b + 1] + r, 0);
+    }
+}
+
 template <typename T, int D, int FMT>
 __global__ void __launch_bounds__(KVQ_THREADS)
 kvq_write_kernel(const llmdot_kvq_pool pool, const llmdot_kvq_batch bt, const T *__restrict__ xk,
                  const T *__restrict__ xv, int64_t ldk, int64_t ldv, int wide)
 {
-    constexpr int L = kvq_lanes<D>();
-    const int64_t item = ((int64_t)blockIdx.x * KVQ_THREADS + threadIdx.x) / L;
-    const int lane = threadIdx.x % L;
-    if (item >= (int64_t)bt.rows * pool.heads_kv) return;  // whole groups leave together
-    const int r = (int)(item / pool.heads_kv), h = (int)(item % pool.heads_kv);
-    const bool v = blockIdx.y != 0, on = lane * 8 < D;
-    const T *x = (v ? xv + r * ldv : xk + r * ldk) + h * D + lane * 8;
-    float f[8] = {};
-    if (on) load8(x, wide != 0, f);
-    float a = 0.0f;
-    bool fine = true;
+    constexpr int L = kvq_lanes<D>(), GR = KVQ_THREADS / L, N = kvq_items<D>();
+    // the rows of N consecutive items are at most N (an item more can begin another row only if heads_kv > 1)
+    __shared__ int64_t s_place[N];
+    const int64_t item0 = (int64_t)blockIdx.x * N, items = (int64_t)bt.rows * pool.heads_kv;
+    const int lane = threadIdx.x % L, grp = threadIdx.x / L, row0 = (int)(item0 / pool.heads_kv);
+    const bool on = lane * 8 < D;
+    float f[KVQ_EACH][2][8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        a = fmaxf(a, fabsf(f[i]));
-        fine = fine && fabsf(f[i]) < INFINITY;
+    for (int i = 0; i < KVQ_EACH; i++) {
+        const int64_t item = item0 + i * GR + grp;
+#pragma unroll
+        for (int v = 0; v < 2; v++) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[i][v][e] = 0.0f;
+            if (item < items && on) {
+                const int r = (int)(item / pool.heads_kv), h = (int)(item % pool.heads_kv);
+                load8((v ? xv + r * ldv : xk + r * ldk) + h * D + lane * 8, wide != 0, f[i][v]);
+            }
+        }
     }
-    // lanes of one group are neighbours; the mask names them, as groups of a warp may have left
-    const unsigned mask = L == 32 ? 0xffffffffu : ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1));
+    kvq_find<D>(pool, bt, item0, s_place);
+    __syncthreads();
+    // lanes of one group are neighbours
+    const unsigned mask = L == 32 ? 0xffffffffu : ((1u << (L & 31)) - 1u) << (threadIdx.x & 31 & ~(L - 1));
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(mask, a, o));
-    fine = __all_sync(mask, fine);
-    const int b = kvq_seq_of(bt.row_start, bt.batch, r);
-    if (b < 0) return;
-    const int64_t at = kvq_place(pool, bt, b, bt.seq_len[b] - bt.row_start[b + 1] + r, h);
-    if (at < 0) return;
-    constexpr float M = FMT == LLMDOT_KVQ_I8 ? 127.0f : 448.0f;
-    const bool some = fine && a >= 1e-30f;
-    if (lane == 0) (v ? pool.v_scale : pool.k_scale)[at] = some ? __fdiv_rn(a, M) : fine ? 0.0f : NAN;
-    if (!on) return;
-    const float inv = some ? __fmul_rn(M, __frcp_rn(a)) : 0.0f;
-    __align__(8) uint8_t c[8];
+    for (int i = 0; i < KVQ_EACH; i++) {
+        const int64_t item = item0 + i * GR + grp;
+        if (item >= items) break;  // a whole group alike
+        const int64_t at0 = s_place[(int)(item / pool.heads_kv) - row0];
+        const int64_t at = at0 + item % pool.heads_kv * KVQ_PAGE;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float y = some ? fminf(fmaxf(__fmul_rn(f[i], inv), -M), M) : 0.0f;
-        if (FMT == LLMDOT_KVQ_I8) c[i] = (uint8_t)(int8_t)__float2int_rn(y);
-        else c[i] = __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+        for (int v = 0; v < 2; v++) {
+            float a = 0.0f;
+            bool fine = true;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                a = fmaxf(a, fabsf(f[i][v][e]));
+                fine = fine && fabsf(f[i][v][e]) < INFINITY;
+            }
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(mask, a, o));
+            fine = __all_sync(mask, fine);
+            if (at0 < 0) continue;
+            constexpr float M = FMT == LLMDOT_KVQ_I8 ? 127.0f : 448.0f;
+            const bool some = fine && a >= 1e-30f;
+            if (lane == 0) (v ? pool.v_scale : pool.k_scale)[at] = some ? __fdiv_rn(a, M) : fine ? 0.0f : NAN;
+            if (!on) continue;
+            const float inv = some ? __fmul_rn(M, __frcp_rn(a)) : 0.0f;
+            __align__(8) uint8_t c[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float y = some ? fminf(fmaxf(__fmul_rn(f[i][v][e], inv), -M), M) : 0.0f;
+                if (FMT == LLMDOT_KVQ_I8) c[e] = (uint8_t)(int8_t)__float2int_rn(y);
+                else c[e] = __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+            }
+            *(uint2 *)((uint8_t *)(v ? pool.v : pool.k) + at * D + lane * 8) = *(const uint2 *)c;
+        }
     }
-    *(uint2 *)((uint8_t *)(v ? pool.v : pool.k) + at * D + lane * 8) = *(const uint2 *)c;
 }
 
 template <typename T, int D, int FMT>
@@ -87,24 +121,46 @@ __global__ void __launch_bounds__(KVQ_THREADS)
 kvq_read_kernel(const llmdot_kvq_pool pool, const llmdot_kvq_batch bt, T *__restrict__ xk, T *__restrict__ xv,
                 int64_t ldk, int64_t ldv, int wide)
 {
-    constexpr int L = kvq_lanes<D>();
-    const int64_t item = ((int64_t)blockIdx.x * KVQ_THREADS + threadIdx.x) / L;
-    const int lane = threadIdx.x % L;
-    if (item >= (int64_t)bt.rows * pool.heads_kv || lane * 8 >= D) return;
-    const int r = (int)(item / pool.heads_kv), h = (int)(item % pool.heads_kv);
-    const bool v = blockIdx.y != 0;
-    const int b = kvq_seq_of(bt.row_start, bt.batch, r);
-    if (b < 0) return;
-    const int64_t at = kvq_place(pool, bt, b, bt.seq_len[b] - bt.row_start[b + 1] + r, h);
-    float f[8] = {};
-    if (at >= 0) {
-        __align__(8) uint8_t c[8];
-        *(uint2 *)c = __ldg((const uint2 *)((const uint8_t *)(v ? pool.v : pool.k) + at * D + lane * 8));
-        const float s = __ldg((v ? pool.v_scale : pool.k_scale) + at);
+    constexpr int L = kvq_lanes<D>(), GR = KVQ_THREADS / L, N = kvq_items<D>();
+    __shared__ int64_t s_place[N];
+    const int64_t item0 = (int64_t)blockIdx.x * N, items = (int64_t)bt.rows * pool.heads_kv;
+    const int lane = threadIdx.x % L, grp = threadIdx.x / L, row0 = (int)(item0 / pool.heads_kv);
+    kvq_find<D>(pool, bt, item0, s_place);
+    __syncthreads();
+    if (lane * 8 >= D) return;
+    uint2 c[KVQ_EACH][2];
+    float s[KVQ_EACH][2];
+    int64_t at0[KVQ_EACH];
 #pragma unroll
-        for (int i = 0; i < 8; i++) f[i] = __fmul_rn(code_value<FMT>(c[i]), s);
+    for (int i = 0; i < KVQ_EACH; i++) {
+        const int64_t item = item0 + i * GR + grp;
+        at0[i] = item < items ? s_place[(int)(item / pool.heads_kv) - row0] : -2;
+        const int64_t at = at0[i] + item % pool.heads_kv * KVQ_PAGE;
+#pragma unroll
+        for (int v = 0; v < 2; v++) {
+            c[i][v] = make_uint2(0, 0);
+            s[i][v] = 0.0f;
+            if (at0[i] >= 0) {
+                c[i][v] = __ldg((const uint2 *)((const uint8_t *)(v ? pool.v : pool.k) + at * D + lane * 8));
+                s[i][v] = __ldg((v ? pool.v_scale : pool.k_scale) + at);
+            }
+        }
     }
-    store8((v ? xv + r * ldv : xk + r * ldk) + h * D + lane * 8, wide != 0, f);
+#pragma unroll
+    for (int i = 0; i < KVQ_EACH; i++) {
+        if (at0[i] == -2) continue;  // no item, or a row of no sequence
+        const int64_t item = item0 + i * GR + grp;
+        const int r = (int)(item / pool.heads_kv), h = (int)(item % pool.heads_kv);
+#pragma unroll
+        for (int v = 0; v < 2; v++) {
+            __align__(8) uint8_t b[8];
+            *(uint2 *)b = c[i][v];
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] = at0[i] < 0 ? 0.0f : __fmul_rn(code_value<FMT>(b[e]), s[i][v]);
+            store8((v ? xv + r * ldv : xk + r * ldk) + h * D + lane * 8, wide != 0, f);
+        }
+    }
 }
 
 // The kernel instance for a type, head dimension and format.
@@ -130,16 +186,16 @@ cudaError_t dispatch(uint32_t type, int dim, int fmt, A... a)
 #undef LLMDOT_KVQ_D
 }
 
-dim3 kvq_grid(int64_t items, int lanes)
+template <int D> unsigned kvq_grid(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b)
 {
-    return dim3((unsigned)((items * lanes + KVQ_THREADS - 1) / KVQ_THREADS), 2);
+    return (unsigned)(((int64_t)b.rows * p.heads_kv + kvq_items<D>() - 1) / kvq_items<D>());
 }
 
 template <typename T, int D, int FMT> struct WriteOp {
     static cudaError_t launch(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const void *k, const void *v, int64_t ldk,
                               int64_t ldv, int wide, cudaStream_t st)
     {
-        kvq_write_kernel<T, D, FMT><<<kvq_grid((int64_t)b.rows * p.heads_kv, kvq_lanes<D>()), KVQ_THREADS, 0, st>>>(
+        kvq_write_kernel<T, D, FMT><<<kvq_grid<D>(p, b), KVQ_THREADS, 0, st>>>(
             p, b, (const T *)k, (const T *)v, ldk, ldv, wide);
         return cudaGetLastError();
     }
@@ -148,7 +204,7 @@ template <typename T, int D, int FMT> struct ReadOp {
     static cudaError_t launch(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, void *k, void *v, int64_t ldk, int64_t ldv,
                               int wide, cudaStream_t st)
     {
-        kvq_read_kernel<T, D, FMT><<<kvq_grid((int64_t)b.rows * p.heads_kv, kvq_lanes<D>()), KVQ_THREADS, 0, st>>>(
+        kvq_read_kernel<T, D, FMT><<<kvq_grid<D>(p, b), KVQ_THREADS, 0, st>>>(
             p, b, (T *)k, (T *)v, ldk, ldv, wide);
         return cudaGetLastError();
     }

@@ -20,6 +20,7 @@ from .native import check, lib
 PAGE = 64
 KVQ_I8, KVQ_E4M3 = 0, 1
 _FORMATS = {torch.int8: KVQ_I8, torch.float8_e4m3fn: KVQ_E4M3}
+_raw_stream = torch._C._cuda_getCurrentRawStream
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 25}
 
 
@@ -27,9 +28,9 @@ def _bad(text: str):
     raise ValueError(text)
 
 
-def _int32(name: str, t: torch.Tensor, shape: tuple, device) -> int:
-    if t.dtype is not torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
-        _bad(f"{name}: needs a contiguous int32 tensor of shape {shape} on {device}")
+def _int32(name: str, t: torch.Tensor, shape: tuple, device: int) -> int:
+    if t.dtype is not torch.int32 or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+        _bad(f"{name}: needs a contiguous int32 tensor of shape {shape} on cuda:{device}")
     return t.data_ptr()
 
 
@@ -37,24 +38,25 @@ class KvqPool:
     """Pages of 8-bit K and V: codes ``[n_pages, heads_kv, 64, head_dim]`` (int8 or float8_e4m3fn) and
     fp32 scales ``[n_pages, heads_kv, 64]``.  Holds the tensors; many batches share one pool."""
 
+    __slots__ = ("k", "v", "k_scale", "v_scale", "device", "n_pages", "heads_kv", "head_dim", "_c")
+
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
-        fmt, shape, device = _FORMATS.get(k.dtype), k.shape, k.device
+        fmt, shape, device = _FORMATS.get(k.dtype), k.shape, k.get_device()
         if fmt is None or v.dtype is not k.dtype:
             _bad("KvqPool: codes must be int8 or float8_e4m3fn, K and V alike")
         if len(shape) != 4 or shape[2] != PAGE or v.shape != shape:
             _bad("KvqPool: codes must be [n_pages, heads_kv, 64, head_dim], K and V alike")
+        self.n_pages, self.heads_kv, _, self.head_dim = shape
         if k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32 or k_scale.shape != shape[:3] \
                 or v_scale.shape != shape[:3]:
             _bad("KvqPool: scales must be float32 [n_pages, heads_kv, 64]")
-        if not (k.is_cuda and v.device == device and k_scale.device == device and v_scale.device == device):
+        if device < 0 or v.get_device() != device or k_scale.get_device() != device or v_scale.get_device() != device:
             _bad("KvqPool: all tensors must be on one CUDA device")
         if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
             _bad("KvqPool: tensors must be contiguous")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.device = device
-        self.n_pages, self.heads_kv, self.head_dim = shape[0], shape[1], shape[3]
-        self._c = native.KvqPool(fmt, shape[3], shape[1], shape[0], k.data_ptr(), v.data_ptr(), k_scale.data_ptr(),
-                                 v_scale.data_ptr())
+        self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, device
+        self._c = native.KvqPool(fmt, self.head_dim, self.heads_kv, self.n_pages, k.data_ptr(), v.data_ptr(),
+                                 k_scale.data_ptr(), v_scale.data_ptr())
 
     @classmethod
     def empty(cls, n_pages: int, heads_kv: int, head_dim: int, dtype: torch.dtype = torch.int8, device="cuda") -> "KvqPool":
@@ -70,40 +72,45 @@ class KvqBatch:
     ``seq_len[b]`` is its length, and rows ``row_start[b] .. row_start[b + 1]`` of a call are its last
     positions.  ``max_rows`` bounds the rows of any one sequence."""
 
+    __slots__ = ("row_start", "seq_len", "pages", "device", "max_rows", "_sizes", "_ptrs")
+
     def __init__(self, row_start: torch.Tensor, seq_len: torch.Tensor, pages: torch.Tensor, max_rows: int):
-        if pages.dim() != 2:
+        shape = pages.shape
+        if len(shape) != 2:
             _bad("KvqBatch: pages must be [batch, max_pages]")
-        B, most = pages.shape
-        device = pages.device
-        if not pages.is_cuda:
+        device = pages.get_device()
+        if device < 0:
             _bad("KvqBatch: tensors must be on a CUDA device")
         if max_rows < 0:
             _bad("KvqBatch: max_rows is negative")
-        self.row_start, self.seq_len, self.pages, self.device = row_start, seq_len, pages, device
-        self._c = native.KvqBatch(B, 0, max_rows, most, _int32("row_start", row_start, (B + 1,), device),
-                                  _int32("seq_len", seq_len, (B,), device), _int32("pages", pages, (B, most), device))
+        self.row_start, self.seq_len, self.pages, self.device, self.max_rows = row_start, seq_len, pages, device, max_rows
+        self._sizes = shape[0], shape[1]
+        self._ptrs = (_int32("row_start", row_start, (shape[0] + 1,), device), _int32("seq_len", seq_len, (shape[0],), device),
+                      _int32("pages", pages, shape, device))
+
+    def _c(self, rows: int) -> native.KvqBatch:
+        return native.KvqBatch(self._sizes[0], rows, self.max_rows, self._sizes[1], *self._ptrs)
 
 
-def _rows(name: str, t: torch.Tensor, heads: int, dim: int, device) -> int:
+def _rows(name: str, t: torch.Tensor, heads: int, dim: int, device: int) -> int:
     """ld of a [rows, heads, dim] tensor whose rows may be strided; its heads and values are dense."""
     s = t.shape
-    if len(s) != 3 or s[1] != heads or s[2] != dim or t.device != device:
-        _bad(f"{name}: needs [rows, {heads}, {dim}] on {device}")
-    st = t.stride()
-    if st[2] != 1 or (st[1] != dim and heads > 1) or (s[0] > 1 and st[0] < heads * dim):
+    if len(s) != 3 or s[1] != heads or s[2] != dim or t.get_device() != device:
+        _bad(f"{name}: needs [rows, {heads}, {dim}] on cuda:{device}")
+    ld, st_head, st_value = t.stride()
+    if st_value != 1 or (st_head != dim and heads > 1) or (ld < heads * dim and s[0] > 1):
         _bad(f"{name}: heads and values of a row must be dense and rows must not overlap")
-    return st[0]
+    return ld
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-class _On:
-    """The library launches on the current device: make it the tensors' one."""
-
-    def __new__(cls, device):
-        return torch.cuda.device(device)
+def _call(fn, device: int, *args) -> None:
+    """fn(*args, stream) on torch's current stream of the tensors' device, made the current device."""
+    stream = _raw_stream(device)
+    if torch.cuda.current_device() == device:
+        check(fn(*args, stream))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, stream))
 
 
 def kvq_write(pool: KvqPool, batch: KvqBatch, k: torch.Tensor, v: torch.Tensor) -> None:
@@ -115,10 +122,8 @@ def kvq_write(pool: KvqPool, batch: KvqBatch, k: torch.Tensor, v: torch.Tensor) 
         _bad("kvq_write: pool and batch are on different devices")
     ld_k = _rows("k", k, pool.heads_kv, pool.head_dim, pool.device)
     ld_v = _rows("v", v, pool.heads_kv, pool.head_dim, pool.device)
-    batch._c.rows = k.shape[0]
-    with _On(pool.device):
-        check(lib().llmdot_cuda_kvq_write(pool._c, batch._c, k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], ld_k, ld_v,
-                                          _stream(pool.device)))
+    _call(lib().llmdot_cuda_kvq_write, pool.device, pool._c, batch._c(k.shape[0]), k.data_ptr(), v.data_ptr(), _TYPES[k.dtype],
+          ld_k, ld_v)
 
 
 def kvq_read(pool: KvqPool, batch: KvqBatch, rows: int, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -127,13 +132,10 @@ def kvq_read(pool: KvqPool, batch: KvqBatch, rows: int, dtype: torch.dtype = tor
         _bad("kvq_read: dtype must be float32, float16 or bfloat16")
     if rows < 0 or batch.device != pool.device:
         _bad("kvq_read: negative rows, or pool and batch on different devices")
-    out = torch.empty((2, rows, pool.heads_kv, pool.head_dim), dtype=dtype, device=pool.device)
+    out = torch.empty((2, rows, pool.heads_kv, pool.head_dim), dtype=dtype, device=pool.k.device)
     ld = pool.heads_kv * pool.head_dim
-    batch._c.rows = rows
-    k, v = out[0], out[1]
-    with _On(pool.device):
-        check(lib().llmdot_cuda_kvq_read(pool._c, batch._c, k.data_ptr(), v.data_ptr(), _TYPES[dtype], ld, ld,
-                                         _stream(pool.device)))
+    k, v = out.unbind(0)
+    _call(lib().llmdot_cuda_kvq_read, pool.device, pool._c, batch._c(rows), k.data_ptr(), v.data_ptr(), _TYPES[dtype], ld, ld)
     return k, v
 
 
@@ -157,19 +159,19 @@ def kvq_attention(pool: KvqPool, batch: KvqBatch, q: torch.Tensor, prefix_pages:
             _bad("kvq_attention: prefix_len without prefix_pages")
         if prefix_pages.dim() != 1 or prefix_pages.shape[0] * PAGE < prefix_len:
             _bad("kvq_attention: prefix_pages holds fewer than prefix_len positions")
-        prefix = _int32("prefix_pages", prefix_pages, tuple(prefix_pages.shape), device)
+        prefix = _int32("prefix_pages", prefix_pages, prefix_pages.shape, device)
+    L, p, b = lib(), pool._c, batch._c(rows)
     a = native.KvqAttn(heads, _TYPES[q.dtype], prefix_len, window, pool.head_dim ** -0.5 if scale is None else scale, softcap,
                        prefix)
-    batch._c.rows = rows
-    out = torch.empty((rows, heads, pool.head_dim), dtype=q.dtype, device=device)
-    lse = torch.empty((rows, heads), dtype=torch.float32, device=device) if return_lse else None
     need = C.c_size_t()
-    check(lib().llmdot_cuda_kvq_attention_workspace(pool._c, batch._c, a, need))
-    work = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
-    with _On(device):
-        check(lib().llmdot_cuda_kvq_attention(pool._c, batch._c, a, q.data_ptr(), ld, out.data_ptr(), heads * pool.head_dim,
-                                              lse.data_ptr() if return_lse else None, work.data_ptr() if need.value else None,
-                                              need.value, _stream(device)))
+    check(L.llmdot_cuda_kvq_attention_workspace(p, b, a, need))
+    out = torch.empty((rows, heads, pool.head_dim), dtype=q.dtype, device=q.device)
+    lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    work, size = None, need.value
+    if size:
+        work = torch.empty(size, dtype=torch.uint8, device=q.device)
+    _call(L.llmdot_cuda_kvq_attention, device, p, b, a, q.data_ptr(), ld, out.data_ptr(), heads * pool.head_dim,
+          lse.data_ptr() if return_lse else None, work.data_ptr() if size else None, size)
     return (out, lse) if return_lse else out
 
 
@@ -184,16 +186,16 @@ def verify_draft(p: torch.Tensor, q: Optional[torch.Tensor], draft: torch.Tensor
     if p.dtype is not torch.float32 or p.dim() != 3 or not p.is_cuda:
         _bad("verify_draft: p must be a float32 CUDA tensor [batch, drafts + 1, vocab]")
     B, k1, V = p.shape
-    device, k = p.device, k1 - 1
+    device, k = p.get_device(), k1 - 1
     if k < 0:
         _bad("verify_draft: p holds no row")
 
     def ld(name, t, n):
-        st = t.stride()
-        if t.dtype is not torch.float32 or t.shape != (B, n, V) or t.device != device or (V > 1 and st[2] != 1) \
-                or (n > 0 and B > 1 and st[0] != n * st[1]) or (n > 1 and st[1] < V):
-            _bad(f"verify_draft: {name} must be float32 [{B}, {n}, {V}] on {device} with evenly strided rows")
-        return max(st[1], V)
+        s0, s1, s2 = t.stride()
+        if t.dtype is not torch.float32 or t.shape != (B, n, V) or t.get_device() != device or (s2 != 1 and V > 1) \
+                or (s0 != n * s1 and n > 0 and B > 1) or (s1 < V and n > 1):
+            _bad(f"verify_draft: {name} must be float32 [{B}, {n}, {V}] on cuda:{device} with evenly strided rows")
+        return max(s1, V)
 
     ld_p = ld("p", p, k1)
     if q is not None and k == 0:
@@ -201,14 +203,13 @@ def verify_draft(p: torch.Tensor, q: Optional[torch.Tensor], draft: torch.Tensor
             _bad(f"verify_draft: q must be [{B}, 0, {V}]")
         q = None  # no draft, nothing to subtract
     ld_q = ld("q", q, k) if q is not None else 0
-    if uniform.dtype is not torch.float32 or uniform.shape != (B, k1) or uniform.device != device or not uniform.is_contiguous():
-        _bad(f"verify_draft: uniform must be contiguous float32 [{B}, {k1}] on {device}")
-    tokens = torch.empty((B, k1), dtype=torch.int32, device=device)
-    accepted = torch.empty((B,), dtype=torch.int32, device=device)
-    a = native.Verify(B, k, V, 0, p.data_ptr(), q.data_ptr() if q is not None else None, ld_p, ld_q,
-                      _int32("draft", draft, (B, k), device), uniform.data_ptr(),
-                      _int32("n_draft", n_draft, (B,), device) if n_draft is not None else None, tokens.data_ptr(),
-                      accepted.data_ptr())
-    with _On(device):
-        check(lib().llmdot_cuda_verify_draft(a, _stream(device)))
+    if uniform.dtype is not torch.float32 or uniform.shape != (B, k1) or uniform.get_device() != device or not uniform.is_contiguous():
+        _bad(f"verify_draft: uniform must be contiguous float32 [{B}, {k1}] on cuda:{device}")
+    tokens = torch.empty((B, k1), dtype=torch.int32, device=p.device)
+    accepted = torch.empty((B,), dtype=torch.int32, device=p.device)
+    _call(lib().llmdot_cuda_verify_draft, device,
+          native.Verify(B, k, V, 0, p.data_ptr(), q.data_ptr() if q is not None else None, ld_p, ld_q,
+                        _int32("draft", draft, (B, k), device), uniform.data_ptr(),
+                        _int32("n_draft", n_draft, (B,), device) if n_draft is not None else None, tokens.data_ptr(),
+                        accepted.data_ptr()))
     return tokens, accepted
