@@ -5,7 +5,9 @@
 // prompts, launch latency for a decode step.  A (row, head) item is held by a group of D / 8 lanes
 // (rounded up to a power of two), eight values per lane: one 16-byte load per lane for 16-bit
 // inputs, one 8-byte store of codes, the maximum by shuffles inside the group.  A group takes K and V
-// of two items, so a lane has four loads in flight while the rows' places are looked up.
+// of one or two items, so a lane has up to four loads in flight while the rows' places are looked up.
+// Instructions come next to bytes: the maxima are taken on packed 16-bit pairs, and the two IEEE
+// divisions of an item are done by one lane per item.
 #include "kvq.cuh"
 
 namespace llmdot {
@@ -35,107 +37,196 @@ namespace {
 
 // Lanes per (row, head): D / 8, rounded up to a power of two (96 leaves 4 of 16 idle).
 template <int D> constexpr int kvq_lanes() { return D == 64 ? 8 : D == 256 ? 32 : 16; }
-constexpr int KVQ_THREADS = 256, KVQ_EACH = 2;
-template <int D> constexpr int kvq_items() { return KVQ_THREADS / kvq_lanes<D>() * KVQ_EACH; }
+constexpr int KVQ_THREADS = 256;
+template <int D, int EACH> constexpr int kvq_items() { return KVQ_THREADS / kvq_lanes<D>() * EACH; }
 
-// Where a block's rows lie: for each row of the block's items the pool row of (page, head 0, slot), or -1.
-// One thread per row, so that the chain of dependent loads (row -> sequence -> length, page) is walked
-// once per row and not once per head, and while the values are already on their way.
-template <int D> __device__ __forceinline__ void kvq_find(const llmdot_kvq_pool &pool, const llmdot_kvq_batch &bt, int64_t item0,
-                                                          int64_t (&place)[kvq_items<D>()])
+// Where a block's rows lie: for each row of the block's items the pool row of (page, head 0, slot), or -1
+// for no position, -2 for no sequence.  One thread per row, so that the chain of dependent loads (row ->
+// sequence -> length, page) is walked once per row and not once per head.
+template <int N> __device__ __forceinline__ void kvq_find(const llmdot_kvq_pool &pool, const llmdot_kvq_batch &bt, int row0,
+                                                          int64_t (&place)[N])
 {
-    const int r = (int)(item0 / pool.heads_kv) + threadIdx.x;
-    if (threadIdx.x < kvq_items<D>() && r < bt.rows) {
+    const int r = row0 + threadIdx.x;
+    if (threadIdx.x < N && r < bt.rows) {
         const int b = kvq_seq_of(bt.row_start, bt.batch, r);
         place[threadIdx.x] = b < 0 ? -2 : kvq_place(pool, bt, b, bt.seq_len[b] - bt.row_start[b + 1] + r, 0);
     }
 }
 
-template <typename T, int D, int FMT>
+// Maxima that a NaN survives: a row is finite when its maximum is.
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// Eight values of one lane as they were loaded, their largest magnitude, and as floats.
+template <typename T> struct Raw8;
+template <> struct Raw8<float> {
+    float x[8];
+    __device__ __forceinline__ float top() const
+    {
+        float a = fabsf(x[0]);
+#pragma unroll
+        for (int e = 1; e < 8; e++) a = max_nan(a, fabsf(x[e]));
+        return a;
+    }
+    __device__ __forceinline__ void floats(float (&f)[8]) const
+    {
+#pragma unroll
+        for (int e = 0; e < 8; e++) f[e] = x[e];
+    }
+};
+template <> struct Raw8<__half> {
+    __half2 x[4];
+    __device__ __forceinline__ float top() const
+    {
+        const __half2 m = __hmax2_nan(__hmax2_nan(__habs2(x[0]), __habs2(x[1])), __hmax2_nan(__habs2(x[2]), __habs2(x[3])));
+        return __half2float(__hmax_nan(__low2half(m), __high2half(m)));
+    }
+    __device__ __forceinline__ void floats(float (&f)[8]) const
+    {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float2 y = __half22float2(x[e]);
+            f[2 * e] = y.x;
+            f[2 * e + 1] = y.y;
+        }
+    }
+};
+template <> struct Raw8<__nv_bfloat16> {
+    __nv_bfloat162 x[4];
+    __device__ __forceinline__ float top() const
+    {
+        const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(__habs2(x[0]), __habs2(x[1])), __hmax2_nan(__habs2(x[2]), __habs2(x[3])));
+        return __bfloat162float(__hmax_nan(__low2bfloat16(m), __high2bfloat16(m)));
+    }
+    __device__ __forceinline__ void floats(float (&f)[8]) const
+    {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float2 y = __bfloat1622float2(x[e]);
+            f[2 * e] = y.x;
+            f[2 * e + 1] = y.y;
+        }
+    }
+};
+template <typename T> __device__ __forceinline__ void load_raw(Raw8<T> &r, const T *__restrict__ p, bool on, bool wide)
+{
+    if (!on) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) ((uint4 *)&r)[i] = make_uint4(0, 0, 0, 0);
+    } else if (wide) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) ((uint4 *)&r)[i] = __ldg((const uint4 *)p + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) ((T *)&r)[i] = p[i];
+    }
+}
+// Codes of eight values.  int8: adding 1.5 * 2^23 rounds to an integer (ties to even) that stands in the
+// low byte; |y| <= 127 (1 + 2^-22) rounds to at most 127.
+template <int FMT> __device__ __forceinline__ uint2 codes8(const float (&f)[8], float inv)
+{
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        if (FMT == LLMDOT_KVQ_I8) {
+            uint32_t y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = __float_as_uint(__fadd_rn(__fmul_rn(f[4 * i + e], inv), 12582912.0f));
+            w[i] = __byte_perm(__byte_perm(y[0], y[1], 0x0040), __byte_perm(y[2], y[3], 0x0040), 0x5410);
+        } else {
+            uint16_t h[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
+                    : "=h"(h[e])
+                    : "f"(__fmul_rn(f[4 * i + 2 * e + 1], inv)), "f"(__fmul_rn(f[4 * i + 2 * e], inv)));
+            w[i] = (uint32_t)h[0] | (uint32_t)h[1] << 16;
+        }
+    }
+    return make_uint2(w[0], w[1]);
+}
+
+template <typename T, int D, int FMT, int EACH>
 __global__ void __launch_bounds__(KVQ_THREADS)
 kvq_write_kernel(const llmdot_kvq_pool pool, const llmdot_kvq_batch bt, const T *__restrict__ xk,
                  const T *__restrict__ xv, int64_t ldk, int64_t ldv, int wide)
 {
-    constexpr int L = kvq_lanes<D>(), GR = KVQ_THREADS / L, N = kvq_items<D>();
-    // the rows of N consecutive items are at most N (an item more can begin another row only if heads_kv > 1)
-    __shared__ int64_t s_place[N];
-    const int64_t item0 = (int64_t)blockIdx.x * N, items = (int64_t)bt.rows * pool.heads_kv;
-    const int lane = threadIdx.x % L, grp = threadIdx.x / L, row0 = (int)(item0 / pool.heads_kv);
+    constexpr int L = kvq_lanes<D>(), GR = KVQ_THREADS / L, N = kvq_items<D, EACH>();
+    __shared__ int64_t s_place[N];  // N consecutive items are of at most N rows
+    const uint32_t Hk = pool.heads_kv, items = bt.rows * Hk, item0 = blockIdx.x * N, row0 = item0 / Hk;
+    const int lane = threadIdx.x % L, grp = threadIdx.x / L;
     const bool on = lane * 8 < D;
-    float f[KVQ_EACH][2][8];
+    Raw8<T> x[EACH][2];
+    uint32_t row[EACH], head[EACH];
 #pragma unroll
-    for (int i = 0; i < KVQ_EACH; i++) {
-        const int64_t item = item0 + i * GR + grp;
-#pragma unroll
-        for (int v = 0; v < 2; v++) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) f[i][v][e] = 0.0f;
-            if (item < items && on) {
-                const int r = (int)(item / pool.heads_kv), h = (int)(item % pool.heads_kv);
-                load8((v ? xv + r * ldv : xk + r * ldk) + h * D + lane * 8, wide != 0, f[i][v]);
-            }
-        }
+    for (int i = 0; i < EACH; i++) {
+        const uint32_t item = item0 + i * GR + grp;
+        row[i] = item / Hk;
+        head[i] = item - row[i] * Hk;
+        const int64_t o = head[i] * D + lane * 8;
+        load_raw(x[i][0], xk + row[i] * ldk + o, on && item < items, wide != 0);
+        load_raw(x[i][1], xv + row[i] * ldv + o, on && item < items, wide != 0);
     }
-    kvq_find<D>(pool, bt, item0, s_place);
-    __syncthreads();
-    // lanes of one group are neighbours
-    const unsigned mask = L == 32 ? 0xffffffffu : ((1u << (L & 31)) - 1u) << (threadIdx.x & 31 & ~(L - 1));
+    kvq_find(pool, bt, (int)row0, s_place);
+    constexpr float M = FMT == LLMDOT_KVQ_I8 ? 127.0f : 448.0f;
+    // the groups' maxima; lane c of a group then divides for combination c (item, K or V)
+    float mine = 0.0f;
 #pragma unroll
-    for (int i = 0; i < KVQ_EACH; i++) {
-        const int64_t item = item0 + i * GR + grp;
-        if (item >= items) break;  // a whole group alike
-        const int64_t at0 = s_place[(int)(item / pool.heads_kv) - row0];
-        const int64_t at = at0 + item % pool.heads_kv * KVQ_PAGE;
+    for (int c = 0; c < 2 * EACH; c++) {
+        float a = x[c >> 1][c & 1].top();
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+        if (lane == c) mine = a;
+    }
+    const bool fine = mine < INFINITY, some = fine && mine >= 1e-30f;
+    const float scale = some ? __fdiv_rn(mine, M) : fine ? 0.0f : NAN;
+    const float inv_mine = some ? __fmul_rn(M, __frcp_rn(mine)) : 0.0f;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+        const bool real = item0 + i * GR + grp < items;
+        const int64_t at0 = real ? s_place[row[i] - row0] : -2, at = at0 + (int64_t)head[i] * KVQ_PAGE;
 #pragma unroll
         for (int v = 0; v < 2; v++) {
-            float a = 0.0f;
-            bool fine = true;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                a = fmaxf(a, fabsf(f[i][v][e]));
-                fine = fine && fabsf(f[i][v][e]) < INFINITY;
-            }
-#pragma unroll
-            for (int o = L / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(mask, a, o));
-            fine = __all_sync(mask, fine);
+            const float inv = __shfl_sync(0xffffffffu, inv_mine, 2 * i + v, L);
             if (at0 < 0) continue;
-            constexpr float M = FMT == LLMDOT_KVQ_I8 ? 127.0f : 448.0f;
-            const bool some = fine && a >= 1e-30f;
-            if (lane == 0) (v ? pool.v_scale : pool.k_scale)[at] = some ? __fdiv_rn(a, M) : fine ? 0.0f : NAN;
+            if (lane == 2 * i + v) (v ? pool.v_scale : pool.k_scale)[at] = scale;
             if (!on) continue;
-            const float inv = some ? __fmul_rn(M, __frcp_rn(a)) : 0.0f;
-            __align__(8) uint8_t c[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float y = some ? fminf(fmaxf(__fmul_rn(f[i][v][e], inv), -M), M) : 0.0f;
-                if (FMT == LLMDOT_KVQ_I8) c[e] = (uint8_t)(int8_t)__float2int_rn(y);
-                else c[e] = __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
-            }
-            *(uint2 *)((uint8_t *)(v ? pool.v : pool.k) + at * D + lane * 8) = *(const uint2 *)c;
+            float f[8];
+            x[i][v].floats(f);
+            const uint2 w = inv == 0.0f ? make_uint2(0, 0) : codes8<FMT>(f, inv);
+            *(uint2 *)((uint8_t *)(v ? pool.v : pool.k) + at * D + lane * 8) = w;
         }
     }
 }
 
-template <typename T, int D, int FMT>
+template <typename T, int D, int FMT, int EACH>
 __global__ void __launch_bounds__(KVQ_THREADS)
 kvq_read_kernel(const llmdot_kvq_pool pool, const llmdot_kvq_batch bt, T *__restrict__ xk, T *__restrict__ xv,
                 int64_t ldk, int64_t ldv, int wide)
 {
-    constexpr int L = kvq_lanes<D>(), GR = KVQ_THREADS / L, N = kvq_items<D>();
+    constexpr int L = kvq_lanes<D>(), GR = KVQ_THREADS / L, N = kvq_items<D, EACH>();
     __shared__ int64_t s_place[N];
-    const int64_t item0 = (int64_t)blockIdx.x * N, items = (int64_t)bt.rows * pool.heads_kv;
-    const int lane = threadIdx.x % L, grp = threadIdx.x / L, row0 = (int)(item0 / pool.heads_kv);
-    kvq_find<D>(pool, bt, item0, s_place);
+    const uint32_t Hk = pool.heads_kv, items = bt.rows * Hk, item0 = blockIdx.x * N, row0 = item0 / Hk;
+    const int lane = threadIdx.x % L, grp = threadIdx.x / L;
+    kvq_find(pool, bt, (int)row0, s_place);
     __syncthreads();
     if (lane * 8 >= D) return;
-    uint2 c[KVQ_EACH][2];
-    float s[KVQ_EACH][2];
-    int64_t at0[KVQ_EACH];
+    uint2 c[EACH][2];
+    float s[EACH][2];
+    int64_t at0[EACH], o[EACH];
+    uint32_t row[EACH];
 #pragma unroll
-    for (int i = 0; i < KVQ_EACH; i++) {
-        const int64_t item = item0 + i * GR + grp;
-        at0[i] = item < items ? s_place[(int)(item / pool.heads_kv) - row0] : -2;
-        const int64_t at = at0[i] + item % pool.heads_kv * KVQ_PAGE;
+    for (int i = 0; i < EACH; i++) {
+        const uint32_t item = item0 + i * GR + grp;
+        row[i] = item / Hk;
+        const uint32_t head = item - row[i] * Hk;
+        o[i] = head * D + lane * 8;
+        at0[i] = item < items ? s_place[row[i] - row0] : -2;
+        const int64_t at = at0[i] + (int64_t)head * KVQ_PAGE;
 #pragma unroll
         for (int v = 0; v < 2; v++) {
             c[i][v] = make_uint2(0, 0);
@@ -147,10 +238,8 @@ kvq_read_kernel(const llmdot_kvq_pool pool, const llmdot_kvq_batch bt, T *__rest
         }
     }
 #pragma unroll
-    for (int i = 0; i < KVQ_EACH; i++) {
+    for (int i = 0; i < EACH; i++) {
         if (at0[i] == -2) continue;  // no item, or a row of no sequence
-        const int64_t item = item0 + i * GR + grp;
-        const int r = (int)(item / pool.heads_kv), h = (int)(item % pool.heads_kv);
 #pragma unroll
         for (int v = 0; v < 2; v++) {
             __align__(8) uint8_t b[8];
@@ -158,7 +247,7 @@ kvq_read_kernel(const llmdot_kvq_pool pool, const llmdot_kvq_batch bt, T *__rest
             float f[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) f[e] = at0[i] < 0 ? 0.0f : __fmul_rn(code_value<FMT>(b[e]), s[i][v]);
-            store8((v ? xv + r * ldv : xk + r * ldk) + h * D + lane * 8, wide != 0, f);
+            store8((v ? xv + row[i] * ldv : xk + row[i] * ldk) + o[i], wide != 0, f);
         }
     }
 }
@@ -186,17 +275,20 @@ cudaError_t dispatch(uint32_t type, int dim, int fmt, A... a)
 #undef LLMDOT_KVQ_D
 }
 
-template <int D> unsigned kvq_grid(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b)
-{
-    return (unsigned)(((int64_t)b.rows * p.heads_kv + kvq_items<D>() - 1) / kvq_items<D>());
-}
-
+// Two items per group once that still gives every SM a few blocks; one for small calls, where the
+// groups' work in sequence is the latency.
 template <typename T, int D, int FMT> struct WriteOp {
     static cudaError_t launch(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const void *k, const void *v, int64_t ldk,
                               int64_t ldv, int wide, cudaStream_t st)
     {
-        kvq_write_kernel<T, D, FMT><<<kvq_grid<D>(p, b), KVQ_THREADS, 0, st>>>(
-            p, b, (const T *)k, (const T *)v, ldk, ldv, wide);
+        const int64_t items = (int64_t)b.rows * p.heads_kv;
+        constexpr int N1 = kvq_items<D, 1>(), N2 = kvq_items<D, 2>();
+        if (items >= 148 * 4 * N2)
+            kvq_write_kernel<T, D, FMT, 2><<<(unsigned)((items + N2 - 1) / N2), KVQ_THREADS, 0, st>>>(p, b, (const T *)k, (const T *)v,
+                                                                                                      ldk, ldv, wide);
+        else
+            kvq_write_kernel<T, D, FMT, 1><<<(unsigned)((items + N1 - 1) / N1), KVQ_THREADS, 0, st>>>(p, b, (const T *)k, (const T *)v,
+                                                                                                      ldk, ldv, wide);
         return cudaGetLastError();
     }
 };
@@ -204,8 +296,12 @@ template <typename T, int D, int FMT> struct ReadOp {
     static cudaError_t launch(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, void *k, void *v, int64_t ldk, int64_t ldv,
                               int wide, cudaStream_t st)
     {
-        kvq_read_kernel<T, D, FMT><<<kvq_grid<D>(p, b), KVQ_THREADS, 0, st>>>(
-            p, b, (T *)k, (T *)v, ldk, ldv, wide);
+        const int64_t items = (int64_t)b.rows * p.heads_kv;
+        constexpr int N1 = kvq_items<D, 1>(), N2 = kvq_items<D, 2>();
+        if (items >= 148 * 4 * N2)
+            kvq_read_kernel<T, D, FMT, 2><<<(unsigned)((items + N2 - 1) / N2), KVQ_THREADS, 0, st>>>(p, b, (T *)k, (T *)v, ldk, ldv, wide);
+        else
+            kvq_read_kernel<T, D, FMT, 1><<<(unsigned)((items + N1 - 1) / N1), KVQ_THREADS, 0, st>>>(p, b, (T *)k, (T *)v, ldk, ldv, wide);
         return cudaGetLastError();
     }
 };
@@ -219,7 +315,7 @@ int check_rows(const char *who, const llmdot_kvq_pool *p, const llmdot_kvq_batch
     const int64_t row = (int64_t)p->heads_kv * p->head_dim;
     if (b->rows > 0 && (!k || !v)) return bad("null K or V rows");
     if (b->rows > 1 && (ldk < row || ldv < row)) return bad("row stride below heads_kv * head_dim");
-    if ((int64_t)b->rows * p->heads_kv > (int64_t)1 << 33) return bad("rows * heads_kv exceeds 2^33");
+    if ((int64_t)b->rows * p->heads_kv > (int64_t)1 << 31) return bad("rows * heads_kv exceeds 2^31");
     const int es = kvq_type_size(type);
     if (((uintptr_t)k | (uintptr_t)v) % es) return bad("K or V rows are not aligned to their type");
     *wide = (((uintptr_t)k | (uintptr_t)v) & 15) == 0 && (b->rows <= 1 || (ldk * es % 16 == 0 && ldv * es % 16 == 0));

@@ -234,10 +234,10 @@ __global__ void __launch_bounds__(NW * 32) kvq_attn_kernel(const __grid_constant
 
     // ---- rows: place, visible range [lo, hi] in the segment's positions, query as fp16
     if (tid < RT) {
-        const int64_t rho = row_first + tid;
+        const uint32_t rho = row_first + tid;  // rows * heads fits 2^30
         int row = -1, lo = 0, hi = 0x7fffffff;
-        if (rho < (int64_t)nrows * G) {
-            const int i = (int)(rho / G);
+        if (rho < (uint32_t)nrows * G) {
+            const int i = rho / (uint32_t)G;
             row = r0 + i;
             int64_t pos;  // relative to the first own position
             if (pre) {
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(NW * 32) kvq_attn_kernel(const __grid_constant
         float x[D / 32], mx = 0.0f;
 #pragma unroll
         for (int i = 0; i < D / 32; i++) {
-            x[i] = row < 0 ? 0.0f : load_any(a.q, row * a.ldq + (int64_t)(kvh * G + (row_first + n) % G) * D + i * 32 + lane, a.at.type);
+            x[i] = row < 0 ? 0.0f : load_any(a.q, row * a.ldq + (kvh * G + (row_first + n) % G) * D + i * 32 + lane, a.at.type);
             mx = fmaxf(mx, fabsf(x[i]));
         }
         mx = warp_max(mx);
@@ -611,7 +611,7 @@ template <int D> __global__ void __launch_bounds__(128) kvq_join_kernel(const __
     const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5), RH = (int64_t)a.bt.rows * a.at.heads;
     const int lane = threadIdx.x & 31;
     if (item >= RH) return;
-    const int row = (int)(item / a.at.heads), head = (int)(item % a.at.heads);
+    const int row = (uint32_t)item / (uint32_t)a.at.heads, head = (uint32_t)item - row * a.at.heads;
     const int b = kvq_seq_of(a.bt.row_start, a.bt.batch, row);
     int nown = 0;
     if (b >= 0) {
