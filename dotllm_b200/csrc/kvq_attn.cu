@@ -26,32 +26,12 @@
 // positions of 16 (4, 8) consecutive dimensions, which shuffle into A fragments by byte permutes.
 #include <algorithm>
 
-#include "kvq.cuh"
+#include "kvq_attn.cuh"
 
 namespace llmdot {
 namespace {
 
 constexpr int NW = 4;  // warps per CTA
-
-struct AttnArgs {
-    llmdot_kvq_pool pool;
-    llmdot_kvq_batch bt;
-    llmdot_kvq_attn at;
-    const void *q;
-    void *out;
-    int64_t ldq, ldo;
-    float *lse;
-    float *part_o;     // [slots][rows * heads][D]
-    float2 *part_ml;   // [slots][rows * heads]: maximum (base 2), sum
-    int group;         // query heads per kv head
-    int npp;           // pages of the prefix
-    int ch_p, ch_s;    // pages per chunk: prefix, own pages
-    int nsp, nss;      // chunks of the prefix; most chunks of a sequence
-    int ptiles, rtiles;
-    int prefix_ctas;
-    int direct;        // one slot: write the output itself
-    int wide;          // the output's rows are 16-byte aligned
-};
 
 __device__ __forceinline__ uint32_t su32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src)
@@ -64,25 +44,6 @@ __device__ __forceinline__ void cp4(uint32_t dst, const void *src)
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float rcp(float x)
-{
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// cap * tanh(s / cap).  16-bit activations: 1 - 2 / (1 + e^{2x}), a few 1e-7 of the cap off, which
-// the hardware's own tanh (2^-11) would not reach; fp32 ones: tanhf, exact to the last places of s.
-template <bool FULL> __device__ __forceinline__ float capped(float s, float cap, float inv_cap2)
-{
-    if (FULL) return cap * tanhf(s * (inv_cap2 * 0.34657359027997264f));
-    return cap - 2.0f * cap * rcp(1.0f + ex2(s * inv_cap2));
-}
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -95,30 +56,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a)
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
-__device__ __forceinline__ uint32_t pack(float lo, float hi)
-{
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b)
-{
-    uint32_t d;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-}
-
-// Two codes, bytes `lo` and `hi` of x, as an fp16 pair.  int8 (x with its sign bits flipped): the byte
-// under the exponent of 1024, minus 1152.  e4m3: sign, exponent and mantissa moved into fp16's places,
-// the value times 2^-8 (which the scale makes good), subnormals included.
-template <int FMT, int LO, int HI> __device__ __forceinline__ uint32_t codes2(uint32_t x)
-{
-    if (FMT == LLMDOT_KVQ_I8) return hsub2(__byte_perm(x, 0x64646464u, LO | 0x40 | (HI << 8) | 0x4000), 0x64806480u);
-    const uint32_t v = __byte_perm(x, 0u, 0x4 | (LO << 4) | 0x400 | (HI << 12));
-    return (v & 0x80008000u) | ((v >> 1) & 0x3F803F80u);
-}
-template <int FMT> constexpr uint32_t code_flip() { return FMT == LLMDOT_KVQ_I8 ? 0x80808080u : 0u; }
-template <int FMT> constexpr float code_unit() { return FMT == LLMDOT_KVQ_I8 ? 1.0f : 256.0f; }
-
 // Shapes of the kernel for a head dimension D and NT tiles of 8 rows.
 template <int D> struct Shape {
     static constexpr int LT = D == 256 ? 32 : 64;   // positions of one unit (slot)
@@ -161,12 +98,6 @@ template <int N> __device__ __forceinline__ void lds(const uint8_t *p, uint32_t 
     for (int i = 0; i < N / 4; i++) w[i] = x[i];
 }
 
-__device__ __forceinline__ float load_any(const void *p, int64_t i, uint32_t type)
-{
-    if (type == T_F32) return __ldg((const float *)p + i);
-    if (type == T_F16) return __half2float(__ldg((const __half *)p + i));
-    return __bfloat162float(__ldg((const __nv_bfloat16 *)p + i));
-}
 __device__ __forceinline__ void store4(void *p, int64_t i, uint32_t type, bool wide, const float (&x)[4])
 {
     if (type == T_F32) {
@@ -199,62 +130,18 @@ __global__ void __launch_bounds__(NW * 32) kvq_attn_kernel(const __grid_constant
     __shared__ int s_lo[RT], s_hi[RT], s_row[RT];
     __half *sq = (__half *)(smem + NW * Sh::WARP);  // [NQ][RT][QS]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int G = a.group, Hk = a.pool.heads_kv, P = a.at.prefix_len, win = a.at.window;
+    const int G = a.group, Hk = a.pool.heads_kv;
 
     pdl_launch();  // the joining kernel may be set up while this one runs
-    // ---- this CTA's segment
-    const bool pre = (int)blockIdx.x < a.prefix_ctas;
-    int rest = pre ? blockIdx.x : blockIdx.x - a.prefix_ctas;
-    const int kvh = rest % Hk;
-    rest /= Hk;
-    const int tiles = pre ? a.ptiles : a.rtiles, tile = rest % tiles;
-    rest /= tiles;
-    int chunk, b = 0, r0 = 0, nrows, own = 0, n_all = 0, len;
-    const int32_t *pages;
-    if (pre) {
-        chunk = rest;
-        nrows = a.bt.rows;
-        len = P;
-        pages = a.at.prefix_pages;
-    } else {
-        chunk = rest % a.nss;
-        b = rest / a.nss;
-        r0 = a.bt.row_start[b];
-        const int r1 = a.bt.row_start[b + 1];
-        n_all = r1 - r0;
-        nrows = min(min(n_all, a.bt.max_rows), a.bt.rows - r0);
-        own = a.bt.seq_len[b];
-        len = (int)min((int64_t)own, (int64_t)a.bt.max_pages * KVQ_PAGE);
-        pages = a.bt.pages + (int64_t)b * a.bt.max_pages;
-        if (r0 < 0) return;
+    Segment sg;
+    if (!segment_of(a, RT, sg)) {
+        if (a.chained) pdl_wait();
+        return;
     }
-    const int ch = pre ? a.ch_p : a.ch_s, row_first = tile * RT;
-    if ((int64_t)row_first >= (int64_t)nrows * G) return;
-    if (!a.direct && chunk * ch * KVQ_PAGE >= len) return;  // the joining kernel does not look for it
-
+    const int kvh = sg.kvh, chunk = sg.chunk, ch = sg.ch, len = sg.len, row_first = sg.tile * RT;
+    const int32_t *pages = sg.pages;
     // ---- rows: place, visible range [lo, hi] in the segment's positions, query as fp16
-    if (tid < RT) {
-        const uint32_t rho = row_first + tid;  // rows * heads fits 2^30
-        int row = -1, lo = 0, hi = 0x7fffffff;
-        if (rho < (uint32_t)nrows * G) {
-            const int i = rho / (uint32_t)G;
-            row = r0 + i;
-            int64_t pos;  // relative to the first own position
-            if (pre) {
-                const int sb = kvq_seq_of(a.bt.row_start, a.bt.batch, row);
-                pos = sb >= 0 ? (int64_t)a.bt.seq_len[sb] - a.bt.row_start[sb + 1] + row : -(int64_t)P - 1;
-                pos += P;
-            } else {
-                pos = (int64_t)own - n_all + i;
-            }
-            hi = (int)min(pos, (int64_t)len - 1);
-            if (pos < 0) hi = -1;
-            if (win > 0) lo = (int)max((int64_t)0, min(pos - win + 1, (int64_t)0x7fffffff));
-        }
-        s_row[tid] = row;
-        s_lo[tid] = lo;
-        s_hi[tid] = hi;
-    }
+    if (tid < RT) row_range(a, sg, row_first + tid, s_row[tid], s_lo[tid], s_hi[tid]);
     __syncthreads();
     for (int n = warp; n < RT; n += NW) {
         const int row = s_row[n];
@@ -265,9 +152,8 @@ __global__ void __launch_bounds__(NW * 32) kvq_attn_kernel(const __grid_constant
             mx = fmaxf(mx, fabsf(x[i]));
         }
         mx = warp_max(mx);
-        int e = 0;  // max |q| into [2^14, 2^15)
-        if (mx > 0.0f && mx < INFINITY) e = min(max(15 - (ilogbf(mx) + 1), -126), 126);
-        const float up = __int_as_float((e + 127) << 23);
+        const int e = row_exponent(mx);
+        const float up = pow2(e);
 #pragma unroll
         for (int i = 0; i < D / 32; i++) {
             const float y = x[i] * up;
@@ -278,7 +164,7 @@ __global__ void __launch_bounds__(NW * 32) kvq_attn_kernel(const __grid_constant
         // scores in base 2, or natural ones for the cap
         if (lane == 0)
             s_qf[n] = a.at.scale * code_unit<FMT>() * (a.at.softcap > 0.0f ? 1.0f : 1.4426950408889634f) *
-                      __int_as_float((127 - e) << 23);
+                      pow2(-e);
     }
     __syncthreads();
     // the tile's ranges (rows that do not exist see everything and are not written)
@@ -453,8 +339,7 @@ __global__ void __launch_bounds__(NW * 32) kvq_attn_kernel(const __grid_constant
                 }
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
-            const float vp = fmaxf(vpow, __int_as_float(min(__float_as_int(vmax), 0x7e800000) & 0x7f800000));
-            const float inv = __int_as_float(0x7f000000 - __float_as_int(vp)), ve = vpow * inv;
+            const float vp = fmaxf(vpow, scale_pow(vmax)), inv = pow_inverse(vp), ve = vpow * inv;
             vpow = vp;
             bool moved = ve != 1.0f;
             float f[NT][2], base[NT][2];
@@ -567,7 +452,7 @@ __global__ void __launch_bounds__(NW * 32) kvq_attn_kernel(const __grid_constant
                 so[(warp * PIECES + (nt * 2 + c) * (D / 32) + k) * 32 + lane] =
                     make_float4(o[nt][2 * k][c], o[nt][2 * k][2 + c], o[nt][2 * k + 1][c], o[nt][2 * k + 1][2 + c]);
     __syncthreads();
-    const int64_t RH = (int64_t)a.bt.rows * a.at.heads, slot = pre ? chunk : a.nsp + chunk;
+    const int64_t RH = (int64_t)a.bt.rows * a.at.heads, slot = sg.pre ? chunk : a.nsp + chunk;
     for (int pc = warp; pc < PIECES; pc += NW) {
         const int nc = pc / (D / 32), k = pc % (D / 32), n = (nc >> 1) * 8 + 2 * t + (nc & 1), row = s_row[n];
         if (row < 0) continue;
@@ -602,6 +487,7 @@ __global__ void __launch_bounds__(NW * 32) kvq_attn_kernel(const __grid_constant
             if (g == 0 && k == 0) a.part_ml[slot * RH + rh] = make_float2(M, L);
         }
     }
+    if (a.chained) pdl_wait();
 }
 
 // Joins a row's partials: one warp per (row, head); the prefix's chunks, then the sequence's.
@@ -667,8 +553,7 @@ template <int D, int FMT, int NT, bool SPLIT> cudaError_t launch_tiles(const Att
     static std::atomic<unsigned long long> done{0};
     cudaError_t e = smem_attr_once(done, kvq_attn_kernel<D, FMT, NT, SPLIT>, smem);
     if (e != cudaSuccess) return e;
-    kvq_attn_kernel<D, FMT, NT, SPLIT><<<(unsigned)grid, NW * 32, smem, st>>>(a);
-    return cudaGetLastError();
+    return launch_kernel(a.chained != 0, kvq_attn_kernel<D, FMT, NT, SPLIT>, dim3((unsigned)grid), dim3(NW * 32), smem, st, a);
 }
 template <int D, int FMT, bool SPLIT> cudaError_t launch_nt(int nt, const AttnArgs &a, int64_t grid, cudaStream_t st)
 {
@@ -680,51 +565,94 @@ template <int D, int FMT, bool SPLIT> cudaError_t launch_nt(int nt, const AttnAr
 }
 template <int D> cudaError_t launch_dim(int nt, const AttnArgs &a, int64_t grid, cudaStream_t st)
 {
-    cudaError_t e;
     const bool split = a.at.type == T_F32;
     if (a.pool.format == LLMDOT_KVQ_I8)
-        e = split ? launch_nt<D, LLMDOT_KVQ_I8, true>(nt, a, grid, st) : launch_nt<D, LLMDOT_KVQ_I8, false>(nt, a, grid, st);
-    else
-        e = split ? launch_nt<D, LLMDOT_KVQ_E4M3, true>(nt, a, grid, st) : launch_nt<D, LLMDOT_KVQ_E4M3, false>(nt, a, grid, st);
-    if (e != cudaSuccess || a.direct) return e;
-    const int64_t items = (int64_t)a.bt.rows * a.at.heads;
-    return launch_kernel(true, kvq_join_kernel<D>, dim3((unsigned)((items + 3) / 4)), dim3(128), 0, st, a);
+        return split ? launch_nt<D, LLMDOT_KVQ_I8, true>(nt, a, grid, st) : launch_nt<D, LLMDOT_KVQ_I8, false>(nt, a, grid, st);
+    return split ? launch_nt<D, LLMDOT_KVQ_E4M3, true>(nt, a, grid, st) : launch_nt<D, LLMDOT_KVQ_E4M3, false>(nt, a, grid, st);
+}
+cudaError_t launch_narrow(int nt, const AttnArgs &a, int64_t grid, cudaStream_t st)
+{
+    switch (a.pool.head_dim) {
+    case 64: return launch_dim<64>(nt, a, grid, st);
+    case 96: return launch_dim<96>(nt, a, grid, st);
+    case 128: return launch_dim<128>(nt, a, grid, st);
+    default: return launch_dim<256>(nt, a, grid, st);
+    }
+}
+cudaError_t launch_join(const AttnArgs &a, cudaStream_t st)
+{
+    const dim3 grid((unsigned)(((int64_t)a.bt.rows * a.at.heads + 3) / 4)), block(128);
+    switch (a.pool.head_dim) {
+    case 64: return launch_kernel(true, kvq_join_kernel<64>, grid, block, 0, st, a);
+    case 96: return launch_kernel(true, kvq_join_kernel<96>, grid, block, 0, st, a);
+    case 128: return launch_kernel(true, kvq_join_kernel<128>, grid, block, 0, st, a);
+    default: return launch_kernel(true, kvq_join_kernel<256>, grid, block, 0, st, a);
+    }
 }
 
-// How a call is cut: row tiles of 8 * nt rows, chunks of pages.  From the sizes the host knows; lengths on
-// the device only decide which CTAs find nothing to do.
+// How a call is cut.  From the sizes the host knows; lengths on the device only decide which CTAs find
+// nothing to do.
 struct Plan {
-    int nt, npp, ch_p, ch_s, nsp, nss, ptiles, rtiles, direct;
-    int64_t prefix_ctas, grid;
+    int wide_p, wide_s;  // the segment kind goes to the wide kernel
+    int nt_p, nt_s;      // 8-row tiles of the narrow kernel
+    int ch_p, ch_s, nsp, nss, ptiles, rtiles, direct;
+    int64_t ctas_p, ctas_s;
     size_t o_bytes, ml_bytes;
 };
 int max_nt(int dim) { return dim == 256 ? 2 : dim == 128 ? 3 : 4; }
+// From this many rows (times heads) per kv head a segment is worth the wide kernel.
+constexpr int64_t WIDE_FROM = 48;
 
 Plan make_plan(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const llmdot_kvq_attn &a)
 {
     Plan x = {};
-    const int64_t G = a.heads / p.heads_kv, own_rows = (int64_t)b.max_rows * G, all_rows = (int64_t)b.rows * G;
-    x.npp = (a.prefix_len + KVQ_PAGE - 1) / KVQ_PAGE;
-    const int64_t most = x.npp > 0 && all_rows > own_rows ? all_rows : own_rows;
-    x.nt = (int)std::min<int64_t>(max_nt(p.head_dim), std::max<int64_t>(1, (most + 7) / 8));
-    x.ptiles = (int)((all_rows + 8 * x.nt - 1) / (8 * x.nt));
-    x.rtiles = (int)std::max<int64_t>(1, (own_rows + 8 * x.nt - 1) / (8 * x.nt));
-    // chunks: enough CTAs to fill the SMs about four times (ragged sequences leave some without work),
-    // at least one page per warp, at most 32 pages, so that long and short sequences balance
-    const int64_t pages = p.heads_kv * ((int64_t)x.ptiles * x.npp + (int64_t)b.batch * x.rtiles * b.max_pages);
-    const int64_t ch = std::min<int64_t>(32, std::max<int64_t>(NW, (pages / (148 * 4) + NW - 1) / NW * NW));
-    x.ch_p = x.ch_s = (int)ch;
-    x.nsp = (int)((x.npp + ch - 1) / ch);
-    x.nss = (int)std::max<int64_t>(1, (b.max_pages + ch - 1) / ch);
-    x.direct = x.nsp == 0 && x.nss == 1;
-    x.prefix_ctas = (int64_t)p.heads_kv * x.ptiles * x.nsp;
-    x.grid = x.prefix_ctas + (int64_t)p.heads_kv * x.rtiles * x.nss * b.batch;
+    const int64_t G = a.heads / p.heads_kv, Hk = p.heads_kv, own_rows = (int64_t)b.max_rows * G, all_rows = (int64_t)b.rows * G;
+    const int64_t npp = (a.prefix_len + KVQ_PAGE - 1) / KVQ_PAGE, wide = kvq_wide_rows(p.head_dim);
+    auto nt_of = [&](int64_t rows) { return (int)std::min<int64_t>(max_nt(p.head_dim), std::max<int64_t>(1, (rows + 7) / 8)); };
+    auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+    x.wide_p = a.type != T_F32 && npp > 0 && all_rows >= WIDE_FROM;
+    x.wide_s = a.type != T_F32 && own_rows >= WIDE_FROM;
+    x.nt_p = nt_of(all_rows);
+    x.nt_s = nt_of(own_rows);
+    if (npp == 0) x.nt_p = x.nt_s;
+    x.ptiles = (int)up(all_rows, x.wide_p ? wide : 8 * x.nt_p);
+    x.rtiles = (int)std::max<int64_t>(1, up(own_rows, x.wide_s ? wide : 8 * x.nt_s));
+    // Chunks.  Narrow: enough CTAs to fill the SMs about four times (ragged sequences leave some without
+    // work), at least one page per warp, at most 32 pages, so that long and short sequences balance.
+    // Wide: one CTA per SM, at least four pages each.
+    const int64_t np = x.wide_p ? 0 : Hk * x.ptiles * npp, ns = x.wide_s ? 0 : Hk * b.batch * x.rtiles * b.max_pages;
+    const int64_t ch = std::min<int64_t>(32, std::max<int64_t>(NW, up(up(np + ns, 148 * 4), NW) * NW));
+    auto wide_ch = [&](int64_t ctas, int64_t pages) { return std::max<int64_t>(4, up(pages, std::max<int64_t>(1, 148 / std::max<int64_t>(1, ctas)))); };
+    x.ch_p = (int)(x.wide_p ? wide_ch(Hk * x.ptiles, npp) : ch);
+    x.ch_s = (int)(x.wide_s ? wide_ch(Hk * x.rtiles * b.batch, b.max_pages) : ch);
+    x.nsp = (int)up(npp, x.ch_p);
+    x.nss = (int)std::max<int64_t>(1, up(b.max_pages, x.ch_s));
+    x.direct = x.nsp == 0 && x.nss == 1 && !x.wide_s;
+    x.ctas_p = Hk * x.ptiles * x.nsp;
+    x.ctas_s = Hk * x.rtiles * x.nss * b.batch;
     if (!x.direct) {
         const size_t rh = (size_t)b.rows * a.heads * (x.nsp + x.nss);
         x.o_bytes = rh * p.head_dim * 4;
         x.ml_bytes = rh * 8;
     }
     return x;
+}
+
+// One to two kernels over the segments (the second over the first, which it outlives), then the join.
+cudaError_t run_plan(const Plan &x, AttnArgs &a, cudaStream_t st)
+{
+    cudaError_t e = cudaSuccess;
+    const bool together = !x.wide_p && !x.wide_s && x.nt_p == x.nt_s;
+    if (!together && x.ctas_p > 0) {
+        a.prefix_ctas = (int)x.ctas_p;
+        e = x.wide_p ? launch_kvq_wide(a, x.ctas_p, false, st) : launch_narrow(x.nt_p, a, x.ctas_p, st);
+        if (e != cudaSuccess) return e;
+        a.chained = 1;
+    }
+    a.prefix_ctas = together ? (int)x.ctas_p : 0;
+    e = x.wide_s ? launch_kvq_wide(a, x.ctas_s, a.chained != 0, st) : launch_narrow(x.nt_s, a, a.prefix_ctas + x.ctas_s, st);
+    if (e != cudaSuccess || x.direct) return e;
+    return launch_join(a, st);
 }
 
 int check_attn(const char *who, const llmdot_kvq_pool *p, const llmdot_kvq_batch *b, const llmdot_kvq_attn *a)
@@ -774,7 +702,7 @@ extern "C" int llmdot_cuda_kvq_attention(const llmdot_kvq_pool *pool, const llmd
         const Plan x = make_plan(*pool, *batch, *attn);
         if (x.o_bytes + x.ml_bytes > 0 && (!d_work || work_bytes < x.o_bytes + x.ml_bytes || ((uintptr_t)d_work & 15)))
             return bad("workspace is null, too small or not 16-byte aligned");
-        if (x.grid > 0x7fffffff) return bad("too many sequences, rows or pages for one call");
+        if (x.ctas_p + x.ctas_s > 0x7fffffff) return bad("too many sequences, rows or pages for one call");
         AttnArgs a = {};
         a.pool = *pool;
         a.bt = *batch;
@@ -787,24 +715,15 @@ extern "C" int llmdot_cuda_kvq_attention(const llmdot_kvq_pool *pool, const llmd
         a.part_o = (float *)d_work;
         a.part_ml = (float2 *)((uint8_t *)d_work + x.o_bytes);
         a.group = attn->heads / pool->heads_kv;
-        a.npp = x.npp;
         a.ch_p = x.ch_p;
         a.ch_s = x.ch_s;
         a.nsp = x.nsp;
         a.nss = x.nss;
         a.ptiles = x.ptiles;
         a.rtiles = x.rtiles;
-        a.prefix_ctas = (int)x.prefix_ctas;
         a.direct = x.direct;
         a.wide = ((uintptr_t)d_out & 15) == 0 && (batch->rows <= 1 || ld_out * es % 16 == 0);
-        const cudaStream_t st = (cudaStream_t)stream;
-        cudaError_t e;
-        switch (pool->head_dim) {
-        case 64: e = launch_dim<64>(x.nt, a, x.grid, st); break;
-        case 96: e = launch_dim<96>(x.nt, a, x.grid, st); break;
-        case 128: e = launch_dim<128>(x.nt, a, x.grid, st); break;
-        default: e = launch_dim<256>(x.nt, a, x.grid, st); break;
-        }
+        const cudaError_t e = run_plan(x, a, (cudaStream_t)stream);
         if (e != cudaSuccess) return cuda_fail(e, "kvq_attention");
         return LLMDOT_OK;
     });
