@@ -141,7 +141,8 @@ __global__ void __launch_bounds__(NW * 32) kvq_attn_kernel(const __grid_constant
     const int kvh = sg.kvh, chunk = sg.chunk, ch = sg.ch, len = sg.len, row_first = sg.tile * RT;
     const int32_t *pages = sg.pages;
     // ---- rows: place, visible range [lo, hi] in the segment's positions, query as fp16
-    if (tid < RT) row_range(a, sg, row_first + tid, s_row[tid], s_lo[tid], s_hi[tid]);
+    const SeqTable seqs = load_seqs(a, sg, (int32_t *)smem, NW * 32);  // (the slots' memory, not in use yet)
+    if (tid < RT) row_range(a, sg, seqs, row_first + tid, s_row[tid], s_lo[tid], s_hi[tid]);
     __syncthreads();
     for (int n = warp; n < RT; n += NW) {
         const int row = s_row[n];
@@ -548,6 +549,7 @@ template <int D> __global__ void __launch_bounds__(128) kvq_join_kernel(const __
 template <int D, int FMT, int NT, bool SPLIT> cudaError_t launch_tiles(const AttnArgs &a, int64_t grid, cudaStream_t st)
 {
     using Sh = Shape<D>;
+    static_assert(NW * Sh::WARP >= (2 * SEQ_TABLE + 1) * 4, "the sequences' tables fit into the slots");
     constexpr int smem = NW * Sh::WARP + (SPLIT ? 2 : 1) * NT * 8 * (D + Sh::QPAD) * 2;
     static_assert(NT * 8 * D * 4 <= Sh::WARP, "the warps' outputs fit into their slots");
     static std::atomic<unsigned long long> done{0};

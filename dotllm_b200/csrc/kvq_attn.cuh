@@ -74,9 +74,29 @@ __device__ __forceinline__ bool segment_of(const AttnArgs &a, int rows, Segment 
     // the joining kernel does not look for a chunk that begins behind the end
     return a.direct || s.chunk * s.ch * KVQ_PAGE < s.len;
 }
+// row_start and seq_len of the batch, in shared memory when they fit: a row's search for its sequence is
+// a chain of dependent loads, half a microsecond each from global memory.
+struct SeqTable {
+    const int32_t *row_start, *seq_len;
+};
+constexpr int SEQ_TABLE = 512;  // sequences
+// Called by all threads; `room`: 2 * SEQ_TABLE + 1 ints of shared memory.  The prefix's rows need it alone.
+__device__ __forceinline__ SeqTable load_seqs(const AttnArgs &a, const Segment &s, int32_t *room, int threads)
+{
+    SeqTable t = {a.bt.row_start, a.bt.seq_len};
+    if (!s.pre || a.bt.batch > SEQ_TABLE) return t;
+    for (int i = threadIdx.x; i <= a.bt.batch; i += threads) {
+        room[i] = a.bt.row_start[i];
+        if (i < a.bt.batch) room[SEQ_TABLE + 1 + i] = a.bt.seq_len[i];
+    }
+    __syncthreads();
+    t.row_start = room;
+    t.seq_len = room + SEQ_TABLE + 1;
+    return t;
+}
 // Row rho (of rows times the group's heads): its packed row (-1: none) and visible positions [lo, hi].
 // Rows that do not exist see everything, so that they hide nothing.
-__device__ __forceinline__ void row_range(const AttnArgs &a, const Segment &s, uint32_t rho, int &row, int &lo, int &hi)
+__device__ __forceinline__ void row_range(const AttnArgs &a, const Segment &s, const SeqTable &q, uint32_t rho, int &row, int &lo, int &hi)
 {
     row = -1;
     lo = 0;
@@ -86,8 +106,8 @@ __device__ __forceinline__ void row_range(const AttnArgs &a, const Segment &s, u
     row = s.r0 + i;
     int64_t pos = (int64_t)s.own - s.n_all + i;  // in the segment's positions
     if (s.pre) {
-        const int b = kvq_seq_of(a.bt.row_start, a.bt.batch, row);
-        pos = b >= 0 ? (int64_t)a.at.prefix_len + a.bt.seq_len[b] - a.bt.row_start[b + 1] + row : -1;
+        const int b = kvq_seq_of(q.row_start, a.bt.batch, row);
+        pos = b >= 0 ? (int64_t)a.at.prefix_len + q.seq_len[b] - q.row_start[b + 1] + row : -1;
     }
     hi = pos < 0 ? -1 : (int)min(pos, (int64_t)s.len - 1);
     if (win > 0) lo = (int)max((int64_t)0, min(pos - win + 1, (int64_t)0x7fffffff));

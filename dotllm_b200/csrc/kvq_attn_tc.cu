@@ -6,56 +6,59 @@
 // Bound: with hundreds of rows per kv head the products, the exponentials (16 per clock and SM) and
 // the conversion of codes to fp16 take about the same time, and HBM little.  So one CTA takes two tiles of
 // 128 rows (one for head_dim 256) over the same positions -- each code is converted once for 256 rows --
-// and its roles overlap, 64 positions (a page) at a time:
-//   warps of a tile (4 each)  a thread per row: S from TMEM, scale, mask, running maximum, exponentials,
-//                             the weights as fp16 back into TMEM over S; rescales O in TMEM only when
-//                             its maximum rose by more than 2^8 (fp16 holds weights up to 2^13)
-//   4 converting warps        codes from global memory (next page's loads in flight) to fp16 K and V^T
-//                             operands in shared memory (three stages), scales beside them
-//   1 warp                    one thread issues tcgen05.mma: S = Q K^T and O += P V with Q, P and the
+// and its roles overlap, 128 positions (two pages; one for head_dim 256) at a time:
+//   warps of a tile (4 each)  a thread per row: S from TMEM 32 columns at a time, weights as fp16 back into
+//                             TMEM over S.  One pass: the weights are taken relative to the maximum so
+//                             far, which may lag by 2^8 (fp16 holds them up to 2^13); when a row's scores
+//                             go above that, its sums, O in TMEM and this unit's earlier weights are
+//                             rescaled, which after the first positions is rare
+//   4 converting warps        codes from global memory (next page's loads in flight) to fp16 K and V
+//                             operands in shared memory, scales beside them
+//   1 warp                    one thread issues tcgen05.mma: S = Q K^T and O += P V with P and the
 //                             accumulators in TMEM; while one tile's rows are in their softmax, the other
-//                             tile's products run
-// Operands in shared memory are unswizzled K-major core matrices (8 rows x 16 bytes).  K: cores adjacent
-// along head_dim 128 bytes apart.  V is transposed on conversion (a lane holds eight positions of eight
-// dimensions and permutes bytes): cores adjacent along positions are 144 bytes apart, which spreads
-// the eight lanes that write one dimension's pieces over all banks.
+//                             tile's products run, and P V starts on the first 64 positions' weights
+// N = 128 in S = Q K^T: a product with N = 64 takes as long (measured 62 clocks and 65, 32 and 64 needed).
+// Operands in shared memory are rows of 64 values (128 bytes) of one position in 8-row groups, the
+// 16-byte pieces swizzled by the row (piece ^ row % 8), which spreads the converting lanes' stores over all
+// banks: K-major for Q and K, and the same layout read as N-major for V, which so needs no transposing.
+// Shared memory and L1 are one data path that the tensor core's operands already fill by half, so a warp
+// loads 512 consecutive bytes of codes at once (loads of 8 separate rows at a time held the whole kernel
+// at a third of this speed).
 // Every wait is bounded; one that gives up leaves NaN partials, so the output shows it.
+#include <type_traits>
+
 #include "kvq_attn.cuh"
 
 namespace llmdot {
 namespace {
 
-constexpr int UN = KVQ_PAGE;  // positions per unit
-constexpr int STAGES = 3;
-constexpr unsigned long long WAIT_NS = 2000000000ull;
+constexpr long long WAIT_CLOCKS = 4000000000ll;  // about two seconds
 constexpr float RAISE = 8.0f;  // the maximum may lag by this power of two
 
 template <int D> struct Wide {
     static constexpr int TILES = D == 256 ? 1 : 2;
+    static constexpr int UNP = D == 256 ? 1 : 2, UN = UNP * KVQ_PAGE;  // pages and positions of a unit
+    static constexpr int STAGES = D == 64 ? 3 : 2;
     static constexpr int THREADS = TILES * 128 + 128 + 32;
-    static constexpr uint32_t K_SBO = D / 8 * 128, V_LBO = 144, V_SBO = 8 * V_LBO;
-    static constexpr uint32_t K_BYTES = 8 * K_SBO, V_BYTES = D / 8 * V_SBO;
-    static constexpr uint32_t STAGE = K_BYTES + V_BYTES;
-    static constexpr uint32_t OFF_SC = STAGES * STAGE;  // per stage: K scales, V scales, {rescale, 2^E, bad, -}
+    static constexpr uint32_t ROW = 128, GROUP = 8 * ROW;  // bytes of an operand's row, of eight
+    static constexpr int KBLK = (D + 63) / 64;             // 64-wide blocks along the head dimension (Q, K)
+    static constexpr uint32_t Q_BLK = 128 * ROW, K_BLK = UN * ROW;
+    static constexpr uint32_t Q_BYTES = KBLK * Q_BLK, K_BYTES = KBLK * K_BLK;
+    static constexpr uint32_t STAGE = 2 * K_BYTES;  // K, then V alike
+    static constexpr uint32_t OFF_Q = STAGES * STAGE;
+    static constexpr uint32_t OFF_SC = OFF_Q + TILES * Q_BYTES;  // per stage: K scales, V scales, {rescale, 2^E, bad pages}
     static constexpr uint32_t SC_STAGE = 2 * UN * 4 + 16;
     static constexpr uint32_t OFF_BAR = OFF_SC + STAGES * SC_STAGE;
-    static constexpr int B_FULL = 0, B_EMPTY = STAGES, B_S = 2 * STAGES, B_P = B_S + 2, B_O = B_P + 2, B_DRAIN = B_O + 2,
-                         B_COUNT = B_DRAIN + 1;
-    static constexpr uint32_t SMEM = OFF_BAR + B_COUNT * 8 + 16;
-    static constexpr int QC = D / 2;  // TMEM columns of Q
-    static constexpr int TILE_COLS = (D + UN + QC + 31) / 32 * 32;
-    static constexpr int C_O = 0, C_S = D, C_Q = D + UN;
+    // barriers: a stage is converted, read; a tile's S, halves of P, of P V; the drain
+    static constexpr int B_FULL = 0, B_EMPTY = STAGES, B_S = 2 * STAGES, B_P = B_S + TILES, B_O = B_P + TILES * UNP,
+                         B_DRAIN = B_O + TILES * UNP, B_COUNT = B_DRAIN + 1;
+    static constexpr uint32_t SMEM = OFF_BAR + B_COUNT * 8 + 1024;  // and up to 1 KB to align the operands
+    static constexpr int TILE_COLS = D + UN, C_O = 0, C_S = D;  // TMEM columns
     static_assert(TILES * TILE_COLS <= 512, "TMEM columns");
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
 __device__ __forceinline__ uint32_t su32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ unsigned long long gtime()
-{
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
 __device__ __forceinline__ void bar_init(uint32_t b, uint32_t count)
 {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b), "r"(count) : "memory");
@@ -75,19 +78,28 @@ __device__ __forceinline__ bool bar_try(uint32_t b, uint32_t parity)
 }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-// shared-memory matrix descriptor: no swizzle, K-major cores; lbo: K-adjacent cores, sbo: 8-row groups
-__device__ __forceinline__ uint64_t sdesc(uint32_t addr, uint32_t lbo, uint32_t sbo)
+// shared-memory matrix descriptor: rows of 128 bytes, 128-byte swizzle, 8-row groups of 1024 bytes.  lbo: bytes
+// between blocks of 64 along N (N-major operands; K-major ones have a block per descriptor)
+__device__ __forceinline__ uint64_t sdesc(uint32_t addr, uint32_t lbo = 16)
 {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
-           ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46);
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
-// kind::f16, fp32 accumulator, fp16 A (TMEM) and B (shared memory), M = 128
+// kind::f16, fp32 accumulator, fp16 A (TMEM) and N-major B (shared memory), M = 128
 template <int N> __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t acc)
 {
-    constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+    constexpr uint32_t idesc = (1u << 4) | (1u << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
     asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
                  " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
                  "r"(a), "l"(b), "r"(idesc), "r"(acc)
+                 : "memory");
+}
+// both operands in shared memory
+template <int N> __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t acc)
+{
+    constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(acc)
                  : "memory");
 }
 __device__ __forceinline__ void umma_commit(uint32_t b)
@@ -105,6 +117,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t ta, uint32_t *v)
                    "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
                  : "r"(ta));
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t ta, uint32_t *v)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+                   "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(ta));
+}
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st16(uint32_t ta, const uint32_t *v)
 {
@@ -114,31 +133,70 @@ __device__ __forceinline__ void tmem_st16(uint32_t ta, const uint32_t *v)
                  : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Loads that stay where they are written, ahead of the waits: the next page's codes.
+__device__ __forceinline__ uint4 ldg128(const void *p)
+{
+    uint4 v;
+    asm volatile("ld.global.nc.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w)
 {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-template <typename T> __device__ __forceinline__ float query_top(const T *q, bool wide, int D)
+// Two fp32 values at once (one instruction each).
+struct F2 {
+    unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float x, float y)
 {
-    float top = 0.0f;
-    for (int c = 0; c < D; c += 8) {
-        float f[8];
-        load8(q + c, wide, f);
-#pragma unroll
-        for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(f[e]));
-    }
-    return top;
+    F2 r;
+    asm("mov.b64 %0, {%1,%2};" : "=l"(r.v) : "f"(x), "f"(y));
+    return r;
 }
-// 32 scaled values of the row as 16 fp16 pairs
-template <typename T> __device__ __forceinline__ void query_pairs(const T *q, bool wide, float up, uint32_t (&v)[16])
+__device__ __forceinline__ void un2(F2 a, float &x, float &y) { asm("mov.b64 {%0,%1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b)
 {
-#pragma unroll
-    for (int c = 0; c < 4; c++) {
-        float f[8];
-        load8(q + 8 * c, wide, f);
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[4 * c + e] = pack(f[2 * e] * up, f[2 * e + 1] * up);
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b)
+{
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c)
+{
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// Four consecutive 16-bit values as floats; `wide`: 8-byte aligned.
+__device__ __forceinline__ void query4(const void *q, int64_t i, bool half, bool wide, float (&f)[4])
+{
+    uint2 v;
+    if (wide) {
+        v = __ldg((const uint2 *)((const uint16_t *)q + i));
+    } else {
+        const uint16_t *p = (const uint16_t *)q + i;
+        v = make_uint2(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16);
+    }
+    if (half) {
+        const float2 a = __half22float2(*reinterpret_cast<__half2 *>(&v.x)), b = __half22float2(*reinterpret_cast<__half2 *>(&v.y));
+        f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
+    } else {
+        f[0] = __uint_as_float(v.x << 16), f[1] = __uint_as_float(v.x & 0xFFFF0000u);
+        f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xFFFF0000u);
     }
 }
 
@@ -146,8 +204,11 @@ template <int D, int FMT>
 __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __grid_constant__ AttnArgs a, const int qwide)
 {
     using W = Wide<D>;
-    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int STAGES = W::STAGES, UN = W::UN, UNP = W::UNP;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + (1024 - (su32(smem_raw) & 1023)) % 1024;
     __shared__ int s_lo[8], s_hi[8], s_abort;
+    __shared__ int64_t s_at[W::TILES * 128];  // a row's place in the partials
     __shared__ uint32_t s_tmem;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = a.group, Hk = a.pool.heads_kv;
@@ -164,9 +225,9 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
     auto wait = [&](int bi, uint32_t parity) -> bool {  // bounded; gives up with another role too
         const uint32_t b = bars + 8 * bi;
         if (bar_try(b, parity)) return true;
-        const unsigned long long t0 = gtime();
+        const long long t0 = clock64();  // a few clocks; %globaltimer takes hundreds
         while (!bar_try(b, parity)) {
-            if (*(volatile int *)&s_abort || gtime() - t0 > WAIT_NS) {
+            if (*(volatile int *)&s_abort || clock64() - t0 > WAIT_CLOCKS) {
                 *(volatile int *)&s_abort = 1;
                 return false;
             }
@@ -178,7 +239,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
     constexpr int SOFT = W::TILES * 128;
     if (tid == SOFT) {
         for (int i = 0; i < W::B_COUNT; i++)
-            bar_init(bars + 8 * i, i < STAGES || (i >= W::B_P && i < W::B_P + 2) ? 128u : 1u);
+            bar_init(bars + 8 * i, i < STAGES || (i >= W::B_P && i < W::B_O) ? 128u : 1u);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -186,9 +247,11 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&s_tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    // (the operands' memory holds the sequences' tables meanwhile)
+    const SeqTable seqs = load_seqs(a, sg, (int32_t *)smem, W::THREADS);
     int row = -1, lo = 0, hi = 0x7fffffff;
     if (tid < SOFT) {
-        row_range(a, sg, row_first + tid, row, lo, hi);
+        row_range(a, sg, seqs, row_first + tid, row, lo, hi);
         const int wlo = __reduce_min_sync(0xffffffffu, row >= 0 ? lo : 0x7fffffff);
         const int whi = __reduce_max_sync(0xffffffffu, row >= 0 ? hi : -1);
         if (lane == 0) {
@@ -206,246 +269,292 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
         lo_min = min(lo_min, s_lo[w]);
         hi_max = max(hi_max, s_hi[w]);
     }
-    const int u0 = max(sg.chunk * sg.ch, lo_min / UN);
-    const int u1 = min((sg.chunk + 1) * sg.ch, hi_max < 0 ? 0 : hi_max / UN + 1), n = max(u1 - u0, 0);
+    // pages [u0, u1) in n units
+    const int u0 = max(sg.chunk * sg.ch, lo_min / KVQ_PAGE);
+    const int u1 = min((sg.chunk + 1) * sg.ch, hi_max < 0 ? 0 : hi_max / KVQ_PAGE + 1), n = (max(u1 - u0, 0) + UNP - 1) / UNP;
 
     if (warp < SOFT / 32) {
         // ------------------------------------------------------------ a row per thread
         const int tile = warp >> 2, head = sg.kvh * G + (row_first + tid) % G;
         const uint32_t tm = tmem + tile * W::TILE_COLS + ((uint32_t)(32 * (warp & 3)) << 16);
-        // the query, scaled by a power of two, into TMEM (zeros for rows that do not exist)
-        float qf;
+        // the queries, scaled by a power of two each, as an operand (zeros for rows that do not exist): a row
+        // at a time per warp, four values per lane, eight rows on the way
+        int e = 0;
         {
-            const int64_t at = row < 0 ? 0 : row * a.ldq + (int64_t)head * D;
+            constexpr int PARTS = (D + 127) / 128;
             const bool half = a.at.type == T_F16;
-            float top = 0.0f;
-            if (row >= 0) top = half ? query_top((const __half *)a.q + at, qwide != 0, D) : query_top((const __nv_bfloat16 *)a.q + at, qwide != 0, D);
-            const int e = row_exponent(top);
-            const float up = a.at.scale < 0.0f ? -pow2(e) : pow2(e);
-            for (int c = 0; c < D / 32; c++) {
-                uint32_t v[16] = {};
-                if (row >= 0) {
-                    if (half) query_pairs((const __half *)a.q + at + 32 * c, qwide != 0, up, v);
-                    else query_pairs((const __nv_bfloat16 *)a.q + at + 32 * c, qwide != 0, up, v);
+            const float sign = a.at.scale < 0.0f ? -1.0f : 1.0f;
+            const int64_t at = row < 0 ? -1 : row * a.ldq + (int64_t)head * D;
+            const uint32_t dst = base + W::OFF_Q + tile * W::Q_BYTES + (warp & 3) * 32 * W::ROW;
+#pragma unroll 1
+            for (int r0 = 0; r0 < 32; r0 += 8) {
+                float f[8][PARTS][4];
+#pragma unroll
+                for (int r = 0; r < 8; r++) {
+                    const int64_t from = __shfl_sync(0xffffffffu, at, r0 + r);
+#pragma unroll
+                    for (int x = 0; x < PARTS; x++) {
+                        f[r][x][0] = f[r][x][1] = f[r][x][2] = f[r][x][3] = 0.0f;
+                        if (from >= 0 && lane * 4 + 128 * x < D) query4(a.q, from + lane * 4 + 128 * x, half, qwide != 0, f[r][x]);
+                    }
                 }
-                __syncwarp();
-                tmem_st16(tm + W::C_Q + 16 * c, v);
+#pragma unroll
+                for (int r = 0; r < 8; r++) {
+                    uint32_t top = 0;  // magnitudes order as integers, NaN above all
+#pragma unroll
+                    for (int x = 0; x < PARTS; x++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) top = max(top, __float_as_uint(f[r][x][k]) & 0x7fffffffu);
+                    const int er = row_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, top)));
+                    if (lane == r0 + r) e = er;
+                    const float up = sign * pow2(er);
+#pragma unroll
+                    for (int x = 0; x < PARTS; x++)
+                        if (lane * 4 + 128 * x < D) {
+                            const int piece = lane / 2 + 16 * x;
+                            const uint32_t d = dst + (piece >> 3) * W::Q_BLK + (r0 + r) * W::ROW + ((piece & 7) ^ r) * 16 + (lane & 1) * 8;
+                            asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(d), "r"(pack(f[r][x][0] * up, f[r][x][1] * up)),
+                                         "r"(pack(f[r][x][2] * up, f[r][x][3] * up))
+                                         : "memory");
+                        }
+                }
             }
-            qf = fabsf(a.at.scale) * code_unit<FMT>() * (a.at.softcap > 0.0f ? 1.0f : 1.4426950408889634f) * pow2(-e);
         }
-        tmem_st_wait();
-        fence_before();
+        const float qf = fabsf(a.at.scale) * code_unit<FMT>() * (a.at.softcap > 0.0f ? 1.0f : 1.4426950408889634f) * pow2(-e);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
         const int lo_max = __reduce_max_sync(0xffffffffu, row >= 0 ? lo : 0);
         const int hi_min = __reduce_min_sync(0xffffffffu, row >= 0 ? hi : 0x7fffffff);
         const bool cap = a.at.softcap > 0.0f;
         const float inv_cap2 = cap ? 2.0f * 1.4426950408889634f / a.at.softcap : 0.0f;
-        float m = -INFINITY, l = 0.0f, vpow = 0.0f;  // maximum in base 2
+        float m = -INFINITY, vpow = 0.0f;  // maximum in base 2
+        F2 l = f2(0.0f, 0.0f);
         bool ok = tile < nact;
-        for (int i = 0; i < n && ok; i++) {
-            const int st = i % STAGES;
-            ok = wait(W::B_S + tile, i & 1) && wait(W::B_FULL + st, (i / STAGES) & 1);
-            if (!(ok = __all_sync(0xffffffffu, ok))) break;
-            fence_after();
-            const float *ks = (const float *)(smem + W::OFF_SC + st * W::SC_STAGE), *vs = ks + UN, *ex = vs + UN;
-            uint32_t s[UN];
-            tmem_ld32(tm + W::C_S, s);
-            tmem_ld32(tm + W::C_S + 32, s + 32);
-            tmem_ld_wait();
-            const int t0 = (u0 + i) * UN;
-            const bool whole = t0 >= lo_max && t0 + UN - 1 <= hi_min && ex[2] == 0.0f;
-            float x[UN], mx = -INFINITY, qx = qf;
-#pragma unroll
-            for (int j = 0; j < UN; j += 4) {
-                const float4 k4 = *(const float4 *)(ks + j);
-                x[j] = __uint_as_float(s[j]) * k4.x;
-                x[j + 1] = __uint_as_float(s[j + 1]) * k4.y;
-                x[j + 2] = __uint_as_float(s[j + 2]) * k4.z;
-                x[j + 3] = __uint_as_float(s[j + 3]) * k4.w;
-            }
-            if (cap) {
-#pragma unroll
-                for (int j = 0; j < UN; j++) x[j] = capped<false>(x[j] * qf, a.at.softcap, inv_cap2) * 1.4426950408889634f;
-                qx = 1.0f;
-            }
-            if (!whole) {
-                const bool bad = ex[2] != 0.0f;
-#pragma unroll
-                for (int j = 0; j < UN; j++)
-                    if (bad || t0 + j < lo || t0 + j > hi || t0 + j >= len) x[j] = -INFINITY;
-            }
-#pragma unroll
-            for (int j = 0; j < UN; j++) mx = fmaxf(mx, x[j]);
-            const float top = mx == -INFINITY ? -INFINITY : mx * qx;
-            const bool raise = top > m + RAISE || (m == -INFINITY && top > -INFINITY);
-            const float f = raise ? ex2(m - top) : 1.0f, ve = ex[0];
-            if (raise) m = top;
-            l *= f;
-            vpow = ex[1];
-            if (i > 0 && __any_sync(0xffffffffu, raise || ve != 1.0f)) {
-                ok = wait(W::B_O + tile, (i - 1) & 1);
-                if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        // The sums so far and `done` 32-column pieces of this half's weights, scaled by f: after the products
+        // that add to O (through half `half` of unit `unit`; -1: none yet) are complete.
+        auto rescale = [&](int unit, int half, int first, int done, float f, float fo) {
+            l = mul2(l, f2(f, f));
+            tmem_st_wait();
+            if (unit >= 0) {
+                ok = wait(W::B_O + tile * UNP + half, unit & 1);
+                if (!(ok = __all_sync(0xffffffffu, ok))) return;
                 fence_after();
-                const float fo = f * ve;
+                const F2 fo2 = f2(fo, fo);
 #pragma unroll 1
                 for (int c = 0; c < D / 32; c++) {
                     uint32_t v[32];
                     tmem_ld32(tm + W::C_O + 32 * c, v);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 32; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * fo);
+                    for (int j = 0; j < 32; j += 2) {
+                        float p, q;
+                        un2(mul2(f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), fo2), p, q);
+                        v[j] = __float_as_uint(p);
+                        v[j + 1] = __float_as_uint(q);
+                    }
                     tmem_st16(tm + W::C_O + 32 * c, v);
                     tmem_st16(tm + W::C_O + 32 * c + 16, v + 16);
                 }
             }
-            const float off = m == -INFINITY ? 0.0f : m;
-            uint32_t p[UN / 2];
+            if (done) {
+                uint32_t v[16];
+                tmem_ld16(tm + W::C_S + 16 * first, v);
+                tmem_ld_wait();
+                const uint32_t h = pack(f, f);
 #pragma unroll
-            for (int j = 0; j < UN; j += 4) {
-                const float4 v4 = *(const float4 *)(vs + j);
-                float y[4], w[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) y[e] = ex2(fmaf(x[j + e], qx, -off));
-                w[0] = y[0] * v4.x;
-                w[1] = y[1] * v4.y;
-                w[2] = y[2] * v4.z;
-                w[3] = y[3] * v4.w;
-                if (!whole) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (x[j + e] == -INFINITY) y[e] = w[e] = 0.0f;  // whatever the unseen position holds
-                }
-                l += (y[0] + y[1]) + (y[2] + y[3]);
-                p[j / 2] = pack(w[0], w[1]);
-                p[j / 2 + 1] = pack(w[2], w[3]);
+                for (int j = 0; j < 16; j++) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(v[j]) : "r"(h));
+                tmem_st16(tm + W::C_S + 16 * first, v);
             }
-            tmem_st16(tm + W::C_S, p);
-            tmem_st16(tm + W::C_S + 16, p + 16);
             tmem_st_wait();
-            fence_before();
-            bar_arrive(bars + 8 * (W::B_P + tile));
+        };
+        // One unit; PLAIN: every row of the warp sees every position and there is no cap.
+        auto unit = [&](int i, auto plain) {
+            constexpr bool PLAIN = decltype(plain)::value;
+            const int st = i % STAGES, t0 = u0 * KVQ_PAGE + i * UN;
+            const float *ks = (const float *)(smem + W::OFF_SC + st * W::SC_STAGE), *vs = ks + UN, *ex = vs + UN;
+            const F2 qf2 = f2(qf, qf);
+            vpow = ex[1];
+            if (i > 0 && ex[0] != 1.0f) {  // the values' unit rose: O follows (every row alike)
+                rescale(i - 1, UNP - 1, 0, 0, 1.0f, ex[0]);
+                if (!ok) return;
+            }
+#pragma unroll 1
+            for (int c = 0; c < UN / 32; c++) {
+                F2 x[16];
+                {
+                    uint32_t s[32];
+                    tmem_ld32(tm + W::C_S + 32 * c, s);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {  // s times the keys' scales
+                        const float4 k4 = *(const float4 *)(ks + 32 * c + 2 * j);
+                        x[j] = mul2(f2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), f2(k4.x, k4.y));
+                        x[j + 1] = mul2(f2(__uint_as_float(s[2 * j + 2]), __uint_as_float(s[2 * j + 3])), f2(k4.z, k4.w));
+                    }
+                }
+                if (!PLAIN) {
+                    const int t = t0 + 32 * c;
+                    const bool bad = ex[2 + 32 * c / KVQ_PAGE] != 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        float p, q;
+                        un2(x[j], p, q);
+                        if (bad || t + 2 * j < lo || t + 2 * j > hi || t + 2 * j >= len) p = -INFINITY;
+                        if (bad || t + 2 * j + 1 < lo || t + 2 * j + 1 > hi || t + 2 * j + 1 >= len) q = -INFINITY;
+                        x[j] = f2(p, q);
+                    }
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    float p, q;
+                    un2(x[j], p, q);
+                    mx[j & 3] = max3(mx[j & 3], p, q);
+                }
+                const float top0 = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+                float top = top0 == -INFINITY ? -INFINITY : top0 * qf;
+                if (!PLAIN && cap && top0 != -INFINITY) top = capped<false>(top, a.at.softcap, inv_cap2) * 1.4426950408889634f;  // monotonic
+                const bool raise = top > m + RAISE || (m == -INFINITY && top > -INFINITY);
+                if (__any_sync(0xffffffffu, raise)) {
+                    // by a power of two, which every factor then is: the rescaled weights stay exact
+                    const float to = m == -INFINITY ? top : m + ceilf(top - m), f = raise ? ex2(m - to) : 1.0f;
+                    if (raise) m = to;
+                    // O holds the units before this one, and this one's first half once that is handed over
+                    rescale(c < 2 ? i - 1 : i, c < 2 ? UNP - 1 : 0, c - 1, c & 1, f, f);
+                    if (!ok) return;
+                }
+                const float off = m == -INFINITY ? 0.0f : m;
+                const F2 off2 = f2(-off, -off);
+                uint32_t p[16];
+                F2 l2[2] = {l, f2(0.0f, 0.0f)};
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) {
+                    const float4 v4 = *(const float4 *)(vs + 32 * c + 2 * j);
+                    const F2 v2[2] = {f2(v4.x, v4.y), f2(v4.z, v4.w)};
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        float y, z;
+                        if (!PLAIN && cap) {
+                            un2(mul2(x[j + h], qf2), y, z);
+                            y = fmaf(capped<false>(y, a.at.softcap, inv_cap2), 1.4426950408889634f, -off);
+                            z = fmaf(capped<false>(z, a.at.softcap, inv_cap2), 1.4426950408889634f, -off);
+                        } else {
+                            un2(fma2(x[j + h], qf2, off2), y, z);
+                        }
+                        y = ex2(y);
+                        z = ex2(z);
+                        float wy, wz;
+                        if (!PLAIN) {  // whatever an unseen position holds
+                            float xy, xz;
+                            un2(x[j + h], xy, xz);
+                            if (xy == -INFINITY) y = 0.0f;
+                            if (xz == -INFINITY) z = 0.0f;
+                            un2(mul2(f2(y, z), v2[h]), wy, wz);
+                            if (xy == -INFINITY) wy = 0.0f;
+                            if (xz == -INFINITY) wz = 0.0f;
+                        } else {
+                            un2(mul2(f2(y, z), v2[h]), wy, wz);
+                        }
+                        l2[h] = add2(l2[h], f2(y, z));
+                        p[j + h] = pack(wy, wz);
+                    }
+                }
+                l = add2(l2[0], l2[1]);
+                tmem_st16(tm + W::C_S + 16 * c, p);  // over scores that were read
+                if (c & 1) {                          // 64 positions' weights are complete
+                    tmem_st_wait();
+                    fence_before();
+                    bar_arrive(bars + 8 * (W::B_P + tile * UNP + c / 2));
+                }
+            }
+        };
+        for (int i = 0; i < n && ok; i++) {
+            const int st = i % STAGES;
+            ok = wait(W::B_S + tile, i & 1) && wait(W::B_FULL + st, (i / STAGES) & 1);
+            if (!(ok = __all_sync(0xffffffffu, ok))) break;
+            fence_after();
+            const float *ex = (const float *)(smem + W::OFF_SC + st * W::SC_STAGE) + 2 * UN;
+            const int t0 = u0 * KVQ_PAGE + i * UN;
+            if (!cap && t0 >= lo_max && t0 + UN - 1 <= hi_min && ex[2] == 0.0f && ex[3] == 0.0f) unit(i, std::true_type{});
+            else unit(i, std::false_type{});
         }
         if (ok && n > 0) {
-            ok = wait(W::B_O + tile, (n - 1) & 1);
+            ok = wait(W::B_O + tile * UNP + UNP - 1, (n - 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
         }
         const int64_t RH = (int64_t)a.bt.rows * a.at.heads, slot = sg.pre ? sg.chunk : a.nsp + sg.chunk;
         const int64_t at = slot * RH + (int64_t)row * a.at.heads + head;
+        s_at[tid] = row >= 0 ? at * D : -1;
         if (ok && n > 0) {
             fence_after();
+            // 32 rows by 32 columns at a time through the tile's query operand (done with), so that a warp
+            // writes 128 consecutive bytes of a row
+            float *tr = (float *)(smem + W::OFF_Q + tile * W::Q_BYTES) + (warp & 3) * 32 * 32;
 #pragma unroll 1
             for (int c = 0; c < D / 32; c++) {
                 uint32_t v[32];
                 tmem_ld32(tm + W::C_O + 32 * c, v);
                 tmem_ld_wait();
-                if (row >= 0) {
-                    float4 *o = (float4 *)(a.part_o + at * D + 32 * c);
+                __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        o[j] = make_float4(__uint_as_float(v[4 * j]) * vpow, __uint_as_float(v[4 * j + 1]) * vpow,
-                                           __uint_as_float(v[4 * j + 2]) * vpow, __uint_as_float(v[4 * j + 3]) * vpow);
+                for (int j = 0; j < 32; j++) tr[lane * 32 + (j ^ lane)] = __uint_as_float(v[j]) * vpow;
+                __syncwarp();
+#pragma unroll 16
+                for (int r = 0; r < 32; r++) {
+                    const int64_t to = s_at[warp * 32 + r];
+                    const float o = tr[r * 32 + (lane ^ r)];
+                    if (to >= 0) a.part_o[to + 32 * c + lane] = o;
                 }
             }
         }
-        if (row >= 0) a.part_ml[at] = ok ? make_float2(m, l) : make_float2(0.0f, NAN);
+        float la, lb;
+        un2(l, la, lb);
+        if (row >= 0) a.part_ml[at] = ok ? make_float2(m, la + lb) : make_float2(0.0f, NAN);
     } else if (warp < SOFT / 32 + 4) {
         // ------------------------------------------------------------ codes to operands
         const int dt = tid - SOFT, dw = dt >> 5;
-        constexpr int KT = D / 32, VT = (D + 127) / 128;
+        // a page's K or V: 4 D pieces of 16 codes, T per thread, a warp's at consecutive addresses
+        constexpr int T = D / 32;
         struct Codes {
-            uint4 k[KT];
-            uint2 v[VT][8];
-            float sc[2];
-            bool bad;
+            uint4 k[T], v[T];
         };
         auto page_of = [&](int u) { return u < u1 ? __ldg(sg.pages + u) : -1; };
+        auto none = [&](int page) { return (unsigned)page >= (unsigned)a.pool.n_pages; };
         auto load = [&](int page, Codes &c) {
-            c.bad = (unsigned)page >= (unsigned)a.pool.n_pages;
-            if (c.bad) {
+            if (none(page)) {
 #pragma unroll
-                for (int i = 0; i < KT; i++) c.k[i] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < VT; i++)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) c.v[i][j] = make_uint2(0, 0);
-                c.sc[0] = c.sc[1] = 0.0f;
+                for (int i = 0; i < T; i++) c.k[i] = c.v[i] = make_uint4(0, 0, 0, 0);
                 return;
             }
-            const int64_t at = ((int64_t)page * Hk + sg.kvh) * KVQ_PAGE;
-            const uint8_t *k = (const uint8_t *)a.pool.k + at * D, *v = (const uint8_t *)a.pool.v + at * D;
+            const int64_t at = (((int64_t)page * Hk + sg.kvh) * KVQ_PAGE) * D + dt * 16;
+            const uint8_t *k = (const uint8_t *)a.pool.k + at, *v = (const uint8_t *)a.pool.v + at;
 #pragma unroll
-            for (int i = 0; i < KT; i++) {
-                const int t = dt + 128 * i, r7 = t & 7, ch = (t >> 3) % (D / 16), rg = (t >> 3) / (D / 16);
-                c.k[i] = __ldg((const uint4 *)(k + (rg * 8 + r7) * D + ch * 16));
-            }
-#pragma unroll
-            for (int i = 0; i < VT; i++) {
-                const int t = dt + 128 * i, tk = t & 7, c8 = t >> 3;
-                if (t < D)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) c.v[i][j] = __ldg((const uint2 *)(v + (tk * 8 + j) * D + c8 * 8));
-            }
-            if (dw < 2) {  // warp 0: V's scales, warp 1: K's
-                const float *s = (dw == 0 ? a.pool.v_scale : a.pool.k_scale) + at;
-                c.sc[0] = __ldg(s + lane);
-                c.sc[1] = __ldg(s + lane + 32);
+            for (int i = 0; i < T; i++) {
+                c.k[i] = ldg128(k + 2048 * i);
+                c.v[i] = ldg128(v + 2048 * i);
             }
         };
-        Codes cur, nxt;
-        load(page_of(u0), cur);
-        int page = page_of(u0 + 1);
-        __syncthreads();
+        // a unit's scales: warp 0 V's, warp 1 K's; lane: positions lane, lane + 32, ...
+        auto load_scales = [&](int page0, int page1, float (&c)[2 * UNP]) {
+            if (dw >= 2) return;
+#pragma unroll
+            for (int x = 0; x < UNP; x++) {
+                const int page = x ? page1 : page0;
+                const float *s = (dw == 0 ? a.pool.v_scale : a.pool.k_scale) + ((int64_t)page * Hk + sg.kvh) * KVQ_PAGE + lane;
+                c[2 * x] = none(page) ? 0.0f : __ldg(s);
+                c[2 * x + 1] = none(page) ? 0.0f : __ldg(s + 32);
+            }
+        };
         float vp = 0.0f;  // 2^E (warp 0)
         bool ok = true;
-        for (int i = 0; i < n && ok; i++) {
-            const int st = i % STAGES;
-            load(page, nxt);
-            page = page_of(u0 + i + 2);
-            if (i >= STAGES) {
-                ok = wait(W::B_EMPTY + st, (i / STAGES - 1) & 1);
-                if (!(ok = __all_sync(0xffffffffu, ok))) break;
-            }
-            const uint32_t ka = base + st * W::STAGE, va = ka + W::K_BYTES;
-#pragma unroll
-            for (int x = 0; x < KT; x++) {
-                const int t = dt + 128 * x, r7 = t & 7, ch = (t >> 3) % (D / 16), rg = (t >> 3) / (D / 16);
-                const uint32_t w[4] = {cur.k[x].x ^ code_flip<FMT>(), cur.k[x].y ^ code_flip<FMT>(), cur.k[x].z ^ code_flip<FMT>(),
-                                       cur.k[x].w ^ code_flip<FMT>()};
-                const uint32_t d = ka + rg * W::K_SBO + ch * 256 + r7 * 16;
-                sts128(d, codes2<FMT, 0, 1>(w[0]), codes2<FMT, 2, 3>(w[0]), codes2<FMT, 0, 1>(w[1]), codes2<FMT, 2, 3>(w[1]));
-                sts128(d + 128, codes2<FMT, 0, 1>(w[2]), codes2<FMT, 2, 3>(w[2]), codes2<FMT, 0, 1>(w[3]), codes2<FMT, 2, 3>(w[3]));
-            }
-#pragma unroll
-            for (int x = 0; x < VT; x++) {
-                const int t = dt + 128 * x, tk = t & 7, c8 = t >> 3;
-                if (t < D) {
-                    const uint32_t d = va + c8 * W::V_SBO + tk * W::V_LBO;
-#pragma unroll
-                    for (int wd = 0; wd < 2; wd++)
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            uint32_t ab[4];
-#pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                const uint32_t r0 = (wd ? cur.v[x][2 * j].y : cur.v[x][2 * j].x) ^ code_flip<FMT>();
-                                const uint32_t r1 = (wd ? cur.v[x][2 * j + 1].y : cur.v[x][2 * j + 1].x) ^ code_flip<FMT>();
-                                ab[j] = __byte_perm(r0, r1, h ? 0x7362 : 0x5140);
-                            }
-                            const int dd = wd * 4 + h * 2;
-                            sts128(d + dd * 16, codes2<FMT, 0, 1>(ab[0]), codes2<FMT, 0, 1>(ab[1]), codes2<FMT, 0, 1>(ab[2]),
-                                   codes2<FMT, 0, 1>(ab[3]));
-                            sts128(d + dd * 16 + 16, codes2<FMT, 2, 3>(ab[0]), codes2<FMT, 2, 3>(ab[1]), codes2<FMT, 2, 3>(ab[2]),
-                                   codes2<FMT, 2, 3>(ab[3]));
-                        }
-                }
-            }
-            float *ks = (float *)(smem + W::OFF_SC + st * W::SC_STAGE), *vs = ks + UN, *ex = vs + UN;
+        auto put_scales = [&](int i, int page0, int page1, const float (&c)[2 * UNP]) {
+            float *ks = (float *)(smem + W::OFF_SC + i % STAGES * W::SC_STAGE), *vs = ks + UN, *ex = vs + UN;
             if (dw == 0) {
-                const int t0 = (u0 + i) * UN + lane;
-                const float v0 = cur.sc[0] * code_unit<FMT>(), v1 = cur.sc[1] * code_unit<FMT>();
+                const int t0 = u0 * KVQ_PAGE + i * UN + lane;
                 float top = 0.0f;  // of positions that exist; a NaN does not count
-                if (t0 < len) top = fmaxf(top, v0);
-                if (t0 + 32 < len) top = fmaxf(top, v1);
+#pragma unroll
+                for (int x = 0; x < 2 * UNP; x++)
+                    if (t0 + 32 * x < len) top = fmaxf(top, c[x] * code_unit<FMT>());
                 const float pw = scale_pow(warp_max(top));
                 float ve = 1.0f;
                 if (i == 0) {
@@ -455,20 +564,77 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                     vp = pw;
                 }
                 const float inv = pow_inverse(vp);
-                vs[lane] = v0 * inv;
-                vs[lane + 32] = v1 * inv;
+#pragma unroll
+                for (int x = 0; x < 2 * UNP; x++) vs[lane + 32 * x] = c[x] * code_unit<FMT>() * inv;
                 if (lane == 0) {
                     ex[0] = ve;
                     ex[1] = vp;
-                    ex[2] = cur.bad ? 1.0f : 0.0f;
+                    ex[2] = none(page0) ? 1.0f : 0.0f;
+                    ex[3] = UNP > 1 && none(page1) ? 1.0f : 0.0f;
                 }
             } else if (dw == 1) {
-                ks[lane] = cur.sc[0];
-                ks[lane + 32] = cur.sc[1];
+#pragma unroll
+                for (int x = 0; x < 2 * UNP; x++) ks[lane + 32 * x] = c[x];
             }
+        };
+        // page h of the segment's share: half h % UNP of unit h / UNP
+        auto convert = [&](int h, const Codes &cur) {
+            const uint32_t d = base + h / UNP % STAGES * W::STAGE + h % UNP * KVQ_PAGE * W::ROW;
+#pragma unroll
+            for (int i = 0; i < T; i++) {
+                // piece t: position r, codes 16 ch ..: two operand pieces of 8.  Lanes of the upper half of a
+                // 128-code row write them in the other order, so that eight lanes meet eight banks.
+                const int t = dt + 128 * i, ch = t % (D / 16), r = t / (D / 16), pc = (ch & 3) * 2, swap = (ch >> 2) & 1;
+                const uint32_t to = d + (ch >> 2) * W::K_BLK + r * W::ROW;
+                const uint32_t o0 = to + ((pc + swap) ^ (r & 7)) * 16, o1 = to + ((pc + 1 - swap) ^ (r & 7)) * 16;
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const uint4 c = x ? cur.v[i] : cur.k[i];
+                    const uint32_t w[4] = {(swap ? c.z : c.x) ^ code_flip<FMT>(), (swap ? c.w : c.y) ^ code_flip<FMT>(),
+                                           (swap ? c.x : c.z) ^ code_flip<FMT>(), (swap ? c.y : c.w) ^ code_flip<FMT>()};
+                    sts128(o0 + x * W::K_BYTES, codes2<FMT, 0, 1>(w[0]), codes2<FMT, 2, 3>(w[0]), codes2<FMT, 0, 1>(w[1]), codes2<FMT, 2, 3>(w[1]));
+                    sts128(o1 + x * W::K_BYTES, codes2<FMT, 0, 1>(w[2]), codes2<FMT, 2, 3>(w[2]), codes2<FMT, 0, 1>(w[3]), codes2<FMT, 2, 3>(w[3]));
+                }
+            }
+        };
+        // two sets of registers in turn (a copy from one to the other would wait for the loads)
+        Codes c0, c1;
+        float sc[2 * UNP];
+        int p0 = page_of(u0), p1 = page_of(u0 + 1);  // this page and the next
+        load(p0, c0);
+        load_scales(p0, p1, sc);
+        __syncthreads();
+        auto slot = [&](int i) {
+            if (i < STAGES) return true;
+            ok = wait(W::B_EMPTY + i % STAGES, (i / STAGES - 1) & 1);
+            return ok = __all_sync(0xffffffffu, ok);
+        };
+        auto done = [&](int i) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // operands: generic writes -> tensor core
-            bar_arrive(bars + 8 * (W::B_FULL + st));
-            cur = nxt;
+            bar_arrive(bars + 8 * (W::B_FULL + i % STAGES));
+        };
+        for (int h = 0; h < n * UNP && ok; h += 2) {  // two pages a round: one unit, or two of one page
+            const int i = h / UNP, p2 = page_of(u0 + h + 2), p3 = page_of(u0 + h + 3);
+            load(p1, c1);
+            if (!slot(i)) break;
+            put_scales(i, p0, p1, sc);
+            if (UNP == 2) load_scales(p2, p3, sc);
+            else load_scales(p1, p1, sc);
+            convert(h, c0);
+            if (UNP == 1) {
+                done(i);
+                if (h + 1 >= n) break;
+                load(p2, c0);
+                if (!slot(i + 1)) break;
+                put_scales(i + 1, p1, p1, sc);
+                load_scales(p2, p2, sc);
+            } else {
+                load(p2, c0);
+            }
+            convert(h + 1, c1);
+            done(UNP == 1 ? i + 1 : i);
+            p0 = p2;
+            p1 = p3;
         }
     } else {
         // ------------------------------------------------------------ products
@@ -476,10 +642,10 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
         if (lane == 0 && n > 0) {
             fence_after();
             auto qk = [&](int t, int st) {
-                const uint32_t k = base + st * W::STAGE, tm = tmem + t * W::TILE_COLS;
+                const uint32_t q = base + W::OFF_Q + t * W::Q_BYTES, k = base + st * W::STAGE, d = tmem + t * W::TILE_COLS + W::C_S;
 #pragma unroll
                 for (int kk = 0; kk < D / 16; kk++)
-                    umma_ts<UN>(tm + W::C_S, tm + W::C_Q + 8 * kk, sdesc(k + kk * 256, 128, W::K_SBO), kk != 0);
+                    umma_ss<UN>(d, sdesc(q + kk / 4 * W::Q_BLK + kk % 4 * 32), sdesc(k + kk / 4 * W::K_BLK + kk % 4 * 32), kk != 0);
                 umma_commit(bars + 8 * (W::B_S + t));
             };
             bool ok = wait(W::B_FULL, 0);
@@ -488,13 +654,18 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             for (int i = 0; i < n && ok; i++) {
                 const int st = i % STAGES, nx = (i + 1) % STAGES;
                 for (int t = 0; t < nact; t++) {
-                    if (!(ok = wait(W::B_P + t, i & 1))) break;
-                    fence_after();
                     const uint32_t v = base + st * W::STAGE + W::K_BYTES, tm = tmem + t * W::TILE_COLS;
 #pragma unroll
-                    for (int kk = 0; kk < UN / 16; kk++)
-                        umma_ts<D>(tm + W::C_O, tm + W::C_S + 8 * kk, sdesc(v + kk * 2 * W::V_LBO, W::V_LBO, W::V_SBO), i != 0 || kk != 0);
-                    umma_commit(bars + 8 * (W::B_O + t));
+                    for (int hf = 0; hf < UNP && ok; hf++) {
+                        if (!(ok = wait(W::B_P + t * UNP + hf, i & 1))) break;
+                        fence_after();
+#pragma unroll
+                        for (int kk = 0; kk < KVQ_PAGE / 16; kk++)
+                            umma_ts<D>(tm + W::C_O, tm + W::C_S + 32 * hf + 8 * kk,
+                                       sdesc(v + (hf * 4 + kk) * 2 * W::GROUP, W::K_BLK), i != 0 || hf != 0 || kk != 0);
+                        umma_commit(bars + 8 * (W::B_O + t * UNP + hf));
+                    }
+                    if (!ok) break;
                     if (t == nact - 1) umma_commit(bars + 8 * (W::B_EMPTY + st));
                     if (i + 1 < n) {
                         if (t == 0) {
@@ -507,8 +678,8 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             }
             // every product issued completes before the TMEM is released
             umma_commit(bars + 8 * W::B_DRAIN);
-            const unsigned long long t0 = gtime();
-            while (!bar_try(bars + 8 * W::B_DRAIN, 0) && gtime() - t0 < WAIT_NS) {}
+            const long long t0 = clock64();
+            while (!bar_try(bars + 8 * W::B_DRAIN, 0) && clock64() - t0 < WAIT_CLOCKS) {}
         }
         __syncwarp();
     }
