@@ -7,13 +7,14 @@
 // the conversion of codes to fp16 take about the same time, and HBM little.  So one CTA takes two tiles of
 // 128 rows (one for head_dim 256) over the same positions -- each code is converted once for 256 rows --
 // and its roles overlap, 128 positions (two pages; one for head_dim 256) at a time:
-//   warps of a tile (4 each)  a thread per row: S from TMEM 32 columns at a time, weights as fp16 back into
-//                             TMEM over S.  One pass: the weights are taken relative to the maximum so
-//                             far, which may lag by 2^8 (fp16 holds them up to 2^13); when a row's scores
-//                             go above that, its sums, O in TMEM and this unit's earlier weights are
-//                             rescaled, which after the first positions is rare
-//   4 converting warps        codes from global memory (next page's loads in flight) to fp16 K and V
-//                             operands in shared memory, scales beside them
+//   warps of a tile (4 each)  S from TMEM 64 columns at a time in fragments of 4 rows by 2 columns a lane
+//                             (a lane so needs a quarter of the columns' scales), weights as fp16 back
+//                             into TMEM over S.  The weights are taken relative to a row's reference, 2^6
+//                             above its maximum when it was set; only when a weight reaches 2 is
+//                             the maximum searched, the reference raised, and the sums and O rescaled, which
+//                             after the first positions is rare
+//   4 converting warps        codes from global memory (three K or V pages' loads in flight) to fp16 K
+//                             and V operands in shared memory, scales beside them
 //   1 warp                    one thread issues tcgen05.mma: S = Q K^T and O += P V with P and the
 //                             accumulators in TMEM; while one tile's rows are in their softmax, the other
 //                             tile's products run, and P V starts on the first 64 positions' weights
@@ -33,13 +34,13 @@ namespace llmdot {
 namespace {
 
 constexpr long long WAIT_CLOCKS = 4000000000ll;  // about two seconds
-constexpr float RAISE = 8.0f;  // the maximum may lag by this power of two
+constexpr float HEAD = 6.0f;  // a row's reference stands this power of two above its maximum
 
 template <int D> struct Wide {
     static constexpr int TILES = D == 256 ? 1 : 2;
     static constexpr int UNP = D == 256 ? 1 : 2, UN = UNP * KVQ_PAGE;  // pages and positions of a unit
     static constexpr int STAGES = D == 64 ? 3 : 2;
-    static constexpr int THREADS = TILES * 128 + 128 + 32;
+    static constexpr int THREADS = TILES * 128 + 256;  // rows, converters, products (one warp of four)
     static constexpr uint32_t ROW = 128, GROUP = 8 * ROW;  // bytes of an operand's row, of eight
     static constexpr int KBLK = (D + 63) / 64;             // 64-wide blocks along the head dimension (Q, K)
     static constexpr uint32_t Q_BLK = 128 * ROW, K_BLK = UN * ROW;
@@ -117,12 +118,24 @@ __device__ __forceinline__ void tmem_ld32(uint32_t ta, uint32_t *v)
                    "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
                  : "r"(ta));
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t ta, uint32_t *v)
+// 16 lanes x 64 columns: register 4 i + 2 h + e of a lane is row lane / 4 + 8 h, column 8 i + 2 (lane % 4) + e
+__device__ __forceinline__ void tmem_ld_frag(uint32_t ta, uint32_t *v)
 {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-                   "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                   "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+                   "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+                   "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
                  : "r"(ta));
+}
+// 16 lanes x 32 columns: register 2 i + h is row lane / 4 + 8 h, column 4 i + lane % 4
+__device__ __forceinline__ void tmem_st_frag(uint32_t ta, const uint32_t *v)
+{
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(ta),
+                 "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+                 "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st16(uint32_t ta, const uint32_t *v)
@@ -174,23 +187,9 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c)
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
     return r;
 }
-__device__ __forceinline__ float max3(float a, float b, float c)
+// Four 16-bit values as floats.
+__device__ __forceinline__ void halves4(uint2 v, bool half, float (&f)[4])
 {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-
-// Four consecutive 16-bit values as floats; `wide`: 8-byte aligned.
-__device__ __forceinline__ void query4(const void *q, int64_t i, bool half, bool wide, float (&f)[4])
-{
-    uint2 v;
-    if (wide) {
-        v = __ldg((const uint2 *)((const uint16_t *)q + i));
-    } else {
-        const uint16_t *p = (const uint16_t *)q + i;
-        v = make_uint2(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16);
-    }
     if (half) {
         const float2 a = __half22float2(*reinterpret_cast<__half2 *>(&v.x)), b = __half22float2(*reinterpret_cast<__half2 *>(&v.y));
         f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
@@ -273,8 +272,11 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
     const int u0 = max(sg.chunk * sg.ch, lo_min / KVQ_PAGE);
     const int u1 = min((sg.chunk + 1) * sg.ch, hi_max < 0 ? 0 : hi_max / KVQ_PAGE + 1), n = (max(u1 - u0, 0) + UNP - 1) / UNP;
 
+    // Registers: 16 warps start with 128 each (2048 warp-registers in all); the row warps hold two pieces of
+    // scores and need more: 8 * 168 + 4 * 128 + 4 * 40 = 2016.
     if (warp < SOFT / 32) {
         // ------------------------------------------------------------ a row per thread
+        if (W::TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
         const int tile = warp >> 2, head = sg.kvh * G + (row_first + tid) % G;
         const uint32_t tm = tmem + tile * W::TILE_COLS + ((uint32_t)(32 * (warp & 3)) << 16);
         // the queries, scaled by a power of two each, as an operand (zeros for rows that do not exist): a row
@@ -288,23 +290,41 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             const uint32_t dst = base + W::OFF_Q + tile * W::Q_BYTES + (warp & 3) * 32 * W::ROW;
 #pragma unroll 1
             for (int r0 = 0; r0 < 32; r0 += 8) {
-                float f[8][PARTS][4];
+                uint2 raw[8][PARTS];  // loaded first, converted after, so that the loads overlap
+                const uint16_t *src[8];
 #pragma unroll
                 for (int r = 0; r < 8; r++) {
                     const int64_t from = __shfl_sync(0xffffffffu, at, r0 + r);
+                    src[r] = from >= 0 ? (const uint16_t *)a.q + from + lane * 4 : nullptr;
+                }
+                if (qwide) {
 #pragma unroll
-                    for (int x = 0; x < PARTS; x++) {
-                        f[r][x][0] = f[r][x][1] = f[r][x][2] = f[r][x][3] = 0.0f;
-                        if (from >= 0 && lane * 4 + 128 * x < D) query4(a.q, from + lane * 4 + 128 * x, half, qwide != 0, f[r][x]);
-                    }
+                    for (int r = 0; r < 8; r++)
+#pragma unroll
+                        for (int x = 0; x < PARTS; x++)
+                            raw[r][x] = src[r] && lane * 4 + 128 * x < D ? __ldg((const uint2 *)(src[r] + 128 * x)) : make_uint2(0, 0);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 8; r++)
+#pragma unroll
+                        for (int x = 0; x < PARTS; x++) {
+                            raw[r][x] = make_uint2(0, 0);
+                            if (src[r] && lane * 4 + 128 * x < D) {
+                                const uint16_t *p = src[r] + 128 * x;
+                                raw[r][x] = make_uint2(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16);
+                            }
+                        }
                 }
 #pragma unroll
                 for (int r = 0; r < 8; r++) {
+                    float f[PARTS][4];
+#pragma unroll
+                    for (int x = 0; x < PARTS; x++) halves4(raw[r][x], half, f[x]);
                     uint32_t top = 0;  // magnitudes order as integers, NaN above all
 #pragma unroll
                     for (int x = 0; x < PARTS; x++)
 #pragma unroll
-                        for (int k = 0; k < 4; k++) top = max(top, __float_as_uint(f[r][x][k]) & 0x7fffffffu);
+                        for (int k = 0; k < 4; k++) top = max(top, __float_as_uint(f[x][k]) & 0x7fffffffu);
                     const int er = row_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, top)));
                     if (lane == r0 + r) e = er;
                     const float up = sign * pow2(er);
@@ -313,8 +333,8 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                         if (lane * 4 + 128 * x < D) {
                             const int piece = lane / 2 + 16 * x;
                             const uint32_t d = dst + (piece >> 3) * W::Q_BLK + (r0 + r) * W::ROW + ((piece & 7) ^ r) * 16 + (lane & 1) * 8;
-                            asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(d), "r"(pack(f[r][x][0] * up, f[r][x][1] * up)),
-                                         "r"(pack(f[r][x][2] * up, f[r][x][3] * up))
+                            asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(d), "r"(pack(f[x][0] * up, f[x][1] * up)),
+                                         "r"(pack(f[x][2] * up, f[x][3] * up))
                                          : "memory");
                         }
                 }
@@ -327,156 +347,177 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
         const int hi_min = __reduce_min_sync(0xffffffffu, row >= 0 ? hi : 0x7fffffff);
         const bool cap = a.at.softcap > 0.0f;
         const float inv_cap2 = cap ? 2.0f * 1.4426950408889634f / a.at.softcap : 0.0f;
-        float m = -INFINITY, vpow = 0.0f;  // maximum in base 2
-        F2 l = f2(0.0f, 0.0f);
+        // ---- fragments: this lane's four rows (of the warp's 32) are g + 8 k, its columns 8 i + 2 t and the next
+        const int g = lane >> 2, t = lane & 3;
+        int flo[4], fhi[4];
+        float fq[4], ref[4], vpow = 0.0f;  // ref: base 2; -infinity until the row has seen a position
+        F2 l[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            flo[k] = __shfl_sync(0xffffffffu, lo, g + 8 * k);
+            fhi[k] = __shfl_sync(0xffffffffu, hi, g + 8 * k);
+            fq[k] = __shfl_sync(0xffffffffu, qf, g + 8 * k);
+            ref[k] = -INFINITY;
+            l[k] = f2(0.0f, 0.0f);
+        }
         bool ok = tile < nact;
-        // The sums so far and `done` 32-column pieces of this half's weights, scaled by f: after the products
-        // that add to O (through half `half` of unit `unit`; -1: none yet) are complete.
-        auto rescale = [&](int unit, int half, int first, int done, float f, float fo) {
-            l = mul2(l, f2(f, f));
-            tmem_st_wait();
-            if (unit >= 0) {
-                ok = wait(W::B_O + tile * UNP + half, unit & 1);
-                if (!(ok = __all_sync(0xffffffffu, ok))) return;
-                fence_after();
-                const F2 fo2 = f2(fo, fo);
+        // O times f (lane = row), once the products that add to it (through half `half` of unit `unit`) are complete.
+        auto rescale_o = [&](int unit, int half, float f) {
+            ok = wait(W::B_O + tile * UNP + half, unit & 1);
+            if (!(ok = __all_sync(0xffffffffu, ok))) return;
+            fence_after();
+            const F2 ff = f2(f, f);
 #pragma unroll 1
-                for (int c = 0; c < D / 32; c++) {
-                    uint32_t v[32];
-                    tmem_ld32(tm + W::C_O + 32 * c, v);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        float p, q;
-                        un2(mul2(f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), fo2), p, q);
-                        v[j] = __float_as_uint(p);
-                        v[j + 1] = __float_as_uint(q);
-                    }
-                    tmem_st16(tm + W::C_O + 32 * c, v);
-                    tmem_st16(tm + W::C_O + 32 * c + 16, v + 16);
-                }
-            }
-            if (done) {
-                uint32_t v[16];
-                tmem_ld16(tm + W::C_S + 16 * first, v);
+            for (int c = 0; c < D / 32; c++) {
+                uint32_t v[32];
+                tmem_ld32(tm + W::C_O + 32 * c, v);
                 tmem_ld_wait();
-                const uint32_t h = pack(f, f);
 #pragma unroll
-                for (int j = 0; j < 16; j++) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(v[j]) : "r"(h));
-                tmem_st16(tm + W::C_S + 16 * first, v);
+                for (int j = 0; j < 32; j += 2) {
+                    float p, q;
+                    un2(mul2(f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), ff), p, q);
+                    v[j] = __float_as_uint(p);
+                    v[j + 1] = __float_as_uint(q);
+                }
+                tmem_st16(tm + W::C_O + 32 * c, v);
+                tmem_st16(tm + W::C_O + 32 * c + 16, v + 16);
             }
             tmem_st_wait();
         };
-        // One unit; PLAIN: every row of the warp sees every position and there is no cap.
-        auto unit = [&](int i, auto plain) {
-            constexpr bool PLAIN = decltype(plain)::value;
-            const int st = i % STAGES, t0 = u0 * KVQ_PAGE + i * UN;
-            const float *ks = (const float *)(smem + W::OFF_SC + st * W::SC_STAGE), *vs = ks + UN, *ex = vs + UN;
-            const F2 qf2 = f2(qf, qf);
-            vpow = ex[1];
-            if (i > 0 && ex[0] != 1.0f) {  // the values' unit rose: O follows (every row alike)
-                rescale(i - 1, UNP - 1, 0, 0, 1.0f, ex[0]);
+        auto hand_over = [&](int half, const uint32_t (&p)[2][16]) {  // 64 positions' weights, over scores that were read
+            tmem_st_frag(tm + W::C_S + 32 * half, p[0]);
+            tmem_st_frag(tm + (16u << 16) + W::C_S + 32 * half, p[1]);
+            tmem_st_wait();
+            fence_before();
+            bar_arrive(bars + 8 * (W::B_P + tile * UNP + half));
+        };
+        // Half a unit whose rows see every position, without a cap: false (and nothing done) when a weight
+        // reaches 2 and the reference has to rise.
+        auto plain_half = [&](const float *ks, const float *vs, int half) -> bool {
+            uint32_t s[2][32], p[2][16], any = 0;
+            tmem_ld_frag(tm + W::C_S + 64 * half, s[0]);
+            tmem_ld_frag(tm + (16u << 16) + W::C_S + 64 * half, s[1]);
+            F2 q2[4], off[4], sum[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                q2[k] = f2(fq[k], fq[k]);
+                off[k] = f2(-ref[k], -ref[k]);
+                sum[k] = f2(0.0f, 0.0f);
+            }
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float2 kf = *(const float2 *)(ks + 64 * half + 8 * i + 2 * t), vf = *(const float2 *)(vs + 64 * half + 8 * i + 2 * t);
+                const F2 k2 = f2(kf.x, kf.y), v2 = f2(vf.x, vf.y);
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t *x = s[k >> 1] + 4 * i + 2 * (k & 1);
+                    float y, z;
+                    un2(fma2(f2(__uint_as_float(x[0]), __uint_as_float(x[1])), mul2(k2, q2[k]), off[k]), y, z);
+                    const F2 e = f2(ex2(y), ex2(z));
+                    sum[k] = add2(sum[k], e);
+                    un2(mul2(e, v2), y, z);
+                    any |= p[k >> 1][2 * i + (k & 1)] = pack(y, z);
+                }
+            }
+            if (__any_sync(0xffffffffu, (any & 0x40004000u) != 0)) return false;  // an exponent bit: 2 or more (or a NaN)
+#pragma unroll
+            for (int k = 0; k < 4; k++) l[k] = add2(l[k], sum[k]);
+            hand_over(half, p);
+            return true;
+        };
+        // The general half: masks, cap, and the search for the rows' maxima.
+        auto full_half = [&](int i, const float *ks, const float *vs, bool bad, int half) {
+            const int j0 = u0 * KVQ_PAGE + i * UN + 64 * half + 2 * t;
+            uint32_t s[32], p[2][16];
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            auto score = [&](int k, int c, int e) {  // row k, columns 8 c + 2 t + e: -infinity where it sees nothing
+                const int j = j0 + 8 * c + e;
+                const float x = __uint_as_float(s[4 * c + 2 * (k & 1) + e]) * ks[64 * half + 8 * c + 2 * t + e];
+                return bad || j < flo[k] || j > fhi[k] || j >= len ? -INFINITY : x;
+            };
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                tmem_ld_frag(tm + ((uint32_t)(16 * h) << 16) + W::C_S + 64 * half, s);
+                tmem_ld_wait();
+#pragma unroll
+                for (int r = 0; r < 2; r++)
+#pragma unroll
+                    for (int c = 0; c < 8; c++) top[2 * h + r] = fmaxf(top[2 * h + r], fmaxf(score(2 * h + r, c, 0), score(2 * h + r, c, 1)));
+            }
+            float f[4];
+            bool moved = false;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
+                top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
+                f[k] = 1.0f;
+                if (top[k] != -INFINITY) {
+                    float x = top[k] * fq[k];
+                    if (cap) x = capped<false>(x, a.at.softcap, inv_cap2) * 1.4426950408889634f;  // monotonic
+                    x += HEAD;
+                    if (x > ref[k]) {
+                        // by a power of two, which the factor then is
+                        const float to = ref[k] == -INFINITY ? x : ref[k] + ceilf(x - ref[k]);
+                        f[k] = ex2(ref[k] - to);
+                        ref[k] = to;
+                        moved = true;
+                    }
+                }
+                l[k] = mul2(l[k], f2(f[k], f[k]));
+            }
+            if ((i > 0 || half > 0) && __any_sync(0xffffffffu, moved)) {
+                float mine = 1.0f;  // of the row that is this lane
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float x = __shfl_sync(0xffffffffu, f[k], (lane & 7) * 4);
+                    if (lane >> 3 == k) mine = x;
+                }
+                // O holds the units before this one, and this one's first half once that is handed over
+                rescale_o(half > 0 ? i : i - 1, half > 0 ? half - 1 : UNP - 1, mine);
                 if (!ok) return;
             }
-#pragma unroll 1
-            for (int c = 0; c < UN / 32; c++) {
-                F2 x[16];
-                {
-                    uint32_t s[32];
-                    tmem_ld32(tm + W::C_S + 32 * c, s);
-                    tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 16; j += 2) {  // s times the keys' scales
-                        const float4 k4 = *(const float4 *)(ks + 32 * c + 2 * j);
-                        x[j] = mul2(f2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), f2(k4.x, k4.y));
-                        x[j + 1] = mul2(f2(__uint_as_float(s[2 * j + 2]), __uint_as_float(s[2 * j + 3])), f2(k4.z, k4.w));
-                    }
-                }
-                if (!PLAIN) {
-                    const int t = t0 + 32 * c;
-                    const bool bad = ex[2 + 32 * c / KVQ_PAGE] != 0.0f;
+            for (int h = 0; h < 2; h++) {
+                tmem_ld_frag(tm + ((uint32_t)(16 * h) << 16) + W::C_S + 64 * half, s);
+                tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        float p, q;
-                        un2(x[j], p, q);
-                        if (bad || t + 2 * j < lo || t + 2 * j > hi || t + 2 * j >= len) p = -INFINITY;
-                        if (bad || t + 2 * j + 1 < lo || t + 2 * j + 1 > hi || t + 2 * j + 1 >= len) q = -INFINITY;
-                        x[j] = f2(p, q);
-                    }
-                }
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                for (int c = 0; c < 8; c++)
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    float p, q;
-                    un2(x[j], p, q);
-                    mx[j & 3] = max3(mx[j & 3], p, q);
-                }
-                const float top0 = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
-                float top = top0 == -INFINITY ? -INFINITY : top0 * qf;
-                if (!PLAIN && cap && top0 != -INFINITY) top = capped<false>(top, a.at.softcap, inv_cap2) * 1.4426950408889634f;  // monotonic
-                const bool raise = top > m + RAISE || (m == -INFINITY && top > -INFINITY);
-                if (__any_sync(0xffffffffu, raise)) {
-                    // by a power of two, which every factor then is: the rescaled weights stay exact
-                    const float to = m == -INFINITY ? top : m + ceilf(top - m), f = raise ? ex2(m - to) : 1.0f;
-                    if (raise) m = to;
-                    // O holds the units before this one, and this one's first half once that is handed over
-                    rescale(c < 2 ? i - 1 : i, c < 2 ? UNP - 1 : 0, c - 1, c & 1, f, f);
-                    if (!ok) return;
-                }
-                const float off = m == -INFINITY ? 0.0f : m;
-                const F2 off2 = f2(-off, -off);
-                uint32_t p[16];
-                F2 l2[2] = {l, f2(0.0f, 0.0f)};
+                    for (int r = 0; r < 2; r++) {
+                        const int k = 2 * h + r;
+                        float w[2], y[2];
 #pragma unroll
-                for (int j = 0; j < 16; j += 2) {
-                    const float4 v4 = *(const float4 *)(vs + 32 * c + 2 * j);
-                    const F2 v2[2] = {f2(v4.x, v4.y), f2(v4.z, v4.w)};
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        float y, z;
-                        if (!PLAIN && cap) {
-                            un2(mul2(x[j + h], qf2), y, z);
-                            y = fmaf(capped<false>(y, a.at.softcap, inv_cap2), 1.4426950408889634f, -off);
-                            z = fmaf(capped<false>(z, a.at.softcap, inv_cap2), 1.4426950408889634f, -off);
-                        } else {
-                            un2(fma2(x[j + h], qf2, off2), y, z);
+                        for (int e = 0; e < 2; e++) {
+                            const float x = score(k, c, e), off = ref[k] == -INFINITY ? 0.0f : ref[k];
+                            const float z = cap ? capped<false>(x * fq[k], a.at.softcap, inv_cap2) * 1.4426950408889634f : x * fq[k];
+                            y[e] = ex2(z - off);
+                            w[e] = y[e] * vs[64 * half + 8 * c + 2 * t + e];
+                            if (x == -INFINITY) y[e] = w[e] = 0.0f;  // whatever an unseen position holds
                         }
-                        y = ex2(y);
-                        z = ex2(z);
-                        float wy, wz;
-                        if (!PLAIN) {  // whatever an unseen position holds
-                            float xy, xz;
-                            un2(x[j + h], xy, xz);
-                            if (xy == -INFINITY) y = 0.0f;
-                            if (xz == -INFINITY) z = 0.0f;
-                            un2(mul2(f2(y, z), v2[h]), wy, wz);
-                            if (xy == -INFINITY) wy = 0.0f;
-                            if (xz == -INFINITY) wz = 0.0f;
-                        } else {
-                            un2(mul2(f2(y, z), v2[h]), wy, wz);
-                        }
-                        l2[h] = add2(l2[h], f2(y, z));
-                        p[j + h] = pack(wy, wz);
+                        l[k] = add2(l[k], f2(y[0], y[1]));
+                        p[h][2 * c + r] = pack(w[0], w[1]);
                     }
-                }
-                l = add2(l2[0], l2[1]);
-                tmem_st16(tm + W::C_S + 16 * c, p);  // over scores that were read
-                if (c & 1) {                          // 64 positions' weights are complete
-                    tmem_st_wait();
-                    fence_before();
-                    bar_arrive(bars + 8 * (W::B_P + tile * UNP + c / 2));
-                }
             }
+            hand_over(half, p);
         };
         for (int i = 0; i < n && ok; i++) {
             const int st = i % STAGES;
             ok = wait(W::B_S + tile, i & 1) && wait(W::B_FULL + st, (i / STAGES) & 1);
             if (!(ok = __all_sync(0xffffffffu, ok))) break;
             fence_after();
-            const float *ex = (const float *)(smem + W::OFF_SC + st * W::SC_STAGE) + 2 * UN;
+            const float *ks = (const float *)(smem + W::OFF_SC + st * W::SC_STAGE), *vs = ks + UN, *ex = vs + UN;
             const int t0 = u0 * KVQ_PAGE + i * UN;
-            if (!cap && t0 >= lo_max && t0 + UN - 1 <= hi_min && ex[2] == 0.0f && ex[3] == 0.0f) unit(i, std::true_type{});
-            else unit(i, std::false_type{});
+            vpow = ex[1];
+            if (i > 0 && ex[0] != 1.0f) {  // the values' unit rose: O follows (every row alike)
+                rescale_o(i - 1, UNP - 1, ex[0]);
+                if (!ok) break;
+            }
+            bool plain = !cap && t0 >= lo_max && t0 + UN - 1 <= hi_min && ex[2] == 0.0f && ex[3] == 0.0f;
+            plain = __all_sync(0xffffffffu, plain && fminf(fminf(ref[0], ref[1]), fminf(ref[2], ref[3])) > -INFINITY);
+#pragma unroll 1
+            for (int half = 0; half < UNP && ok; half++)
+                if (!plain || !plain_half(ks, vs, half)) full_half(i, ks, vs, ex[2 + half] != 0.0f, half);
         }
         if (ok && n > 0) {
             ok = wait(W::B_O + tile * UNP + UNP - 1, (n - 1) & 1);
@@ -499,40 +540,52 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
 #pragma unroll
                 for (int j = 0; j < 32; j++) tr[lane * 32 + (j ^ lane)] = __uint_as_float(v[j]) * vpow;
                 __syncwarp();
-#pragma unroll 16
-                for (int r = 0; r < 32; r++) {
-                    const int64_t to = s_at[warp * 32 + r];
-                    const float o = tr[r * 32 + (lane ^ r)];
-                    if (to >= 0) a.part_o[to + 32 * c + lane] = o;
+#pragma unroll 1
+                for (int r0 = 0; r0 < 32; r0 += 8) {  // read first: the compiler keeps loads behind stores
+                    float o[8];
+                    int64_t to[8];
+#pragma unroll
+                    for (int r = 0; r < 8; r++) {
+                        o[r] = tr[(r0 + r) * 32 + (lane ^ (r0 + r))];
+                        to[r] = s_at[warp * 32 + r0 + r];
+                    }
+#pragma unroll
+                    for (int r = 0; r < 8; r++)
+                        if (to[r] >= 0) a.part_o[to[r] + 32 * c + lane] = o[r];
                 }
             }
         }
-        float la, lb;
-        un2(l, la, lb);
-        if (row >= 0) a.part_ml[at] = ok ? make_float2(m, la + lb) : make_float2(0.0f, NAN);
+        // a row's sum lies in four lanes, its reference in each of them
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            float x, y;
+            un2(l[k], x, y);
+            x += y;
+            x += __shfl_xor_sync(0xffffffffu, x, 1);
+            x += __shfl_xor_sync(0xffffffffu, x, 2);
+            const int64_t to = s_at[warp * 32 + g + 8 * k];
+            if (t == 0 && to >= 0) a.part_ml[to / D] = ok ? make_float2(ref[k], x) : make_float2(0.0f, NAN);
+        }
     } else if (warp < SOFT / 32 + 4) {
         // ------------------------------------------------------------ codes to operands
         const int dt = tid - SOFT, dw = dt >> 5;
         // a page's K or V: 4 D pieces of 16 codes, T per thread, a warp's at consecutive addresses
         constexpr int T = D / 32;
         struct Codes {
-            uint4 k[T], v[T];
+            uint4 c[T];
         };
         auto page_of = [&](int u) { return u < u1 ? __ldg(sg.pages + u) : -1; };
         auto none = [&](int page) { return (unsigned)page >= (unsigned)a.pool.n_pages; };
-        auto load = [&](int page, Codes &c) {
+        auto load = [&](int page, bool v, Codes &x) {
             if (none(page)) {
 #pragma unroll
-                for (int i = 0; i < T; i++) c.k[i] = c.v[i] = make_uint4(0, 0, 0, 0);
+                for (int i = 0; i < T; i++) x.c[i] = make_uint4(0, 0, 0, 0);
                 return;
             }
-            const int64_t at = (((int64_t)page * Hk + sg.kvh) * KVQ_PAGE) * D + dt * 16;
-            const uint8_t *k = (const uint8_t *)a.pool.k + at, *v = (const uint8_t *)a.pool.v + at;
+            const uint8_t *p = (const uint8_t *)(v ? a.pool.v : a.pool.k) + (((int64_t)page * Hk + sg.kvh) * KVQ_PAGE) * D + dt * 16;
 #pragma unroll
-            for (int i = 0; i < T; i++) {
-                c.k[i] = ldg128(k + 2048 * i);
-                c.v[i] = ldg128(v + 2048 * i);
-            }
+            for (int i = 0; i < T; i++) x.c[i] = ldg128(p + 2048 * i);
         };
         // a unit's scales: warp 0 V's, warp 1 K's; lane: positions lane, lane + 32, ...
         auto load_scales = [&](int page0, int page1, float (&c)[2 * UNP]) {
@@ -577,31 +630,31 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                 for (int x = 0; x < 2 * UNP; x++) ks[lane + 32 * x] = c[x];
             }
         };
-        // page h of the segment's share: half h % UNP of unit h / UNP
-        auto convert = [&](int h, const Codes &cur) {
-            const uint32_t d = base + h / UNP % STAGES * W::STAGE + h % UNP * KVQ_PAGE * W::ROW;
+        // K or V of page h of the segment's share: half h % UNP of unit h / UNP
+        auto convert = [&](int h, bool v, const Codes &x) {
+            const uint32_t d = base + h / UNP % STAGES * W::STAGE + h % UNP * KVQ_PAGE * W::ROW + (v ? W::K_BYTES : 0u);
 #pragma unroll
             for (int i = 0; i < T; i++) {
                 // piece t: position r, codes 16 ch ..: two operand pieces of 8.  Lanes of the upper half of a
                 // 128-code row write them in the other order, so that eight lanes meet eight banks.
                 const int t = dt + 128 * i, ch = t % (D / 16), r = t / (D / 16), pc = (ch & 3) * 2, swap = (ch >> 2) & 1;
                 const uint32_t to = d + (ch >> 2) * W::K_BLK + r * W::ROW;
-                const uint32_t o0 = to + ((pc + swap) ^ (r & 7)) * 16, o1 = to + ((pc + 1 - swap) ^ (r & 7)) * 16;
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const uint4 c = x ? cur.v[i] : cur.k[i];
-                    const uint32_t w[4] = {(swap ? c.z : c.x) ^ code_flip<FMT>(), (swap ? c.w : c.y) ^ code_flip<FMT>(),
-                                           (swap ? c.x : c.z) ^ code_flip<FMT>(), (swap ? c.y : c.w) ^ code_flip<FMT>()};
-                    sts128(o0 + x * W::K_BYTES, codes2<FMT, 0, 1>(w[0]), codes2<FMT, 2, 3>(w[0]), codes2<FMT, 0, 1>(w[1]), codes2<FMT, 2, 3>(w[1]));
-                    sts128(o1 + x * W::K_BYTES, codes2<FMT, 0, 1>(w[2]), codes2<FMT, 2, 3>(w[2]), codes2<FMT, 0, 1>(w[3]), codes2<FMT, 2, 3>(w[3]));
-                }
+                const uint4 c = x.c[i];
+                const uint32_t w[4] = {(swap ? c.z : c.x) ^ code_flip<FMT>(), (swap ? c.w : c.y) ^ code_flip<FMT>(),
+                                       (swap ? c.x : c.z) ^ code_flip<FMT>(), (swap ? c.y : c.w) ^ code_flip<FMT>()};
+                sts128(to + ((pc + swap) ^ (r & 7)) * 16, codes2<FMT, 0, 1>(w[0]), codes2<FMT, 2, 3>(w[0]), codes2<FMT, 0, 1>(w[1]),
+                       codes2<FMT, 2, 3>(w[1]));
+                sts128(to + ((pc + 1 - swap) ^ (r & 7)) * 16, codes2<FMT, 0, 1>(w[2]), codes2<FMT, 2, 3>(w[2]),
+                       codes2<FMT, 0, 1>(w[3]), codes2<FMT, 2, 3>(w[3]));
             }
         };
-        // two sets of registers in turn (a copy from one to the other would wait for the loads)
-        Codes c0, c1;
+        // four sets of registers in turn, three loads ahead (a copy between sets would wait for them)
+        Codes k0, v0, k1, v1;
         float sc[2 * UNP];
-        int p0 = page_of(u0), p1 = page_of(u0 + 1);  // this page and the next
-        load(p0, c0);
+        int p0 = page_of(u0), p1 = page_of(u0 + 1), p2 = page_of(u0 + 2), p3 = page_of(u0 + 3);
+        load(p0, false, k0);
+        load(p0, true, v0);
+        load(p1, false, k1);
         load_scales(p0, p1, sc);
         __syncthreads();
         auto slot = [&](int i) {
@@ -614,38 +667,46 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             bar_arrive(bars + 8 * (W::B_FULL + i % STAGES));
         };
         for (int h = 0; h < n * UNP && ok; h += 2) {  // two pages a round: one unit, or two of one page
-            const int i = h / UNP, p2 = page_of(u0 + h + 2), p3 = page_of(u0 + h + 3);
-            load(p1, c1);
+            const int i = h / UNP, p4 = page_of(u0 + h + 4), p5 = page_of(u0 + h + 5);
+            load(p1, true, v1);
             if (!slot(i)) break;
             put_scales(i, p0, p1, sc);
             if (UNP == 2) load_scales(p2, p3, sc);
             else load_scales(p1, p1, sc);
-            convert(h, c0);
+            convert(h, false, k0);
+            load(p2, false, k0);
+            convert(h, true, v0);
             if (UNP == 1) {
                 done(i);
                 if (h + 1 >= n) break;
-                load(p2, c0);
                 if (!slot(i + 1)) break;
                 put_scales(i + 1, p1, p1, sc);
                 load_scales(p2, p2, sc);
-            } else {
-                load(p2, c0);
             }
-            convert(h + 1, c1);
+            load(p2, true, v0);
+            convert(h + 1, false, k1);
+            load(p3, false, k1);
+            convert(h + 1, true, v1);
             done(UNP == 1 ? i + 1 : i);
             p0 = p2;
             p1 = p3;
+            p2 = p4;
+            p3 = p5;
         }
     } else {
         // ------------------------------------------------------------ products
+        if (W::TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         __syncthreads();
-        if (lane == 0 && n > 0) {
+        if (warp == SOFT / 32 + 4 && lane == 0 && n > 0) {
             fence_after();
+            // descriptors differ in their address field (units of 16 bytes): one addition each
+            const uint64_t qd = sdesc(base + W::OFF_Q), kd = sdesc(base), vd = sdesc(base + W::K_BYTES, W::K_BLK);
             auto qk = [&](int t, int st) {
-                const uint32_t q = base + W::OFF_Q + t * W::Q_BYTES, k = base + st * W::STAGE, d = tmem + t * W::TILE_COLS + W::C_S;
+                const uint64_t q = qd + t * (W::Q_BYTES / 16), k = kd + st * (W::STAGE / 16);
+                const uint32_t d = tmem + t * W::TILE_COLS + W::C_S;
 #pragma unroll
                 for (int kk = 0; kk < D / 16; kk++)
-                    umma_ss<UN>(d, sdesc(q + kk / 4 * W::Q_BLK + kk % 4 * 32), sdesc(k + kk / 4 * W::K_BLK + kk % 4 * 32), kk != 0);
+                    umma_ss<UN>(d, q + (kk / 4 * W::Q_BLK + kk % 4 * 32) / 16, k + (kk / 4 * W::K_BLK + kk % 4 * 32) / 16, kk != 0);
                 umma_commit(bars + 8 * (W::B_S + t));
             };
             bool ok = wait(W::B_FULL, 0);
@@ -654,7 +715,8 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             for (int i = 0; i < n && ok; i++) {
                 const int st = i % STAGES, nx = (i + 1) % STAGES;
                 for (int t = 0; t < nact; t++) {
-                    const uint32_t v = base + st * W::STAGE + W::K_BYTES, tm = tmem + t * W::TILE_COLS;
+                    const uint64_t v = vd + st * (W::STAGE / 16);
+                    const uint32_t tm = tmem + t * W::TILE_COLS;
 #pragma unroll
                     for (int hf = 0; hf < UNP && ok; hf++) {
                         if (!(ok = wait(W::B_P + t * UNP + hf, i & 1))) break;
@@ -662,7 +724,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
 #pragma unroll
                         for (int kk = 0; kk < KVQ_PAGE / 16; kk++)
                             umma_ts<D>(tm + W::C_O, tm + W::C_S + 32 * hf + 8 * kk,
-                                       sdesc(v + (hf * 4 + kk) * 2 * W::GROUP, W::K_BLK), i != 0 || hf != 0 || kk != 0);
+                                       v + (hf * 4 + kk) * 2 * W::GROUP / 16, i != 0 || hf != 0 || kk != 0);
                         umma_commit(bars + 8 * (W::B_O + t * UNP + hf));
                     }
                     if (!ok) break;
