@@ -273,10 +273,10 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
     const int u1 = min((sg.chunk + 1) * sg.ch, hi_max < 0 ? 0 : hi_max / KVQ_PAGE + 1), n = (max(u1 - u0, 0) + UNP - 1) / UNP;
 
     // Registers: 16 warps start with 128 each (2048 warp-registers in all); the row warps hold two pieces of
-    // scores and need more: 8 * 168 + 4 * 128 + 4 * 40 = 2016.
+    // scores and need more: 8 * 152 + 4 * 128 + 4 * 80 = 2048.
     if (warp < SOFT / 32) {
         // ------------------------------------------------------------ a row per thread
-        if (W::TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        if (W::TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
         const int tile = warp >> 2, head = sg.kvh * G + (row_first + tid) % G;
         const uint32_t tm = tmem + tile * W::TILE_COLS + ((uint32_t)(32 * (warp & 3)) << 16);
         // the queries, scaled by a power of two each, as an operand (zeros for rows that do not exist): a row
@@ -343,7 +343,9 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
         const float qf = fabsf(a.at.scale) * code_unit<FMT>() * (a.at.softcap > 0.0f ? 1.0f : 1.4426950408889634f) * pow2(-e);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
-        const int lo_max = __reduce_max_sync(0xffffffffu, row >= 0 ? lo : 0);
+        // this warp's rows: positions that all of them see, and that any does
+        const int lo_max = __reduce_max_sync(0xffffffffu, row >= 0 ? lo : 0), hi_end = s_hi[warp];
+        lo_min = s_lo[warp];
         const int hi_min = __reduce_min_sync(0xffffffffu, row >= 0 ? hi : 0x7fffffff);
         const bool cap = a.at.softcap > 0.0f;
         const float inv_cap2 = cap ? 2.0f * 1.4426950408889634f / a.at.softcap : 0.0f;
@@ -426,24 +428,30 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             hand_over(half, p);
             return true;
         };
-        // The general half: masks, cap, and the search for the rows' maxima.
-        auto full_half = [&](int i, const float *ks, const float *vs, bool bad, int half) {
+        // The search for the rows' maxima over half a unit, and the references raised where they stand less than
+        // HEAD above.  MASKED: scores of positions that a row does not see do not count.
+        auto search = [&](int i, const float *ks, int half, auto masked) {
+            constexpr bool MASKED = decltype(masked)::value;
             const int j0 = u0 * KVQ_PAGE + i * UN + 64 * half + 2 * t;
-            uint32_t s[32], p[2][16];
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            auto score = [&](int k, int c, int e) {  // row k, columns 8 c + 2 t + e: -infinity where it sees nothing
-                const int j = j0 + 8 * c + e;
-                const float x = __uint_as_float(s[4 * c + 2 * (k & 1) + e]) * ks[64 * half + 8 * c + 2 * t + e];
-                return bad || j < flo[k] || j > fhi[k] || j >= len ? -INFINITY : x;
-            };
 #pragma unroll
             for (int h = 0; h < 2; h++) {
+                uint32_t s[32];
                 tmem_ld_frag(tm + ((uint32_t)(16 * h) << 16) + W::C_S + 64 * half, s);
                 tmem_ld_wait();
 #pragma unroll
-                for (int r = 0; r < 2; r++)
+                for (int c = 0; c < 8; c++) {
+                    const float2 kf = *(const float2 *)(ks + 64 * half + 8 * c + 2 * t);
+                    const int j = j0 + 8 * c;
 #pragma unroll
-                    for (int c = 0; c < 8; c++) top[2 * h + r] = fmaxf(top[2 * h + r], fmaxf(score(2 * h + r, c, 0), score(2 * h + r, c, 1)));
+                    for (int r = 0; r < 2; r++) {
+                        const int k = 2 * h + r;
+                        float x = __uint_as_float(s[4 * c + 2 * r]) * kf.x, y = __uint_as_float(s[4 * c + 2 * r + 1]) * kf.y;
+                        if (MASKED && (j < flo[k] || j > fhi[k])) x = -INFINITY;
+                        if (MASKED && (j + 1 < flo[k] || j + 1 > fhi[k])) y = -INFINITY;
+                        top[k] = fmaxf(top[k], fmaxf(x, y));
+                    }
+                }
             }
             float f[4];
             bool moved = false;
@@ -475,29 +483,36 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                 }
                 // O holds the units before this one, and this one's first half once that is handed over
                 rescale_o(half > 0 ? i : i - 1, half > 0 ? half - 1 : UNP - 1, mine);
-                if (!ok) return;
             }
+        };
+        // The weights of half a unit, with masks and cap.
+        auto masked_half = [&](int i, const float *ks, const float *vs, int half) {
+            const int j0 = u0 * KVQ_PAGE + i * UN + 64 * half + 2 * t;
+            uint32_t p[2][16];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
+                uint32_t s[32];
                 tmem_ld_frag(tm + ((uint32_t)(16 * h) << 16) + W::C_S + 64 * half, s);
                 tmem_ld_wait();
 #pragma unroll
-                for (int c = 0; c < 8; c++)
+                for (int c = 0; c < 8; c++) {
+                    const float2 kf = *(const float2 *)(ks + 64 * half + 8 * c + 2 * t), vf = *(const float2 *)(vs + 64 * half + 8 * c + 2 * t);
 #pragma unroll
                     for (int r = 0; r < 2; r++) {
-                        const int k = 2 * h + r;
-                        float w[2], y[2];
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const float x = score(k, c, e), off = ref[k] == -INFINITY ? 0.0f : ref[k];
-                            const float z = cap ? capped<false>(x * fq[k], a.at.softcap, inv_cap2) * 1.4426950408889634f : x * fq[k];
-                            y[e] = ex2(z - off);
-                            w[e] = y[e] * vs[64 * half + 8 * c + 2 * t + e];
-                            if (x == -INFINITY) y[e] = w[e] = 0.0f;  // whatever an unseen position holds
+                        const int k = 2 * h + r, j = j0 + 8 * c;
+                        const float off = ref[k] == -INFINITY ? 0.0f : ref[k];
+                        float x = __uint_as_float(s[4 * c + 2 * r]) * kf.x * fq[k], y = __uint_as_float(s[4 * c + 2 * r + 1]) * kf.y * fq[k];
+                        if (cap) {
+                            x = capped<false>(x, a.at.softcap, inv_cap2) * 1.4426950408889634f;
+                            y = capped<false>(y, a.at.softcap, inv_cap2) * 1.4426950408889634f;
                         }
-                        l[k] = add2(l[k], f2(y[0], y[1]));
-                        p[h][2 * c + r] = pack(w[0], w[1]);
+                        x = ex2(x - off);
+                        y = ex2(y - off);
+                        const bool gx = j < flo[k] || j > fhi[k], gy = j + 1 < flo[k] || j + 1 > fhi[k];
+                        l[k] = add2(l[k], f2(gx ? 0.0f : x, gy ? 0.0f : y));
+                        p[h][2 * c + r] = pack(gx ? 0.0f : x * vf.x, gy ? 0.0f : y * vf.y);  // whatever an unseen position holds
                     }
+                }
             }
             hand_over(half, p);
         };
@@ -513,11 +528,22 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                 rescale_o(i - 1, UNP - 1, ex[0]);
                 if (!ok) break;
             }
-            bool plain = !cap && t0 >= lo_max && t0 + UN - 1 <= hi_min && ex[2] == 0.0f && ex[3] == 0.0f;
-            plain = __all_sync(0xffffffffu, plain && fminf(fminf(ref[0], ref[1]), fminf(ref[2], ref[3])) > -INFINITY);
+            const bool known = __all_sync(0xffffffffu, fminf(fminf(ref[0], ref[1]), fminf(ref[2], ref[3])) > -INFINITY);
 #pragma unroll 1
-            for (int half = 0; half < UNP && ok; half++)
-                if (!plain || !plain_half(ks, vs, half)) full_half(i, ks, vs, ex[2 + half] != 0.0f, half);
+            for (int half = 0; half < UNP && ok; half++) {
+                const int p0 = t0 + 64 * half;
+                if (ex[2 + half] != 0.0f || p0 > hi_end || p0 + KVQ_PAGE <= lo_min) {  // nothing for this warp's rows
+                    const uint32_t zero[2][16] = {};
+                    hand_over(half, zero);
+                } else if (!cap && p0 >= lo_max && p0 + KVQ_PAGE - 1 <= hi_min) {  // everything
+                    if ((known || half > 0) && plain_half(ks, vs, half)) continue;
+                    search(i, ks, half, std::false_type{});
+                    if (ok && !plain_half(ks, vs, half)) masked_half(i, ks, vs, half);  // (a NaN stays one)
+                } else {
+                    search(i, ks, half, std::true_type{});
+                    if (ok) masked_half(i, ks, vs, half);
+                }
+            }
         }
         if (ok && n > 0) {
             ok = wait(W::B_O + tile * UNP + UNP - 1, (n - 1) & 1);
@@ -695,7 +721,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
         }
     } else {
         // ------------------------------------------------------------ products
-        if (W::TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (W::TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         __syncthreads();
         if (warp == SOFT / 32 + 4 && lane == 0 && n > 0) {
             fence_after();
