@@ -15,15 +15,19 @@
 // its rows -- times kv heads, row tiles and chunks of pages.  The prefix is read once per row tile of
 // the whole batch, not once per sequence.  Each CTA leaves a partial (m, l, O) of its chunk; a second kernel
 // (programmatic dependent launch) joins a row's partials in chunk order.  A call with one chunk in
-// all writes its output directly.
+// all writes its output directly.  Segments with many rows go to kvq_attn_tc.cu.
 //
-// Bound: HBM (the codes) while a kv head has few rows.  Inside a CTA each of four warps streams its own
-// units of LT positions (cp.async, one K and one V slot in flight per warp, no block barrier in
-// the loop) and forms S^T = K Q^T and O^T = V^T P^T with mma.m16n8k16: positions and head dimensions
-// take the 16-wide side and the rows the 8-wide side, so 4 rows (one token of a group of 4 heads) waste
-// half a tile rather than three quarters.  The order of k inside a tile is free as long as both
-// operands agree; it is chosen so that a lane's K bytes are 16 consecutive ones, and its V bytes four
-// positions of 16 (4, 8) consecutive dimensions, which shuffle into A fragments by byte permutes.
+// This kernel, for few rows per kv head, is bound by HBM (the codes), and below that by instructions: the
+// codes of a page become fp16 fragments with about 1.3 instructions a code.  Four warps share a page of 64
+// positions.  For S^T = K Q^T (mma.m16n8k16; positions and head dimensions take the 16-wide side, rows
+// the 8-wide side, so one token of a group of 4 heads wastes half a tile, not three quarters) each
+// warp has 16 positions; the weights pass through shared memory, one barrier per page; and for O^T = V^T P^T
+// each warp has 32 head dimensions and all positions, so that O needs a quarter of the registers (many
+// CTAs per SM hide the latencies) and no joining of warps at the end.  The order of k inside a tile is free
+// as long as both operands agree; it is chosen so that a lane's K bytes are 16 consecutive ones, and its V
+// bytes four positions of four consecutive dimensions, which byte permutes turn into fragments.
+// A row's weights are taken relative to a reference above its maximum at the time; while no weight comes
+// near fp16's limit no maximum is searched, and the barrier's vote tells all warps when one does.
 #include <algorithm>
 
 #include "kvq_attn.cuh"
@@ -56,19 +60,17 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a)
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
-// Shapes of the kernel for a head dimension D and NT tiles of 8 rows.
+// Shapes of the kernel for a head dimension D.
 template <int D> struct Shape {
-    static constexpr int LT = D == 256 ? 32 : 64;   // positions of one unit (slot)
-    static constexpr int CPR = D / 16;              // 16-byte pieces of a position's codes
-    static constexpr int SLOT = LT * D;             // bytes of a K or V slot
-    static constexpr int KB = D == 96 ? 8 : 16;     // K bytes a lane takes at once
-    static constexpr int KC = D / (4 * KB);         // such pieces
-    static constexpr int VB = D == 64 ? 8 : D == 96 ? 4 : 16;  // V bytes a lane takes at once
-    static constexpr int VC = D / (8 * VB);
-    static constexpr int MAX_NT = D == 256 ? 2 : D == 128 ? 3 : 4;  // O^T in registers: D / 4 * NT of them
-    static constexpr int QPAD = D == 96 ? 0 : 8;    // halves between query rows against bank conflicts
-    static constexpr int WARP = 2 * SLOT + 2 * LT * 4;  // bytes per warp: K, V and their scales
+    static constexpr int CPR = D / 16;                         // 16-byte pieces of a position's codes
+    static constexpr int SLOT = KVQ_PAGE * D;                  // bytes of a page's K or V
+    static constexpr int KB = D == 96 ? 8 : 16, KC = D / (4 * KB);  // K bytes a lane takes at once; such pieces
+    static constexpr int GPW = D == 256 ? 2 : 1;               // 32-dimension groups of O per warp (64: two warps share one, 96: three have one)
+    static constexpr int MAX_NT = D == 256 ? 4 : 8;
+    static constexpr int QPAD = D == 96 ? 0 : 8;               // halves between query rows against bank conflicts
+    static constexpr int OFF_SC = 4 * SLOT, OFF_Q = OFF_SC + 4 * KVQ_PAGE * 4;  // K 0, K 1, V 0, V 1, scales, queries, weights
 };
+constexpr int PS = 80;  // halves from one row's weights to the next (64 and 16 against bank conflicts)
 // Where 16-byte piece c of position r lies in its slot: chosen so that the lanes of one shared-memory
 // access (K: 8 or 16 lanes on positions a, a + 4, ...; V: on positions 4 i .. 4 i + 3) meet distinct banks.
 template <int D> __device__ __forceinline__ int k_piece(int r, int c)
@@ -119,16 +121,26 @@ __device__ __forceinline__ void store4(void *p, int64_t i, uint32_t type, bool w
     }
 }
 
+// What a row's reference stands above its maximum when it is set (powers of two), and the test that a packed
+// weight has come too near fp16's limit.  One fp16 per weight: 2^6 above, weights of 2 and more (an exponent
+// bit).  hi + lo: 2^4 below, so that lo stays a normal number; 2^13 and more.
+template <bool SPLIT> constexpr float ref_head() { return SPLIT ? -4.0f : 6.0f; }
+template <bool SPLIT> __device__ __forceinline__ uint32_t too_large(uint32_t p)
+{
+    return SPLIT ? ((p & 0x70007000u) + 0x10001000u) & 0x80008000u : p & 0x40004000u;
+}
+
 template <int D, int FMT, int NT, bool SPLIT>
 __global__ void __launch_bounds__(NW * 32) kvq_attn_kernel(const __grid_constant__ AttnArgs a)
 {
     using Sh = Shape<D>;
-    constexpr int LT = Sh::LT, MT = LT / 16, RT = 8 * NT, QS = D + Sh::QPAD, NQ = SPLIT ? 2 : 1;
+    constexpr int RT = 8 * NT, QS = D + Sh::QPAD, NQ = SPLIT ? 2 : 1;
+    constexpr bool QREG = NT * NQ * D / 8 <= 32;  // the query's fragments stay in registers
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float s_qf[RT], s_m[NW][RT], s_l[NW][RT];
-    __shared__ float s_e[NW];
+    __shared__ float s_qf[RT], s_max[NW][RT], s_l[NW][RT], s_vmax[NW];
     __shared__ int s_lo[RT], s_hi[RT], s_row[RT];
-    __half *sq = (__half *)(smem + NW * Sh::WARP);  // [NQ][RT][QS]
+    __half *sq = (__half *)(smem + Sh::OFF_Q);  // [NQ][RT][QS]
+    __half *sp = sq + NQ * RT * QS;             // [2][NQ][RT][PS]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int G = a.group, Hk = a.pool.heads_kv;
 
@@ -144,6 +156,43 @@ __global__ void __launch_bounds__(NW * 32) kvq_attn_kernel(const __grid_constant
     const SeqTable seqs = load_seqs(a, sg, (int32_t *)smem, NW * 32);  // (the slots' memory, not in use yet)
     if (tid < RT) row_range(a, sg, seqs, row_first + tid, s_row[tid], s_lo[tid], s_hi[tid]);
     __syncthreads();
+    // the tile's ranges (rows that do not exist see everything and are not written)
+    int lo_min = 0x7fffffff, lo_max = 0, hi_min = 0x7fffffff, hi_max = -1;
+#pragma unroll
+    for (int n = lane; n < (RT + 31) / 32 * 32; n += 32) {
+        const bool on = n < RT && s_row[n < RT ? n : 0] >= 0;
+        const int lo = on ? s_lo[n] : 0, hi = on ? s_hi[n] : 0;
+        lo_min = min(lo_min, __reduce_min_sync(0xffffffffu, on ? lo : 0x7fffffff));
+        lo_max = max(lo_max, __reduce_max_sync(0xffffffffu, on ? lo : 0));
+        hi_min = min(hi_min, __reduce_min_sync(0xffffffffu, on ? hi : 0x7fffffff));
+        hi_max = max(hi_max, __reduce_max_sync(0xffffffffu, on ? hi : -1));
+    }
+    // ---- pages [u0, u1) of the segment's list
+    const int u0 = max(chunk * ch, lo_min / KVQ_PAGE);
+    const int u1 = min((chunk + 1) * ch, hi_max < 0 ? 0 : hi_max / KVQ_PAGE + 1);
+    const uint32_t smem_s = su32(smem);
+    auto place = [&](int u) -> int64_t {  // the page's first position in rows of one head, or -1
+        const int page = u < u1 ? __ldg(pages + u) : -1;
+        return (unsigned)page < (unsigned)a.pool.n_pages ? ((int64_t)page * Hk + kvh) * KVQ_PAGE : -1;
+    };
+    auto fetch = [&](int64_t at, int slot, bool v) {  // K with both scales, or V, into slot 0 or 1
+        if (at >= 0) {
+            const uint8_t *src = (const uint8_t *)(v ? a.pool.v : a.pool.k) + at * D + tid * 16;
+            const uint32_t dst = smem_s + ((v ? 2 : 0) + slot) * Sh::SLOT;
+#pragma unroll
+            for (int i = 0; i < Sh::SLOT / 2048; i++) {
+                const int idx = i * 128 + tid, r = idx / Sh::CPR, c = idx % Sh::CPR;
+                cp16(dst + 16 * (v ? v_piece<D>(r, c) : k_piece<D>(r, c)), src + i * 2048);
+            }
+            if (!v) cp4(smem_s + Sh::OFF_SC + (slot * 128 + tid) * 4, (tid < 64 ? a.pool.k_scale + at : a.pool.v_scale + at - 64) + tid);
+        }
+        cp_commit();
+    };
+    int64_t at = place(u0), at1 = place(u0 + 1), at2 = place(u0 + 2);
+    fetch(at, 0, false);
+    fetch(at, 0, true);
+    fetch(at1, 1, false);
+
     for (int n = warp; n < RT; n += NW) {
         const int row = s_row[n];
         float x[D / 32], mx = 0.0f;
@@ -164,329 +213,285 @@ __global__ void __launch_bounds__(NW * 32) kvq_attn_kernel(const __grid_constant
         }
         // scores in base 2, or natural ones for the cap
         if (lane == 0)
-            s_qf[n] = a.at.scale * code_unit<FMT>() * (a.at.softcap > 0.0f ? 1.0f : 1.4426950408889634f) *
-                      pow2(-e);
+            s_qf[n] = a.at.scale * code_unit<FMT>() * (a.at.softcap > 0.0f ? 1.0f : 1.4426950408889634f) * pow2(-e);
     }
+    cp_wait<0>();
     __syncthreads();
-    // the tile's ranges (rows that do not exist see everything and are not written)
-    int lo_min = 0x7fffffff, lo_max = 0, hi_min = 0x7fffffff, hi_max = -1;
-    {
-        const bool on = lane < RT && s_row[lane < RT ? lane : 0] >= 0;
-        const int lo = on ? s_lo[lane] : 0, hi = on ? s_hi[lane] : 0;
-        lo_min = __reduce_min_sync(0xffffffffu, on ? lo : 0x7fffffff);
-        lo_max = __reduce_max_sync(0xffffffffu, on ? lo : 0);
-        hi_min = __reduce_min_sync(0xffffffffu, on ? hi : 0x7fffffff);
-        hi_max = __reduce_max_sync(0xffffffffu, on ? hi : -1);
-    }
-    float qf[NT][2];
+    // this lane's rows are nt * 8 + 2 t and the next
+    float qf[NT][2], ref[NT][2], l[NT][2], o[Sh::GPW][2][NT][4];
     int clo[NT][2], chi[NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)
+    for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
         for (int c = 0; c < 2; c++) {
             const int n = nt * 8 + 2 * t + c;
             qf[nt][c] = s_qf[n];
             clo[nt][c] = s_lo[n];
             chi[nt][c] = s_hi[n];
+            ref[nt][c] = -INFINITY;
+            l[nt][c] = 0.0f;
         }
-
-    // ---- this warp's units: u0 + warp, + NW, ...
-    constexpr int UPP = KVQ_PAGE / LT;
-    int u0 = max(chunk * ch * UPP, lo_min / LT);
-    const int u1 = (int)min((int64_t)(chunk + 1) * ch * UPP, hi_max < 0 ? 0 : (int64_t)hi_max / LT + 1);
-    uint8_t *kslot = smem + warp * Sh::WARP, *vslot = kslot + Sh::SLOT;
-    float *ksc = (float *)(vslot + Sh::SLOT), *vsc = ksc + LT;
-    const uint32_t kslot_s = su32(kslot), vslot_s = su32(vslot), ksc_s = su32(ksc), vsc_s = su32(vsc);
-    auto place = [&](int u) -> int64_t {  // first position of unit u in rows of one head, or -1
-        if (u >= u1) return -1;
-        const int page = __ldg(pages + u / UPP);
-        if ((unsigned)page >= (unsigned)a.pool.n_pages) return -1;
-        return ((int64_t)page * Hk + kvh) * KVQ_PAGE + (u % UPP) * LT;
-    };
-    auto fetch = [&](int64_t at, bool v) {
-        if (at >= 0) {
-            const uint8_t *src = (const uint8_t *)(v ? a.pool.v : a.pool.k) + at * D + lane * 16;
-            const uint32_t dst = v ? vslot_s : kslot_s;
 #pragma unroll
-            for (int i = 0; i < Sh::SLOT / 512; i++) {
-                const int idx = i * 32 + lane, r = idx / Sh::CPR, c = idx % Sh::CPR;
-                cp16(dst + 16 * (v ? v_piece<D>(r, c) : k_piece<D>(r, c)), src + i * 512);
-            }
-            const float *sc = (v ? a.pool.v_scale : a.pool.k_scale) + at + lane;
+        for (int q = 0; q < Sh::GPW; q++)
 #pragma unroll
-            for (int i = 0; i < LT / 32; i++) cp4((v ? vsc_s : ksc_s) + 4 * (lane + 32 * i), sc + 32 * i);
-        }
-        cp_commit();
-    };
-    float o[NT][D / 16][4], m[NT][2], l[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-        for (int j = 0; j < D / 16; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[nt][j][e] = 0.0f;
-        m[nt][0] = m[nt][1] = -INFINITY;
-        l[nt][0] = l[nt][1] = 0.0f;
+            for (int e = 0; e < 4; e++) o[q][0][nt][e] = o[q][1][nt][e] = 0.0f;
     }
     float vpow = 1.17549435e-38f;  // 2^E: O is in units of it
     const bool cap = a.at.softcap > 0.0f;
     const float inv_cap2 = cap ? 2.0f * 1.4426950408889634f / a.at.softcap : 0.0f;
-
-    int u = u0 + warp;
-    int64_t at = place(u), at_next = place(u + NW);
-    fetch(at, false);
-    fetch(at, true);
-    for (; u < u1; u += NW) {
-        const int64_t after = place(u + 2 * NW);
-        cp_wait<1>();
-        __syncwarp();
-        // ---- S^T = K Q^T
-        float s[MT][NT][4];
+    auto query = [&](int c, uint32_t (&qb)[NQ][NT][Sh::KB / 2]) {  // B fragments of piece c
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+        for (int h = 0; h < NQ; h++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                const uint8_t *p = (const uint8_t *)(sq + (h * RT + nt * 8 + g) * QS + (c * 4 + t) * Sh::KB);
+#pragma unroll
+                for (int i = 0; i < Sh::KB / 8; i++) {
+                    uint32_t w[4];
+                    lds<16>(p + 16 * i, w);
+#pragma unroll
+                    for (int x = 0; x < 4; x++) qb[h][nt][4 * i + x] = w[x];
+                }
+            }
+    };
+    uint32_t qr[QREG ? Sh::KC : 1][NQ][NT][Sh::KB / 2];
+    if (QREG)
+#pragma unroll
+        for (int c = 0; c < Sh::KC; c++) query(c, qr[QREG ? c : 0]);
+
+    const int j16 = warp * 16 + row_position(g);  // this lane's positions of a page in S^T: j16 and j16 + 8
+    const int grp = D == 64 ? warp & 1 : warp, mt0 = D == 64 ? (warp >> 1) * 2 : 0;
+    for (int u = u0, sl = 0; u < u1; u++, sl ^= 1) {
+        const int64_t now = at;
+        at = at1;
+        at1 = at2;
+        at2 = place(u + 3);
+        bool again = false;
+        const int t0 = u * KVQ_PAGE + j16;
+        __half *pw = sp + sl * NQ * RT * PS;
+        float s[NT][4], ln[NT][2], vf[2] = {0.0f, 0.0f};
+        const bool whole = u * KVQ_PAGE >= lo_max && u * KVQ_PAGE + KVQ_PAGE - 1 <= hi_min;
+        // the weights of this warp's positions into shared memory, relative to the references
+        auto weights = [&]() {
+            const float inv = pow_inverse(vpow);
+            uint32_t any = 0;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float p[4];
+                ln[nt][0] = ln[nt][1] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float x = s[nt][e];
+                    float y = ex2(x - ref[nt][e & 1]);
+                    p[e] = y * (vf[e >> 1] * inv);
+                    if (!whole && x == -INFINITY) y = p[e] = 0.0f;  // whatever the unseen position holds
+                    ln[nt][e & 1] += y;
+                }
+                uint32_t b[NQ][2];
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++) {
+                    const uint32_t hi = pack(p[2 * hf], p[2 * hf + 1]);
+                    any |= too_large<SPLIT>(hi);
+                    b[0][hf] = transpose8(hi);
+                    if (SPLIT) {
+                        const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+                        b[NQ - 1][hf] = transpose8(pack(p[2 * hf] - back.x, p[2 * hf + 1] - back.y));
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < NQ; h++)
+                    *(uint2 *)(pw + (h * RT + nt * 8 + g) * PS + warp * 16 + t * 4) = make_uint2(b[h][0], b[h][1]);
+            }
+            return any != 0;
+        };
+        if (now >= 0) {
+            // ---- S^T = K Q^T: 16 positions
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[mt][nt][e] = 0.0f;
-        if (at >= 0) {
-            const int kr = (g >> 1) + 4 * (g & 1);
+                for (int e = 0; e < 4; e++) s[nt][e] = 0.0f;
+            const uint8_t *kslot = smem + sl * Sh::SLOT;
+            const float *ksc = (const float *)(smem + Sh::OFF_SC) + sl * 128;
+            const float kf[2] = {ksc[j16], ksc[j16 + 8]};
+            vf[0] = ksc[64 + j16] * code_unit<FMT>();
+            vf[1] = ksc[64 + j16 + 8] * code_unit<FMT>();
 #pragma unroll
             for (int c = 0; c < Sh::KC; c++) {
-                uint32_t qb[NQ][NT][Sh::KB / 2];
+                uint32_t ql[NQ][NT][Sh::KB / 2];
+                if (!QREG) query(c, ql);
+                const uint32_t (&qb)[NQ][NT][Sh::KB / 2] = QREG ? qr[QREG ? c : 0] : ql;
+                uint32_t w[2][Sh::KB / 4];
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++) {
+                    const int r = j16 + hf * 8, byte = (c * 4 + t) * Sh::KB;
+                    lds<Sh::KB>(kslot + 16 * k_piece<D>(r, byte / 16) + byte % 16, w[hf]);
+                }
+#pragma unroll
+                for (int k = 0; k < Sh::KB / 4; k++) {
+                    const uint32_t x0 = w[0][k] ^ code_flip<FMT>(), x1 = w[1][k] ^ code_flip<FMT>();
+                    const uint32_t f[4] = {codes2<FMT, 0, 1>(x0), codes2<FMT, 0, 1>(x1), codes2<FMT, 2, 3>(x0), codes2<FMT, 2, 3>(x1)};
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int h = 0; h < NQ; h++) mma(s[nt], f, qb[h][nt][2 * k], qb[h][nt][2 * k + 1]);
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    s[nt][e] *= kf[e >> 1] * qf[nt][e & 1];
+                    if (cap) s[nt][e] = capped<SPLIT>(s[nt][e], a.at.softcap, inv_cap2) * 1.4426950408889634f;
+                }
+            if (!whole)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int j = t0 + (e >> 1) * 8;
+                        if (j < clo[nt][e & 1] || j > chi[nt][e & 1] || j >= len) s[nt][e] = -INFINITY;
+                    }
+            again = weights();
+        }
+        cp_wait<0>();                  // V of this page and K of the next, this thread's part
+        again = __syncthreads_or(again);  // everybody's, and all weights
+        fetch(at, sl ^ 1, true);
+        fetch(at1, sl, false);
+        if (now < 0) continue;
+        if (again) {
+            // ---- some weight is near the limit (or a reference is not set): search the page's maxima, raise
+            float vmax = t0 < len ? fmaxf(vf[0], 0.0f) : 0.0f;  // of positions that exist; a NaN does not count
+            if (t0 + 8 < len) vmax = fmaxf(vmax, vf[1]);
+            vmax = warp_max(vmax);
+            if (lane == 0) s_vmax[warp] = vmax;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    float mx = fmaxf(s[nt][c], s[nt][c + 2]);
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                    if (g == 0) s_max[warp][nt * 8 + 2 * t + c] = mx;
+                }
+            __syncthreads();
+            const float vp = fmaxf(vpow, scale_pow(fmaxf(fmaxf(s_vmax[0], s_vmax[1]), fmaxf(s_vmax[2], s_vmax[3]))));
+            const float ve = vpow * pow_inverse(vp);
+            vpow = vp;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const int n = nt * 8 + 2 * t + c;
+                    const float top = fmaxf(fmaxf(s_max[0][n], s_max[1][n]), fmaxf(s_max[2][n], s_max[3][n])) + ref_head<SPLIT>();
+                    float f = 1.0f;
+                    if (top > ref[nt][c]) {
+                        f = ex2(ref[nt][c] - top);  // nothing seen before: exp2(-inf) = 0
+                        ref[nt][c] = top;
+                        l[nt][c] *= f;
+                    }
+                    f *= ve;
+#pragma unroll
+                    for (int q = 0; q < Sh::GPW; q++)
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            o[q][j][nt][c] *= f;
+                            o[q][j][nt][c + 2] *= f;
+                        }
+                }
+            weights();
+            __syncthreads();
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            l[nt][0] += ln[nt][0];
+            l[nt][1] += ln[nt][1];
+        }
+        // ---- O^T += V^T P^T: 32 dimensions
+        if (D != 96 || warp < 3) {
+            const uint8_t *vslot = smem + (2 + sl) * Sh::SLOT;
+#pragma unroll
+            for (int m = 0; m < (D == 64 ? 2 : 4); m++) {
+                const int mt = mt0 + m;
+                uint2 pb[NQ][NT];
 #pragma unroll
                 for (int h = 0; h < NQ; h++)
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        const uint8_t *p = (const uint8_t *)(sq + (h * RT + nt * 8 + g) * QS + (c * 4 + t) * Sh::KB);
+                    for (int nt = 0; nt < NT; nt++) pb[h][nt] = *(const uint2 *)(pw + (h * RT + nt * 8 + g) * PS + mt * 16 + t * 4);
 #pragma unroll
-                        for (int i = 0; i < Sh::KB / 8; i++) {
-                            uint32_t w[4];
-                            lds<16>(p + 16 * i, w);
+                for (int q = 0; q < Sh::GPW; q++) {
+                    uint32_t x[4];
 #pragma unroll
-                            for (int x = 0; x < 4; x++) qb[h][nt][4 * i + x] = w[x];
-                        }
+                    for (int i = 0; i < 4; i++) {
+                        const int r = mt * 16 + 4 * i + t, byte = (grp + 4 * q) * 32 + g * 4;
+                        x[i] = *(const uint32_t *)(vslot + 16 * v_piece<D>(r, byte / 16) + byte % 16) ^ code_flip<FMT>();
                     }
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++) {
-                    uint32_t w[2][Sh::KB / 4];
-#pragma unroll
-                    for (int hf = 0; hf < 2; hf++) {
-                        const int r = mt * 16 + hf * 8 + kr, byte = (c * 4 + t) * Sh::KB;
-                        lds<Sh::KB>(kslot + 16 * k_piece<D>(r, byte / 16) + byte % 16, w[hf]);
-                    }
-#pragma unroll
-                    for (int k = 0; k < Sh::KB / 4; k++) {
-                        const uint32_t x0 = w[0][k] ^ code_flip<FMT>(), x1 = w[1][k] ^ code_flip<FMT>();
-                        const uint32_t f[4] = {codes2<FMT, 0, 1>(x0), codes2<FMT, 0, 1>(x1), codes2<FMT, 2, 3>(x0),
-                                               codes2<FMT, 2, 3>(x1)};
+                    for (int hf = 0; hf < 2; hf++) {  // dimensions 0, 1 and 2, 3 of the four bytes
+                        const uint32_t ab = __byte_perm(x[0], x[1], hf ? 0x7362 : 0x5140), cd = __byte_perm(x[2], x[3], hf ? 0x7362 : 0x5140);
+                        const uint32_t fr[4] = {codes2<FMT, 0, 1>(ab), codes2<FMT, 2, 3>(ab), codes2<FMT, 0, 1>(cd), codes2<FMT, 2, 3>(cd)};
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                            for (int h = 0; h < NQ; h++) mma(s[mt][nt], f, qb[h][nt][2 * k], qb[h][nt][2 * k + 1]);
+                            for (int h = 0; h < NQ; h++) mma(o[q][hf][nt], fr, pb[h][nt].x, pb[h][nt].y);
                     }
                 }
             }
         }
-        float kf[MT][2];
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-            for (int hf = 0; hf < 2; hf++) kf[mt][hf] = ksc[mt * 16 + hf * 8 + row_position(g)];
-        __syncwarp();
-        const int64_t now = at;
-        fetch(at_next, false);
-        // ---- softmax over the unit
-        const int t0 = u * LT;
-        const bool whole = t0 >= lo_max && t0 + LT - 1 <= hi_min;
-        if (now >= 0) {
-            float mx[NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int c = 0; c < 2; c++) mx[nt][c] = -INFINITY;
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        float x = s[mt][nt][e] * (kf[mt][e >> 1] * qf[nt][e & 1]);
-                        if (cap) x = capped<SPLIT>(x, a.at.softcap, inv_cap2) * 1.4426950408889634f;
-                        if (!whole) {
-                            const int j = t0 + mt * 16 + (e >> 1) * 8 + row_position(g);
-                            if (j < clo[nt][e & 1] || j > chi[nt][e & 1] || j >= len) x = -INFINITY;
-                        }
-                        s[mt][nt][e] = x;
-                        mx[nt][e & 1] = fmaxf(mx[nt][e & 1], x);
-                    }
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-#pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) mx[nt][c] = fmaxf(mx[nt][c], __shfl_xor_sync(0xffffffffu, mx[nt][c], d));
-                    mx[nt][c] = fmaxf(mx[nt][c], m[nt][c]);
-                }
-            cp_wait<1>();  // V and its scales
-            __syncwarp();
-            float vf[MT][2], vmax = 0.0f;
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int hf = 0; hf < 2; hf++) {
-                    const int j = mt * 16 + hf * 8 + row_position(g);
-                    vf[mt][hf] = vsc[j] * code_unit<FMT>();
-                    if (t0 + j < len) vmax = fmaxf(vmax, vf[mt][hf]);  // a NaN scale does not count
-                }
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
-            const float vp = fmaxf(vpow, scale_pow(vmax)), inv = pow_inverse(vp), ve = vpow * inv;
-            vpow = vp;
-            bool moved = ve != 1.0f;
-            float f[NT][2], base[NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    base[nt][c] = mx[nt][c] == -INFINITY ? 0.0f : mx[nt][c];
-                    f[nt][c] = ex2(m[nt][c] - base[nt][c]);  // nothing seen before: exp2(-inf) = 0
-                    m[nt][c] = mx[nt][c];
-                    l[nt][c] *= f[nt][c];
-                    f[nt][c] *= ve;
-                    moved = moved || f[nt][c] != 1.0f;
-                }
-            if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int j = 0; j < D / 16; j++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) o[nt][j][e] *= f[nt][e & 1];
-            }
-            // ---- P^T fragments: the S^T tile transposed
-            uint32_t pb[NQ][MT][NT][2];
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                const float w0 = vf[mt][0] * inv, w1 = vf[mt][1] * inv;
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    float p[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float x = s[mt][nt][e], y = ex2(x - base[nt][e & 1]);
-                        l[nt][e & 1] += y;
-                        p[e] = y * (e < 2 ? w0 : w1);
-                        if (!whole && x == -INFINITY) p[e] = 0.0f;  // whatever the unseen position holds
-                    }
-#pragma unroll
-                    for (int hf = 0; hf < 2; hf++) {
-                        const uint32_t hi = pack(p[2 * hf], p[2 * hf + 1]);
-                        pb[0][mt][nt][hf] = transpose8(hi);
-                        if (SPLIT) {
-                            const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-                            pb[NQ - 1][mt][nt][hf] = transpose8(pack(p[2 * hf] - back.x, p[2 * hf + 1] - back.y));
-                        }
-                    }
-                }
-            }
-            // ---- O^T += V^T P^T
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int c = 0; c < Sh::VC; c++) {
-                    uint32_t w[4][Sh::VB / 4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int r = mt * 16 + 4 * i + t, byte = (c * 8 + g) * Sh::VB;
-                        lds<Sh::VB>(vslot + 16 * v_piece<D>(r, byte / 16) + byte % 16, w[i]);
-                    }
-#pragma unroll
-                    for (int k = 0; k < Sh::VB / 4; k++) {
-                        const uint32_t x0 = w[0][k] ^ code_flip<FMT>(), x1 = w[1][k] ^ code_flip<FMT>();
-                        const uint32_t x2 = w[2][k] ^ code_flip<FMT>(), x3 = w[3][k] ^ code_flip<FMT>();
-#pragma unroll
-                        for (int hf = 0; hf < 2; hf++) {  // dimensions 0, 1 and 2, 3 of the four bytes
-                            const uint32_t ab = __byte_perm(x0, x1, hf ? 0x7362 : 0x5140), cd = __byte_perm(x2, x3, hf ? 0x7362 : 0x5140);
-                            const uint32_t fr[4] = {codes2<FMT, 0, 1>(ab), codes2<FMT, 2, 3>(ab), codes2<FMT, 0, 1>(cd),
-                                                    codes2<FMT, 2, 3>(cd)};
-                            const int j = (c * Sh::VB / 4 + k) * 2 + hf;
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                                for (int h = 0; h < NQ; h++) mma(o[nt][j], fr, pb[h][mt][nt][0], pb[h][mt][nt][1]);
-                        }
-                    }
-                }
-        } else {
-            cp_wait<1>();
-        }
-        __syncwarp();
-        fetch(at_next, true);
-        at = at_next;
-        at_next = after;
     }
     cp_wait<0>();
-    __syncthreads();
 
-    // ---- join the warps: sums over the lanes that share a row, then O through shared memory in
-    // register order (one float4 of four consecutive dimensions per lane)
+    // ---- the rows' sums over the warps; with head_dim 64 the two warps of a group
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int c = 0; c < 2; c++) {
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], d);
-            if (g == 0) {
-                s_m[warp][nt * 8 + 2 * t + c] = m[nt][c];
-                s_l[warp][nt * 8 + 2 * t + c] = l[nt][c];
-            }
+            if (g == 0) s_l[warp][nt * 8 + 2 * t + c] = l[nt][c];
         }
-    if (lane == 0) s_e[warp] = vpow;
-    constexpr int PIECES = NT * 2 * (D / 32);  // float4 pieces of a lane: (nt, column, four dimensions)
-    float4 *so = (float4 *)smem;               // [NW][PIECES][32]
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int c = 0; c < 2; c++)
-#pragma unroll
-            for (int k = 0; k < D / 32; k++)
-                so[(warp * PIECES + (nt * 2 + c) * (D / 32) + k) * 32 + lane] =
-                    make_float4(o[nt][2 * k][c], o[nt][2 * k][2 + c], o[nt][2 * k + 1][c], o[nt][2 * k + 1][2 + c]);
     __syncthreads();
+    float4 *so = (float4 *)smem;  // [warp & 1][nt, column][lane]
+    if (D == 64 && warp >= 2) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int c = 0; c < 2; c++)
+                so[((warp & 1) * NT * 2 + nt * 2 + c) * 32 + lane] = make_float4(o[0][0][nt][c], o[0][0][nt][c + 2], o[0][1][nt][c], o[0][1][nt][c + 2]);
+    }
+    if (D == 64) __syncthreads();
     const int64_t RH = (int64_t)a.bt.rows * a.at.heads, slot = sg.pre ? chunk : a.nsp + chunk;
-    for (int pc = warp; pc < PIECES; pc += NW) {
-        const int nc = pc / (D / 32), k = pc % (D / 32), n = (nc >> 1) * 8 + 2 * t + (nc & 1), row = s_row[n];
-        if (row < 0) continue;
-        float M = -INFINITY;
+    if (warp < (D == 64 ? 2 : D == 96 ? 3 : 4)) {
 #pragma unroll
-        for (int w = 0; w < NW; w++) M = fmaxf(M, s_m[w][n]);
-        float L = 0.0f, x[4] = {};
+        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int w = 0; w < NW; w++) {
-            if (s_m[w][n] == -INFINITY && !(s_l[w][n] != s_l[w][n])) continue;  // this warp saw nothing
-            const float f = ex2(s_m[w][n] - M), fo = f * s_e[w];
-            L = fmaf(s_l[w][n], f, L);
-            const float4 v = so[(w * PIECES + pc) * 32 + lane];
-            x[0] = fmaf(v.x, fo, x[0]);
-            x[1] = fmaf(v.y, fo, x[1]);
-            x[2] = fmaf(v.z, fo, x[2]);
-            x[3] = fmaf(v.w, fo, x[3]);
-        }
-        const int head = kvh * G + (row_first + n) % G, word = k;  // four dimensions of this lane
-        const int d = word / (Sh::VB / 4) * 8 * Sh::VB + g * Sh::VB + word % (Sh::VB / 4) * 4;
-        if (a.direct) {
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-            float y[4];
+            for (int c = 0; c < 2; c++) {
+                const int n = nt * 8 + 2 * t + c, row = s_row[n];
+                if (row < 0) continue;
+                const float L = (s_l[0][n] + s_l[1][n]) + (s_l[2][n] + s_l[3][n]);
+                const int head = kvh * G + (row_first + n) % G;
+                const int64_t rh = (int64_t)row * a.at.heads + head;
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = L == 0.0f ? 0.0f : x[e] * inv;
-            store4(a.out, row * a.ldo + (int64_t)head * D + d, a.at.type, a.wide != 0, y);
-            if (a.lse && g == 0 && k == 0)
-                a.lse[(int64_t)row * a.at.heads + head] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
-        } else {
-            const int64_t rh = (int64_t)row * a.at.heads + head;
-            *(float4 *)(a.part_o + (slot * RH + rh) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
-            if (g == 0 && k == 0) a.part_ml[slot * RH + rh] = make_float2(M, L);
-        }
+                for (int q = 0; q < Sh::GPW; q++) {
+                    float x[4] = {o[q][0][nt][c], o[q][0][nt][c + 2], o[q][1][nt][c], o[q][1][nt][c + 2]};
+                    if (D == 64) {
+                        const float4 v = so[(warp * NT * 2 + nt * 2 + c) * 32 + lane];
+                        x[0] += v.x;
+                        x[1] += v.y;
+                        x[2] += v.z;
+                        x[3] += v.w;
+                    }
+                    const int d = (grp + 4 * q) * 32 + g * 4;
+                    const float f = a.direct ? (L == 0.0f ? 0.0f : vpow / L) : vpow;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] = a.direct && L == 0.0f ? 0.0f : x[e] * f;
+                    if (a.direct) store4(a.out, row * a.ldo + (int64_t)head * D + d, a.at.type, a.wide != 0, x);
+                    else *(float4 *)(a.part_o + (slot * RH + rh) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+                }
+                if (warp == 0 && g == 0) {
+                    if (!a.direct) a.part_ml[slot * RH + rh] = make_float2(ref[nt][c], L);
+                    else if (a.lse) a.lse[rh] = L == 0.0f ? -INFINITY : (ref[nt][c] + log2f(L)) * 0.6931471805599453f;
+                }
+            }
     }
     if (a.chained) pdl_wait();
 }
@@ -549,9 +554,9 @@ template <int D> __global__ void __launch_bounds__(128) kvq_join_kernel(const __
 template <int D, int FMT, int NT, bool SPLIT> cudaError_t launch_tiles(const AttnArgs &a, int64_t grid, cudaStream_t st)
 {
     using Sh = Shape<D>;
-    static_assert(NW * Sh::WARP >= (2 * SEQ_TABLE + 1) * 4, "the sequences' tables fit into the slots");
-    constexpr int smem = NW * Sh::WARP + (SPLIT ? 2 : 1) * NT * 8 * (D + Sh::QPAD) * 2;
-    static_assert(NT * 8 * D * 4 <= Sh::WARP, "the warps' outputs fit into their slots");
+    constexpr int NQ = SPLIT ? 2 : 1, smem = Sh::OFF_Q + NQ * NT * 8 * (D + Sh::QPAD + 2 * PS) * 2;
+    static_assert(4 * Sh::SLOT >= (2 * SEQ_TABLE + 1) * 4, "the sequences' tables fit into the slots");
+    static_assert(D != 64 || 4 * Sh::SLOT >= 2 * NT * 2 * 512, "two warps' outputs fit into the slots");
     static std::atomic<unsigned long long> done{0};
     cudaError_t e = smem_attr_once(done, kvq_attn_kernel<D, FMT, NT, SPLIT>, smem);
     if (e != cudaSuccess) return e;
@@ -559,11 +564,13 @@ template <int D, int FMT, int NT, bool SPLIT> cudaError_t launch_tiles(const Att
 }
 template <int D, int FMT, bool SPLIT> cudaError_t launch_nt(int nt, const AttnArgs &a, int64_t grid, cudaStream_t st)
 {
-    constexpr int MX = Shape<D>::MAX_NT;
-    if (nt == 1) return launch_tiles<D, FMT, 1, SPLIT>(a, grid, st);
-    if (nt == 2 || MX == 2) return launch_tiles<D, FMT, 2, SPLIT>(a, grid, st);
-    if (nt == 3 || MX == 3) return launch_tiles<D, FMT, MX < 3 ? 2 : 3, SPLIT>(a, grid, st);
-    return launch_tiles<D, FMT, MX < 4 ? 2 : 4, SPLIT>(a, grid, st);
+    switch (nt) {
+    case 1: return launch_tiles<D, FMT, 1, SPLIT>(a, grid, st);
+    case 2: return launch_tiles<D, FMT, 2, SPLIT>(a, grid, st);
+    case 3: return launch_tiles<D, FMT, 3, SPLIT>(a, grid, st);
+    case 4: return launch_tiles<D, FMT, 4, SPLIT>(a, grid, st);
+    default: return launch_tiles<D, FMT, Shape<D>::MAX_NT, SPLIT>(a, grid, st);
+    }
 }
 template <int D> cudaError_t launch_dim(int nt, const AttnArgs &a, int64_t grid, cudaStream_t st)
 {
@@ -601,7 +608,11 @@ struct Plan {
     int64_t ctas_p, ctas_s;
     size_t o_bytes, ml_bytes;
 };
-int max_nt(int dim) { return dim == 256 ? 2 : dim == 128 ? 3 : 4; }
+int tiles_of(int dim, int64_t rows)  // 8-row tiles per CTA: 1, 2, 3, 4 or 8 (4 with head_dim 256)
+{
+    const int64_t n = std::max<int64_t>(1, (rows + 7) / 8);
+    return (int)(n <= 4 ? n : dim == 256 ? 4 : 8);
+}
 // From this many rows (times heads) per kv head a segment is worth the wide kernel.
 constexpr int64_t WIDE_FROM = 48;
 
@@ -610,20 +621,19 @@ Plan make_plan(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const llmdot
     Plan x = {};
     const int64_t G = a.heads / p.heads_kv, Hk = p.heads_kv, own_rows = (int64_t)b.max_rows * G, all_rows = (int64_t)b.rows * G;
     const int64_t npp = (a.prefix_len + KVQ_PAGE - 1) / KVQ_PAGE, wide = kvq_wide_rows(p.head_dim);
-    auto nt_of = [&](int64_t rows) { return (int)std::min<int64_t>(max_nt(p.head_dim), std::max<int64_t>(1, (rows + 7) / 8)); };
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
     x.wide_p = a.type != T_F32 && npp > 0 && all_rows >= WIDE_FROM;
     x.wide_s = a.type != T_F32 && own_rows >= WIDE_FROM;
-    x.nt_p = nt_of(all_rows);
-    x.nt_s = nt_of(own_rows);
+    x.nt_p = tiles_of(p.head_dim, all_rows);
+    x.nt_s = tiles_of(p.head_dim, own_rows);
     if (npp == 0) x.nt_p = x.nt_s;
     x.ptiles = (int)up(all_rows, x.wide_p ? wide : 8 * x.nt_p);
     x.rtiles = (int)std::max<int64_t>(1, up(own_rows, x.wide_s ? wide : 8 * x.nt_s));
-    // Chunks.  Narrow: enough CTAs to fill the SMs about four times (ragged sequences leave some without
-    // work), at least one page per warp, at most 32 pages, so that long and short sequences balance.
-    // Wide: one CTA per SM, at least four pages each.
+    // Chunks.  Narrow: enough CTAs to fill the SMs (five each) about twice over (ragged sequences leave
+    // some without work), at most 32 pages, so that long and short sequences balance.  Wide: one CTA per SM,
+    // at least four pages each.
     const int64_t np = x.wide_p ? 0 : Hk * x.ptiles * npp, ns = x.wide_s ? 0 : Hk * b.batch * x.rtiles * b.max_pages;
-    const int64_t ch = std::min<int64_t>(32, std::max<int64_t>(NW, up(up(np + ns, 148 * 4), NW) * NW));
+    const int64_t ch = std::min<int64_t>(32, std::max<int64_t>(1, up(np + ns, 148 * 10)));
     auto wide_ch = [&](int64_t ctas, int64_t pages) { return std::max<int64_t>(4, up(pages, std::max<int64_t>(1, 148 / std::max<int64_t>(1, ctas)))); };
     x.ch_p = (int)(x.wide_p ? wide_ch(Hk * x.ptiles, npp) : ch);
     x.ch_s = (int)(x.wide_s ? wide_ch(Hk * x.rtiles * b.batch, b.max_pages) : ch);
