@@ -496,13 +496,16 @@ __global__ void __launch_bounds__(NW * 32) kvq_attn_kernel(const __grid_constant
     if (a.chained) pdl_wait();
 }
 
-// Joins a row's partials: one warp per (row, head); the prefix's chunks, then the sequence's.
-template <int D> __global__ void __launch_bounds__(128) kvq_join_kernel(const __grid_constant__ AttnArgs a)
+// Joins a row's partials in chunk order: W warps per (row, head), each every W-th chunk, then the prefix's
+// chunks first.  One warp where there are many rows or few chunks; four else, since a warp has only
+// a few loads in flight.
+template <int D, int W> __global__ void __launch_bounds__(128) kvq_join_kernel(const __grid_constant__ AttnArgs a)
 {
     constexpr int N = D / 32;
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5), RH = (int64_t)a.bt.rows * a.at.heads;
-    const int lane = threadIdx.x & 31;
-    if (item >= RH) return;
+    __shared__ float s_x[W > 1 ? 4 : 1][W > 1 ? D : 1], s_l[4];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % W;
+    const int64_t item = (int64_t)blockIdx.x * (4 / W) + warp / W, RH = (int64_t)a.bt.rows * a.at.heads;
+    if (item >= RH) return;  // with W = 4 a whole CTA
     const int row = (uint32_t)item / (uint32_t)a.at.heads, head = (uint32_t)item - row * a.at.heads;
     const int b = kvq_seq_of(a.bt.row_start, a.bt.batch, row);
     int nown = 0;
@@ -518,36 +521,48 @@ template <int D> __global__ void __launch_bounds__(128) kvq_join_kernel(const __
     for (int s = lane; s < slots; s += 32) M = fmaxf(M, __ldcg(ml + s * RH).x);
     M = warp_max(M);
     float L = 0.0f, x[N] = {};
-    for (int s0 = 0; s0 < slots; s0 += 32) {
+    for (int s0 = 0; s0 < slots; s0 += 32 * W) {
         float w = 0.0f;
-        if (s0 + lane < slots) {
-            const float2 v = __ldcg(ml + (s0 + lane) * RH);
+        const int mine = s0 + lane * W + part;
+        if (mine < slots) {
+            const float2 v = __ldcg(ml + mine * RH);
             if (v.x != -INFINITY || v.y != v.y) {
                 w = ex2(v.x - M);
                 L = fmaf(v.y, w, L);
             }
         }
-        const int n = min(32, slots - s0);
+        const int n = min(32, (slots - s0 - part + W - 1) / W);
 #pragma unroll 4
         for (int s = 0; s < n; s++) {
             const float f = __shfl_sync(0xffffffffu, w, s);
-            if (f == 0.0f) continue;
-            const float *p = a.part_o + ((s0 + s) * RH + item) * D + lane;
+            const float *p = a.part_o + ((int64_t)(s0 + s * W + part) * RH + item) * D + lane;
+            float v[N];
 #pragma unroll
-            for (int i = 0; i < N; i++) x[i] = fmaf(__ldcg(p + 32 * i), f, x[i]);
+            for (int i = 0; i < N; i++) v[i] = __ldcg(p + 32 * i);
+#pragma unroll
+            for (int i = 0; i < N; i++) x[i] = f == 0.0f ? x[i] : fmaf(v[i], f, x[i]);  // a chunk that saw nothing wrote nothing
         }
     }
     L = warp_sum(L);
+    if (W > 1) {
+#pragma unroll
+        for (int i = 0; i < N; i++) s_x[warp][32 * i + lane] = x[i];
+        if (lane == 0) s_l[warp] = L;
+        __syncthreads();
+        L = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+    }
     const float inv = 1.0f / L;
 #pragma unroll
     for (int i = 0; i < N; i++) {
+        if (W > 1 && i % W != part) continue;
+        if (W > 1) x[i] = (s_x[0][32 * i + lane] + s_x[1][32 * i + lane]) + (s_x[2][32 * i + lane] + s_x[3][32 * i + lane]);
         const float y = L == 0.0f ? 0.0f : x[i] * inv;
         const int64_t at = row * a.ldo + (int64_t)head * D + 32 * i + lane;
         if (a.at.type == T_F32) ((float *)a.out)[at] = y;
         else if (a.at.type == T_F16) ((__half *)a.out)[at] = __float2half_rn(y);
         else ((__nv_bfloat16 *)a.out)[at] = __float2bfloat16_rn(y);
     }
-    if (a.lse && lane == 0) a.lse[item] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+    if (a.lse && part == 0 && lane == 0) a.lse[item] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
 // ------------------------------------------------------------------ launch
@@ -588,14 +603,20 @@ cudaError_t launch_narrow(int nt, const AttnArgs &a, int64_t grid, cudaStream_t 
     default: return launch_dim<256>(nt, a, grid, st);
     }
 }
+template <int D> cudaError_t launch_join_dim(const AttnArgs &a, cudaStream_t st)
+{
+    const int64_t items = (int64_t)a.bt.rows * a.at.heads;
+    if (a.nsp + a.nss <= 4 || items > 148 * 32)
+        return launch_kernel(true, kvq_join_kernel<D, 1>, dim3((unsigned)((items + 3) / 4)), dim3(128), 0, st, a);
+    return launch_kernel(true, kvq_join_kernel<D, 4>, dim3((unsigned)items), dim3(128), 0, st, a);
+}
 cudaError_t launch_join(const AttnArgs &a, cudaStream_t st)
 {
-    const dim3 grid((unsigned)(((int64_t)a.bt.rows * a.at.heads + 3) / 4)), block(128);
     switch (a.pool.head_dim) {
-    case 64: return launch_kernel(true, kvq_join_kernel<64>, grid, block, 0, st, a);
-    case 96: return launch_kernel(true, kvq_join_kernel<96>, grid, block, 0, st, a);
-    case 128: return launch_kernel(true, kvq_join_kernel<128>, grid, block, 0, st, a);
-    default: return launch_kernel(true, kvq_join_kernel<256>, grid, block, 0, st, a);
+    case 64: return launch_join_dim<64>(a, st);
+    case 96: return launch_join_dim<96>(a, st);
+    case 128: return launch_join_dim<128>(a, st);
+    default: return launch_join_dim<256>(a, st);
     }
 }
 
@@ -630,11 +651,11 @@ Plan make_plan(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const llmdot
     x.ptiles = (int)up(all_rows, x.wide_p ? wide : 8 * x.nt_p);
     x.rtiles = (int)std::max<int64_t>(1, up(own_rows, x.wide_s ? wide : 8 * x.nt_s));
     // Chunks.  Narrow: enough CTAs to fill the SMs (five each) about twice over (ragged sequences leave
-    // some without work), at most 32 pages, so that long and short sequences balance.  Wide: one CTA per SM,
-    // at least four pages each.
+    // some without work), at least four pages (fewer leave the join with more to read than the chunks
+    // save), at most 32, so that long and short sequences balance.  Wide: one CTA per SM, at least two pages.
     const int64_t np = x.wide_p ? 0 : Hk * x.ptiles * npp, ns = x.wide_s ? 0 : Hk * b.batch * x.rtiles * b.max_pages;
-    const int64_t ch = std::min<int64_t>(32, std::max<int64_t>(1, up(np + ns, 148 * 10)));
-    auto wide_ch = [&](int64_t ctas, int64_t pages) { return std::max<int64_t>(4, up(pages, std::max<int64_t>(1, 148 / std::max<int64_t>(1, ctas)))); };
+    const int64_t ch = std::min<int64_t>(32, std::max<int64_t>(4, up(np + ns, 148 * 10)));
+    auto wide_ch = [&](int64_t ctas, int64_t pages) { return std::max<int64_t>(2, up(pages, std::max<int64_t>(1, 148 / std::max<int64_t>(1, ctas)))); };
     x.ch_p = (int)(x.wide_p ? wide_ch(Hk * x.ptiles, npp) : ch);
     x.ch_s = (int)(x.wide_s ? wide_ch(Hk * x.rtiles * b.batch, b.max_pages) : ch);
     x.nsp = (int)up(npp, x.ch_p);

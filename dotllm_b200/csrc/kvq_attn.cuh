@@ -159,7 +159,8 @@ template <int FMT> constexpr float code_unit() { return FMT == LLMDOT_KVQ_I8 ? 1
 // Exponent that brings a row's largest magnitude into [2^14, 2^15); 0 for zero and non-finite rows.
 __device__ __forceinline__ int row_exponent(float top)
 {
-    return top > 0.0f && top < INFINITY ? min(max(14 - ilogbf(top), -126), 126) : 0;
+    const int b = __float_as_int(top);
+    return b > 0 && b < 0x7f800000 ? min(14 + 127 - (b >> 23), 126) : 0;
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 // The power of two (normal, at most 2^126) not above a value scale; its inverse is exact.

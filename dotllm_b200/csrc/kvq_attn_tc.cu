@@ -187,18 +187,6 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c)
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
     return r;
 }
-// Four 16-bit values as floats.
-__device__ __forceinline__ void halves4(uint2 v, bool half, float (&f)[4])
-{
-    if (half) {
-        const float2 a = __half22float2(*reinterpret_cast<__half2 *>(&v.x)), b = __half22float2(*reinterpret_cast<__half2 *>(&v.y));
-        f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
-    } else {
-        f[0] = __uint_as_float(v.x << 16), f[1] = __uint_as_float(v.x & 0xFFFF0000u);
-        f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xFFFF0000u);
-    }
-}
-
 template <int D, int FMT>
 __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __grid_constant__ AttnArgs a, const int qwide)
 {
@@ -207,7 +195,6 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
     extern __shared__ __align__(16) uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (1024 - (su32(smem_raw) & 1023)) % 1024;
     __shared__ int s_lo[8], s_hi[8], s_abort;
-    __shared__ int64_t s_at[W::TILES * 128];  // a row's place in the partials
     __shared__ uint32_t s_tmem;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = a.group, Hk = a.pool.heads_kv;
@@ -246,6 +233,35 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&s_tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    // The queries of this warp's 32 rows (16 of them for head_dim 256), four values per lane: on their way
+    // while the rest is set up.
+    constexpr int PARTS = (D + 127) / 128, QROWS = PARTS == 1 ? 32 : 16;
+    uint2 raw[QROWS][PARTS];
+    auto load_queries = [&](int r0) {
+        uint32_t rho = row_first + warp * 32 + r0;
+        int i = rho / (uint32_t)G, hg = rho - i * G;
+#pragma unroll
+        for (int r = 0; r < QROWS; r++) {
+            const uint16_t *q = (const uint16_t *)a.q + (sg.r0 + i) * a.ldq + (int64_t)(sg.kvh * G + hg) * D + lane * 4;
+            const bool real = i < sg.nrows;
+#pragma unroll
+            for (int x = 0; x < PARTS; x++) {
+                const bool on = real && lane * 4 + 128 * x < D;
+                raw[r][x] = make_uint2(0, 0);
+                if (qwide) {
+                    if (on) raw[r][x] = __ldg((const uint2 *)(q + 128 * x));
+                } else if (on) {
+                    const uint16_t *p = q + 128 * x;
+                    raw[r][x] = make_uint2(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16);
+                }
+            }
+            if (++hg == G) {
+                hg = 0;
+                i++;
+            }
+        }
+    };
+    if (tid < SOFT) load_queries(0);
     // (the operands' memory holds the sequences' tables meanwhile)
     const SeqTable seqs = load_seqs(a, sg, (int32_t *)smem, W::THREADS);
     int row = -1, lo = 0, hi = 0x7fffffff;
@@ -279,64 +295,43 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
         if (W::TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
         const int tile = warp >> 2, head = sg.kvh * G + (row_first + tid) % G;
         const uint32_t tm = tmem + tile * W::TILE_COLS + ((uint32_t)(32 * (warp & 3)) << 16);
-        // the queries, scaled by a power of two each, as an operand (zeros for rows that do not exist): a row
-        // at a time per warp, four values per lane, eight rows on the way
+        // the queries as an operand: fp16 ones as they are, bf16 ones scaled by a power of two each (zeros for rows
+        // that do not exist); a negative scale's sign goes into them
         int e = 0;
-        {
-            constexpr int PARTS = (D + 127) / 128;
-            const bool half = a.at.type == T_F16;
-            const float sign = a.at.scale < 0.0f ? -1.0f : 1.0f;
-            const int64_t at = row < 0 ? -1 : row * a.ldq + (int64_t)head * D;
-            const uint32_t dst = base + W::OFF_Q + tile * W::Q_BYTES + (warp & 3) * 32 * W::ROW;
-#pragma unroll 1
-            for (int r0 = 0; r0 < 32; r0 += 8) {
-                uint2 raw[8][PARTS];  // loaded first, converted after, so that the loads overlap
-                const uint16_t *src[8];
+        const uint32_t qdst = base + W::OFF_Q + tile * W::Q_BYTES + (warp & 3) * 32 * W::ROW + (lane & 1) * 8;
+        const bool negative = a.at.scale < 0.0f;
+        auto put_query = [&](int r, int x, uint32_t lo, uint32_t hi) {
+            const uint32_t flip = negative ? 0x80008000u : 0u, piece = lane / 2 + 16 * x;
+            if (lane * 4 + 128 * x < D)
+                asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(qdst + (piece >> 3) * W::Q_BLK + r * W::ROW + ((piece & 7) ^ (r & 7)) * 16),
+                             "r"(lo ^ flip), "r"(hi ^ flip)
+                             : "memory");
+        };
 #pragma unroll
-                for (int r = 0; r < 8; r++) {
-                    const int64_t from = __shfl_sync(0xffffffffu, at, r0 + r);
-                    src[r] = from >= 0 ? (const uint16_t *)a.q + from + lane * 4 : nullptr;
-                }
-                if (qwide) {
+        for (int r0 = 0; r0 < 32; r0 += QROWS) {
+            if (r0 > 0) load_queries(r0);
+            if (a.at.type == T_F16) {
 #pragma unroll
-                    for (int r = 0; r < 8; r++)
+                for (int r = 0; r < QROWS; r++)
 #pragma unroll
-                        for (int x = 0; x < PARTS; x++)
-                            raw[r][x] = src[r] && lane * 4 + 128 * x < D ? __ldg((const uint2 *)(src[r] + 128 * x)) : make_uint2(0, 0);
-                } else {
+                    for (int x = 0; x < PARTS; x++) put_query(r0 + r, x, raw[r][x].x, raw[r][x].y);
+            } else {
 #pragma unroll
-                    for (int r = 0; r < 8; r++)
-#pragma unroll
-                        for (int x = 0; x < PARTS; x++) {
-                            raw[r][x] = make_uint2(0, 0);
-                            if (src[r] && lane * 4 + 128 * x < D) {
-                                const uint16_t *p = src[r] + 128 * x;
-                                raw[r][x] = make_uint2(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16);
-                            }
-                        }
-                }
-#pragma unroll
-                for (int r = 0; r < 8; r++) {
-                    float f[PARTS][4];
-#pragma unroll
-                    for (int x = 0; x < PARTS; x++) halves4(raw[r][x], half, f[x]);
+                for (int r = 0; r < QROWS; r++) {
                     uint32_t top = 0;  // magnitudes order as integers, NaN above all
 #pragma unroll
-                    for (int x = 0; x < PARTS; x++)
-#pragma unroll
-                        for (int k = 0; k < 4; k++) top = max(top, __float_as_uint(f[x][k]) & 0x7fffffffu);
+                    for (int x = 0; x < PARTS; x++) {
+                        top = max(top, max((raw[r][x].x << 16) & 0x7fffffffu, raw[r][x].x & 0x7fff0000u));
+                        top = max(top, max((raw[r][x].y << 16) & 0x7fffffffu, raw[r][x].y & 0x7fff0000u));
+                    }
                     const int er = row_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, top)));
                     if (lane == r0 + r) e = er;
-                    const float up = sign * pow2(er);
+                    const float up = pow2(er);
 #pragma unroll
                     for (int x = 0; x < PARTS; x++)
-                        if (lane * 4 + 128 * x < D) {
-                            const int piece = lane / 2 + 16 * x;
-                            const uint32_t d = dst + (piece >> 3) * W::Q_BLK + (r0 + r) * W::ROW + ((piece & 7) ^ r) * 16 + (lane & 1) * 8;
-                            asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(d), "r"(pack(f[x][0] * up, f[x][1] * up)),
-                                         "r"(pack(f[x][2] * up, f[x][3] * up))
-                                         : "memory");
-                        }
+                        put_query(r0 + r, x,
+                                  pack(__uint_as_float(raw[r][x].x << 16) * up, __uint_as_float(raw[r][x].x & 0xFFFF0000u) * up),
+                                  pack(__uint_as_float(raw[r][x].y << 16) * up, __uint_as_float(raw[r][x].y & 0xFFFF0000u) * up));
                 }
             }
         }
@@ -550,48 +545,43 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             ok = __all_sync(0xffffffffu, ok);
         }
         const int64_t RH = (int64_t)a.bt.rows * a.at.heads, slot = sg.pre ? sg.chunk : a.nsp + sg.chunk;
-        const int64_t at = slot * RH + (int64_t)row * a.at.heads + head;
-        s_at[tid] = row >= 0 ? at * D : -1;
-        if (ok && n > 0) {
-            fence_after();
-            // 32 rows by 32 columns at a time through the tile's query operand (done with), so that a warp
-            // writes 128 consecutive bytes of a row
-            float *tr = (float *)(smem + W::OFF_Q + tile * W::Q_BYTES) + (warp & 3) * 32 * 32;
-#pragma unroll 1
-            for (int c = 0; c < D / 32; c++) {
-                uint32_t v[32];
-                tmem_ld32(tm + W::C_O + 32 * c, v);
-                tmem_ld_wait();
-                __syncwarp();
-#pragma unroll
-                for (int j = 0; j < 32; j++) tr[lane * 32 + (j ^ lane)] = __uint_as_float(v[j]) * vpow;
-                __syncwarp();
-#pragma unroll 1
-                for (int r0 = 0; r0 < 32; r0 += 8) {  // read first: the compiler keeps loads behind stores
-                    float o[8];
-                    int64_t to[8];
-#pragma unroll
-                    for (int r = 0; r < 8; r++) {
-                        o[r] = tr[(r0 + r) * 32 + (lane ^ (r0 + r))];
-                        to[r] = s_at[warp * 32 + r0 + r];
-                    }
-#pragma unroll
-                    for (int r = 0; r < 8; r++)
-                        if (to[r] >= 0) a.part_o[to[r] + 32 * c + lane] = o[r];
-                }
-            }
-        }
-        // a row's sum lies in four lanes, its reference in each of them
+        const int at = row < 0 ? -1 : row * a.at.heads + head;  // rows * heads fits 2^30
+        int to[4];
         __syncwarp();
 #pragma unroll
         for (int k = 0; k < 4; k++) {
+            to[k] = __shfl_sync(0xffffffffu, at, g + 8 * k);
+            // a row's sum lies in four lanes, its reference in each of them
             float x, y;
             un2(l[k], x, y);
             x += y;
             x += __shfl_xor_sync(0xffffffffu, x, 1);
             x += __shfl_xor_sync(0xffffffffu, x, 2);
-            const int64_t to = s_at[warp * 32 + g + 8 * k];
-            if (t == 0 && to >= 0) a.part_ml[to / D] = ok ? make_float2(ref[k], x) : make_float2(0.0f, NAN);
+            if (t == 0 && to[k] >= 0) a.part_ml[slot * RH + to[k]] = ok ? make_float2(ref[k], x) : make_float2(0.0f, NAN);
+        }
+        if (ok && n > 0) {  // O: four lanes write 32 consecutive bytes of a row
+            fence_after();
+            const F2 vp2 = f2(vpow, vpow);
+#pragma unroll 1
+            for (int c = 0; c < (D + 63) / 64; c++) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t v[32];
+                    tmem_ld_frag(tm + ((uint32_t)(16 * h) << 16) + W::C_O + 64 * c, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        const int k = 2 * h + r;
+                        float2 *o = (float2 *)(a.part_o + (slot * RH + to[k]) * D + 64 * c + 2 * t);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            float x, y;
+                            un2(mul2(f2(__uint_as_float(v[4 * i + 2 * r]), __uint_as_float(v[4 * i + 2 * r + 1])), vp2), x, y);
+                            if (to[k] >= 0 && 64 * c + 8 * i < D) o[4 * i] = make_float2(x, y);
+                        }
+                    }
+                }
+            }
         }
     } else if (warp < SOFT / 32 + 4) {
         // ------------------------------------------------------------ codes to operands
