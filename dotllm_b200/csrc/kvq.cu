@@ -203,6 +203,36 @@ kvq_write_kernel(const llmdot_kvq_pool pool, const llmdot_kvq_batch bt, const T 
     }
 }
 
+// Four codes of a word as floats.
+template <int FMT> __device__ __forceinline__ void floats4(uint32_t w, float s, float (&f)[4])
+{
+    if (FMT == LLMDOT_KVQ_I8) {  // the byte, sign bit flipped, under the exponent of 2^23: an exact difference
+        w ^= 0x80808080u;
+        f[0] = __fmul_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440)) - 8388736.0f, s);
+        f[1] = __fmul_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7441)) - 8388736.0f, s);
+        f[2] = __fmul_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7442)) - 8388736.0f, s);
+        f[3] = __fmul_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7443)) - 8388736.0f, s);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) f[e] = __fmul_rn(code_value<FMT>((uint8_t)(w >> (8 * e))), s);
+    }
+}
+template <typename T> __device__ __forceinline__ void store4v(T *p, bool wide, const float (&f)[4])
+{
+    __align__(16) T t[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) t[e] = from_f32<T>(f[e]);
+    if (wide) {
+        if (sizeof(T) == 4) *(uint4 *)p = *(const uint4 *)t;
+        else *(uint2 *)p = *(const uint2 *)t;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) p[e] = t[e];
+    }
+}
+
+// A lane's eight values: neighbours for 16-bit outputs (one 16-byte store); for fp32 four in each half of
+// the row, so that the lanes of a store write consecutive bytes.
 template <typename T, int D, int FMT, int EACH>
 __global__ void __launch_bounds__(KVQ_THREADS)
 kvq_read_kernel(const llmdot_kvq_pool pool, const llmdot_kvq_batch bt, T *__restrict__ xk, T *__restrict__ xv,
@@ -215,6 +245,7 @@ kvq_read_kernel(const llmdot_kvq_pool pool, const llmdot_kvq_batch bt, T *__rest
     kvq_find(pool, bt, (int)row0, s_place);
     __syncthreads();
     if (lane * 8 >= D) return;
+    constexpr int d0 = sizeof(T) == 4 ? 4 : 8, d1 = sizeof(T) == 4 ? D / 2 : 4;  // lane's first value, its second four
     uint2 c[EACH][2];
     float s[EACH][2];
     int64_t at0[EACH], o[EACH];
@@ -224,7 +255,7 @@ kvq_read_kernel(const llmdot_kvq_pool pool, const llmdot_kvq_batch bt, T *__rest
         const uint32_t item = item0 + i * GR + grp;
         row[i] = item / Hk;
         const uint32_t head = item - row[i] * Hk;
-        o[i] = head * D + lane * 8;
+        o[i] = head * D + lane * d0;
         at0[i] = item < items ? s_place[row[i] - row0] : -2;
         const int64_t at = at0[i] + (int64_t)head * KVQ_PAGE;
 #pragma unroll
@@ -232,7 +263,9 @@ kvq_read_kernel(const llmdot_kvq_pool pool, const llmdot_kvq_batch bt, T *__rest
             c[i][v] = make_uint2(0, 0);
             s[i][v] = 0.0f;
             if (at0[i] >= 0) {
-                c[i][v] = __ldg((const uint2 *)((const uint8_t *)(v ? pool.v : pool.k) + at * D + lane * 8));
+                const uint8_t *p = (const uint8_t *)(v ? pool.v : pool.k) + at * D + lane * d0;
+                if (sizeof(T) == 4) c[i][v] = make_uint2(__ldg((const uint32_t *)p), __ldg((const uint32_t *)(p + d1)));
+                else c[i][v] = __ldg((const uint2 *)p);
                 s[i][v] = __ldg((v ? pool.v_scale : pool.k_scale) + at);
             }
         }
@@ -242,12 +275,20 @@ kvq_read_kernel(const llmdot_kvq_pool pool, const llmdot_kvq_batch bt, T *__rest
         if (at0[i] == -2) continue;  // no item, or a row of no sequence
 #pragma unroll
         for (int v = 0; v < 2; v++) {
-            __align__(8) uint8_t b[8];
-            *(uint2 *)b = c[i][v];
-            float f[8];
+            T *to = (v ? xv + row[i] * ldv : xk + row[i] * ldk) + o[i];
+            float f[4], h[4];
+            floats4<FMT>(c[i][v].x, s[i][v], f);
+            floats4<FMT>(c[i][v].y, s[i][v], h);
+            if (at0[i] < 0)
 #pragma unroll
-            for (int e = 0; e < 8; e++) f[e] = at0[i] < 0 ? 0.0f : __fmul_rn(code_value<FMT>(b[e]), s[i][v]);
-            store8((v ? xv + row[i] * ldv : xk + row[i] * ldk) + o[i], wide != 0, f);
+                for (int e = 0; e < 4; e++) f[e] = h[e] = 0.0f;
+            if (sizeof(T) == 4) {
+                store4v(to, wide != 0, f);
+                store4v(to + d1, wide != 0, h);
+            } else {
+                const float x[8] = {f[0], f[1], f[2], f[3], h[0], h[1], h[2], h[3]};
+                store8(to, wide != 0, x);
+            }
         }
     }
 }

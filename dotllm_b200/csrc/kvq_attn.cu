@@ -131,7 +131,7 @@ template <bool SPLIT> __device__ __forceinline__ uint32_t too_large(uint32_t p)
 }
 
 template <int D, int FMT, int NT, bool SPLIT>
-__global__ void __launch_bounds__(NW * 32) kvq_attn_kernel(const __grid_constant__ AttnArgs a)
+__global__ void __launch_bounds__(NW * 32, NT <= 3 && D <= 128 ? 4 : 1) kvq_attn_kernel(const __grid_constant__ AttnArgs a)
 {
     using Sh = Shape<D>;
     constexpr int RT = 8 * NT, QS = D + Sh::QPAD, NQ = SPLIT ? 2 : 1;
@@ -650,14 +650,19 @@ Plan make_plan(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const llmdot
     if (npp == 0) x.nt_p = x.nt_s;
     x.ptiles = (int)up(all_rows, x.wide_p ? wide : 8 * x.nt_p);
     x.rtiles = (int)std::max<int64_t>(1, up(own_rows, x.wide_s ? wide : 8 * x.nt_s));
-    // Chunks.  Narrow: enough CTAs to fill the SMs (five each) about twice over (ragged sequences leave
-    // some without work), at least four pages (fewer leave the join with more to read than the chunks
-    // save), at most 32, so that long and short sequences balance.  Wide: one CTA per SM, at least two pages.
-    const int64_t np = x.wide_p ? 0 : Hk * x.ptiles * npp, ns = x.wide_s ? 0 : Hk * b.batch * x.rtiles * b.max_pages;
-    const int64_t ch = std::min<int64_t>(32, std::max<int64_t>(4, up(np + ns, 148 * 10)));
+    // Chunks.  Narrow: about one CTA per place on the SMs for the prefix, two for the sequences' own pages
+    // (max_pages is a bound: ragged sequences leave some without work), at most 32 pages, so that long
+    // and short sequences balance.  Wide: one CTA per SM, at least two pages.
+    auto places = [&](int nt) {  // CTAs on the SMs: shared memory and registers (as built) of an instance
+        const int d = p.head_dim, nq = a.type == T_F32 ? 2 : 1, bytes = 4 * 64 * d + 1024 + nq * nt * 8 * (d + 168) * 2 + 2048;
+        const int regs = d == 256 ? (nt <= 2 ? 4 : nt == 3 ? 3 : 2) : nt == 1 ? 5 : nt <= 3 ? 4 : nt == 4 ? 3 : 2;
+        return 148 * (int64_t)std::max(1, std::min(regs, 227 * 1024 / bytes));
+    };
+    auto chunk = [&](int64_t pages, int64_t ctas) { return std::min<int64_t>(32, std::max<int64_t>(1, up(pages, ctas))); };
     auto wide_ch = [&](int64_t ctas, int64_t pages) { return std::max<int64_t>(2, up(pages, std::max<int64_t>(1, 148 / std::max<int64_t>(1, ctas)))); };
-    x.ch_p = (int)(x.wide_p ? wide_ch(Hk * x.ptiles, npp) : ch);
-    x.ch_s = (int)(x.wide_s ? wide_ch(Hk * x.rtiles * b.batch, b.max_pages) : ch);
+    x.ch_p = (int)(x.wide_p ? wide_ch(Hk * x.ptiles, npp) : chunk(Hk * x.ptiles * npp, places(x.nt_p)));
+    x.ch_s = (int)(x.wide_s ? wide_ch(Hk * x.rtiles * b.batch, b.max_pages)
+                            : chunk(Hk * b.batch * x.rtiles * b.max_pages, 2 * places(x.nt_s)));
     x.nsp = (int)up(npp, x.ch_p);
     x.nss = (int)std::max<int64_t>(1, up(b.max_pages, x.ch_s));
     x.direct = x.nsp == 0 && x.nss == 1 && !x.wide_s;
