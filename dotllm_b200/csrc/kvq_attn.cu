@@ -131,7 +131,7 @@ template <bool SPLIT> __device__ __forceinline__ uint32_t too_large(uint32_t p)
 }
 
 template <int D, int FMT, int NT, bool SPLIT>
-__global__ void __launch_bounds__(NW * 32, NT <= 3 && D <= 128 ? 4 : 1) kvq_attn_kernel(const __grid_constant__ AttnArgs a)
+__global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 ? 4 : 1) kvq_attn_kernel(const __grid_constant__ AttnArgs a)
 {
     using Sh = Shape<D>;
     constexpr int RT = 8 * NT, QS = D + Sh::QPAD, NQ = SPLIT ? 2 : 1;
@@ -658,11 +658,11 @@ Plan make_plan(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const llmdot
         const int regs = d == 256 ? (nt <= 2 ? 4 : nt == 3 ? 3 : 2) : nt == 1 ? 5 : nt <= 3 ? 4 : nt == 4 ? 3 : 2;
         return 148 * (int64_t)std::max(1, std::min(regs, 227 * 1024 / bytes));
     };
-    auto chunk = [&](int64_t pages, int64_t ctas) { return std::min<int64_t>(32, std::max<int64_t>(1, up(pages, ctas))); };
+    auto chunk = [&](int64_t pages, int64_t ctas, int64_t least) { return std::min<int64_t>(32, std::max<int64_t>(least, up(pages, ctas))); };
     auto wide_ch = [&](int64_t ctas, int64_t pages) { return std::max<int64_t>(2, up(pages, std::max<int64_t>(1, 148 / std::max<int64_t>(1, ctas)))); };
-    x.ch_p = (int)(x.wide_p ? wide_ch(Hk * x.ptiles, npp) : chunk(Hk * x.ptiles * npp, places(x.nt_p)));
+    x.ch_p = (int)(x.wide_p ? wide_ch(Hk * x.ptiles, npp) : chunk(Hk * x.ptiles * npp, places(x.nt_p), 1));
     x.ch_s = (int)(x.wide_s ? wide_ch(Hk * x.rtiles * b.batch, b.max_pages)
-                            : chunk(Hk * b.batch * x.rtiles * b.max_pages, 2 * places(x.nt_s)));
+                            : chunk(Hk * b.batch * x.rtiles * b.max_pages, 2 * places(x.nt_s), 2));
     x.nsp = (int)up(npp, x.ch_p);
     x.nss = (int)std::max<int64_t>(1, up(b.max_pages, x.ch_s));
     x.direct = x.nsp == 0 && x.nss == 1 && !x.wide_s;

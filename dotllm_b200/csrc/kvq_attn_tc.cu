@@ -6,7 +6,7 @@
 // Bound: with hundreds of rows per kv head the products, the exponentials (16 per clock and SM) and
 // the conversion of codes to fp16 take about the same time, and HBM little.  So one CTA takes two tiles of
 // 128 rows (one for head_dim 256) over the same positions -- each code is converted once for 256 rows --
-// and its roles overlap, 128 positions (two pages; one for head_dim 256) at a time:
+// and its roles overlap, 64 positions (a page) at a time:
 //   warps of a tile (4 each)  S from TMEM 64 columns at a time in fragments of 4 rows by 2 columns a lane
 //                             (a lane so needs a quarter of the columns' scales), weights as fp16 back
 //                             into TMEM over S.  The weights are taken relative to a row's reference, 2^6
@@ -16,9 +16,11 @@
 //   4 converting warps        codes from global memory (three K or V pages' loads in flight) to fp16 K
 //                             and V operands in shared memory, scales beside them
 //   1 warp                    one thread issues tcgen05.mma: S = Q K^T and O += P V with P and the
-//                             accumulators in TMEM; while one tile's rows are in their softmax, the other
-//                             tile's products run, and P V starts on the first 64 positions' weights
-// N = 128 in S = Q K^T: a product with N = 64 takes as long (measured 62 clocks and 65, 32 and 64 needed).
+//                             accumulators in TMEM.  S has two places per tile, so that the scores of the next
+//                             page are there when a page's weights are done.  (With one place of two pages the
+//                             products with N = 128 need half the time -- N = 64 takes as long, measured 62
+//                             clocks against 65 -- but a tile's products and its softmax then take turns, and
+//                             the kernel took 1.5 times as long.)
 // Operands in shared memory are rows of 64 values (128 bytes) of one position in 8-row groups, the
 // 16-byte pieces swizzled by the row (piece ^ row % 8), which spreads the converting lanes' stores over all
 // banks: K-major for Q and K, and the same layout read as N-major for V, which so needs no transposing.
@@ -38,8 +40,8 @@ constexpr float HEAD = 6.0f;  // a row's reference stands this power of two abov
 
 template <int D> struct Wide {
     static constexpr int TILES = D == 256 ? 1 : 2;
-    static constexpr int UNP = D == 256 ? 1 : 2, UN = UNP * KVQ_PAGE;  // pages and positions of a unit
-    static constexpr int STAGES = D == 64 ? 3 : 2;
+    static constexpr int UN = KVQ_PAGE;               // positions of a unit
+    static constexpr int STAGES = D == 256 ? 2 : 4;
     static constexpr int THREADS = TILES * 128 + 256;  // rows, converters, products (one warp of four)
     static constexpr uint32_t ROW = 128, GROUP = 8 * ROW;  // bytes of an operand's row, of eight
     static constexpr int KBLK = (D + 63) / 64;             // 64-wide blocks along the head dimension (Q, K)
@@ -47,14 +49,14 @@ template <int D> struct Wide {
     static constexpr uint32_t Q_BYTES = KBLK * Q_BLK, K_BYTES = KBLK * K_BLK;
     static constexpr uint32_t STAGE = 2 * K_BYTES;  // K, then V alike
     static constexpr uint32_t OFF_Q = STAGES * STAGE;
-    static constexpr uint32_t OFF_SC = OFF_Q + TILES * Q_BYTES;  // per stage: K scales, V scales, {rescale, 2^E, bad pages}
+    static constexpr uint32_t OFF_SC = OFF_Q + TILES * Q_BYTES;  // per stage: K scales, V scales, {rescale, 2^E, no page, -}
     static constexpr uint32_t SC_STAGE = 2 * UN * 4 + 16;
     static constexpr uint32_t OFF_BAR = OFF_SC + STAGES * SC_STAGE;
-    // barriers: a stage is converted, read; a tile's S, halves of P, of P V; the drain
-    static constexpr int B_FULL = 0, B_EMPTY = STAGES, B_S = 2 * STAGES, B_P = B_S + TILES, B_O = B_P + TILES * UNP,
-                         B_DRAIN = B_O + TILES * UNP, B_COUNT = B_DRAIN + 1;
+    // barriers: a stage is converted, read; S, P and P V of a tile's two places; the drain
+    static constexpr int B_FULL = 0, B_EMPTY = STAGES, B_S = 2 * STAGES, B_P = B_S + 2 * TILES, B_O = B_P + 2 * TILES,
+                         B_DRAIN = B_O + 2 * TILES, B_COUNT = B_DRAIN + 1;
     static constexpr uint32_t SMEM = OFF_BAR + B_COUNT * 8 + 1024;  // and up to 1 KB to align the operands
-    static constexpr int TILE_COLS = D + UN, C_O = 0, C_S = D;  // TMEM columns
+    static constexpr int TILE_COLS = D + 2 * UN, C_O = 0, C_S = D;  // TMEM columns
     static_assert(TILES * TILE_COLS <= 512, "TMEM columns");
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
@@ -153,6 +155,12 @@ __device__ __forceinline__ uint4 ldg128(const void *p)
     asm volatile("ld.global.nc.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
+__device__ __forceinline__ uint4 lds128(uint32_t a)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w)
 {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -191,7 +199,7 @@ template <int D, int FMT>
 __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __grid_constant__ AttnArgs a, const int qwide)
 {
     using W = Wide<D>;
-    constexpr int STAGES = W::STAGES, UN = W::UN, UNP = W::UNP;
+    constexpr int STAGES = W::STAGES, UN = W::UN;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (1024 - (su32(smem_raw) & 1023)) % 1024;
     __shared__ int s_lo[8], s_hi[8], s_abort;
@@ -233,35 +241,31 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&s_tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // The queries of this warp's 32 rows (16 of them for head_dim 256), four values per lane: on their way
-    // while the rest is set up.
-    constexpr int PARTS = (D + 127) / 128, QROWS = PARTS == 1 ? 32 : 16;
-    uint2 raw[QROWS][PARTS];
-    auto load_queries = [&](int r0) {
-        uint32_t rho = row_first + warp * 32 + r0;
-        int i = rho / (uint32_t)G, hg = rho - i * G;
+    // The queries of this warp's 32 rows go into their operand as they are, 16 bytes at a time, while the
+    // rest is set up; rows that do not exist are zeros.
+    if (tid < SOFT) {
+        const uint32_t rho = row_first + tid;
+        const int i = rho / (uint32_t)G;
+        const int64_t mine = i < sg.nrows ? (sg.r0 + i) * a.ldq + (int64_t)(sg.kvh * G + (rho - i * G)) * D : -1;
+        const uint32_t dst = base + W::OFF_Q + (warp >> 2) * W::Q_BYTES + (warp & 3) * 32 * W::ROW;
+#pragma unroll 2
+        for (int x = lane; x < 4 * D; x += 32) {  // 32 rows of D / 8 pieces
+            const int r = x / (D / 8), c = x % (D / 8);
+            const int64_t from = __shfl_sync(0xffffffffu, mine, r);
+            const uint32_t to = dst + (c >> 3) * W::Q_BLK + r * W::ROW + ((c & 7) ^ (r & 7)) * 16;
+            const uint16_t *src = (const uint16_t *)a.q + (from < 0 ? 0 : from + c * 8);
+            if (qwide) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(from < 0 ? 0 : 16) : "memory");
+            } else {
+                uint32_t w[4] = {};
+                if (from >= 0)
 #pragma unroll
-        for (int r = 0; r < QROWS; r++) {
-            const uint16_t *q = (const uint16_t *)a.q + (sg.r0 + i) * a.ldq + (int64_t)(sg.kvh * G + hg) * D + lane * 4;
-            const bool real = i < sg.nrows;
-#pragma unroll
-            for (int x = 0; x < PARTS; x++) {
-                const bool on = real && lane * 4 + 128 * x < D;
-                raw[r][x] = make_uint2(0, 0);
-                if (qwide) {
-                    if (on) raw[r][x] = __ldg((const uint2 *)(q + 128 * x));
-                } else if (on) {
-                    const uint16_t *p = q + 128 * x;
-                    raw[r][x] = make_uint2(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16);
-                }
-            }
-            if (++hg == G) {
-                hg = 0;
-                i++;
+                    for (int k = 0; k < 4; k++) w[k] = src[2 * k] | (uint32_t)src[2 * k + 1] << 16;
+                sts128(to, w[0], w[1], w[2], w[3]);
             }
         }
-    };
-    if (tid < SOFT) load_queries(0);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
     // (the operands' memory holds the sequences' tables meanwhile)
     const SeqTable seqs = load_seqs(a, sg, (int32_t *)smem, W::THREADS);
     int row = -1, lo = 0, hi = 0x7fffffff;
@@ -284,9 +288,9 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
         lo_min = min(lo_min, s_lo[w]);
         hi_max = max(hi_max, s_hi[w]);
     }
-    // pages [u0, u1) in n units
+    // pages [u0, u1)
     const int u0 = max(sg.chunk * sg.ch, lo_min / KVQ_PAGE);
-    const int u1 = min((sg.chunk + 1) * sg.ch, hi_max < 0 ? 0 : hi_max / KVQ_PAGE + 1), n = (max(u1 - u0, 0) + UNP - 1) / UNP;
+    const int u1 = min((sg.chunk + 1) * sg.ch, hi_max < 0 ? 0 : hi_max / KVQ_PAGE + 1), n = max(u1 - u0, 0);
 
     // Registers: 16 warps start with 128 each (2048 warp-registers in all); the row warps hold two pieces of
     // scores and need more: 8 * 152 + 4 * 128 + 4 * 80 = 2048.
@@ -295,43 +299,39 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
         if (W::TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
         const int tile = warp >> 2, head = sg.kvh * G + (row_first + tid) % G;
         const uint32_t tm = tmem + tile * W::TILE_COLS + ((uint32_t)(32 * (warp & 3)) << 16);
-        // the queries as an operand: fp16 ones as they are, bf16 ones scaled by a power of two each (zeros for rows
-        // that do not exist); a negative scale's sign goes into them
+        // bf16 queries become fp16 ones, scaled by a power of two per row; a negative scale's sign goes into the query
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncwarp();
         int e = 0;
-        const uint32_t qdst = base + W::OFF_Q + tile * W::Q_BYTES + (warp & 3) * 32 * W::ROW + (lane & 1) * 8;
-        const bool negative = a.at.scale < 0.0f;
-        auto put_query = [&](int r, int x, uint32_t lo, uint32_t hi) {
-            const uint32_t flip = negative ? 0x80008000u : 0u, piece = lane / 2 + 16 * x;
-            if (lane * 4 + 128 * x < D)
-                asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(qdst + (piece >> 3) * W::Q_BLK + r * W::ROW + ((piece & 7) ^ (r & 7)) * 16),
-                             "r"(lo ^ flip), "r"(hi ^ flip)
-                             : "memory");
-        };
-#pragma unroll
-        for (int r0 = 0; r0 < 32; r0 += QROWS) {
-            if (r0 > 0) load_queries(r0);
+        if (a.at.type != T_F16 || a.at.scale < 0.0f) {
+            const uint32_t mine = base + W::OFF_Q + tile * W::Q_BYTES + (tid & 127) * W::ROW;
+            const uint32_t flip = a.at.scale < 0.0f ? 0x80008000u : 0u;
+            auto piece = [&](int c) { return mine + (c >> 3) * W::Q_BLK + ((c & 7) ^ (lane & 7)) * 16; };
             if (a.at.type == T_F16) {
-#pragma unroll
-                for (int r = 0; r < QROWS; r++)
-#pragma unroll
-                    for (int x = 0; x < PARTS; x++) put_query(r0 + r, x, raw[r][x].x, raw[r][x].y);
+#pragma unroll 4
+                for (int c = 0; c < D / 8; c++) {
+                    const uint4 v = lds128(piece(c));
+                    sts128(piece(c), v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+                }
             } else {
+                uint32_t top = 0;  // magnitudes order as integers, NaN above all
+#pragma unroll 4
+                for (int c = 0; c < D / 8; c++) {
+                    const uint4 v = lds128(piece(c));
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (int r = 0; r < QROWS; r++) {
-                    uint32_t top = 0;  // magnitudes order as integers, NaN above all
+                    for (int k = 0; k < 4; k++) top = max(top, max((w[k] << 16) & 0x7fffffffu, w[k] & 0x7fff0000u));
+                }
+                e = row_exponent(__uint_as_float(top));
+                const float up = pow2(e);
+#pragma unroll 4
+                for (int c = 0; c < D / 8; c++) {
+                    const uint4 v = lds128(piece(c));
+                    const uint32_t w[4] = {v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip};
+                    uint32_t h[4];
 #pragma unroll
-                    for (int x = 0; x < PARTS; x++) {
-                        top = max(top, max((raw[r][x].x << 16) & 0x7fffffffu, raw[r][x].x & 0x7fff0000u));
-                        top = max(top, max((raw[r][x].y << 16) & 0x7fffffffu, raw[r][x].y & 0x7fff0000u));
-                    }
-                    const int er = row_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, top)));
-                    if (lane == r0 + r) e = er;
-                    const float up = pow2(er);
-#pragma unroll
-                    for (int x = 0; x < PARTS; x++)
-                        put_query(r0 + r, x,
-                                  pack(__uint_as_float(raw[r][x].x << 16) * up, __uint_as_float(raw[r][x].x & 0xFFFF0000u) * up),
-                                  pack(__uint_as_float(raw[r][x].y << 16) * up, __uint_as_float(raw[r][x].y & 0xFFFF0000u) * up));
+                    for (int k = 0; k < 4; k++) h[k] = pack(__uint_as_float(w[k] << 16) * up, __uint_as_float(w[k] & 0xFFFF0000u) * up);
+                    sts128(piece(c), h[0], h[1], h[2], h[3]);
                 }
             }
         }
@@ -358,9 +358,9 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             l[k] = f2(0.0f, 0.0f);
         }
         bool ok = tile < nact;
-        // O times f (lane = row), once the products that add to it (through half `half` of unit `unit`) are complete.
-        auto rescale_o = [&](int unit, int half, float f) {
-            ok = wait(W::B_O + tile * UNP + half, unit & 1);
+        // O times f (lane = row), once the products that add to it (through unit i) are complete.
+        auto rescale_o = [&](int i, float f) {
+            ok = wait(W::B_O + tile * 2 + (i & 1), (i >> 1) & 1);
             if (!(ok = __all_sync(0xffffffffu, ok))) return;
             fence_after();
             const F2 ff = f2(f, f);
@@ -381,19 +381,19 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             }
             tmem_st_wait();
         };
-        auto hand_over = [&](int half, const uint32_t (&p)[2][16]) {  // 64 positions' weights, over scores that were read
-            tmem_st_frag(tm + W::C_S + 32 * half, p[0]);
-            tmem_st_frag(tm + (16u << 16) + W::C_S + 32 * half, p[1]);
+        auto hand_over = [&](int buf, const uint32_t (&p)[2][16]) {  // a page's weights, over scores that were read
+            tmem_st_frag(tm + W::C_S + 64 * buf, p[0]);
+            tmem_st_frag(tm + (16u << 16) + W::C_S + 64 * buf, p[1]);
             tmem_st_wait();
             fence_before();
-            bar_arrive(bars + 8 * (W::B_P + tile * UNP + half));
+            bar_arrive(bars + 8 * (W::B_P + tile * 2 + buf));
         };
-        // Half a unit whose rows see every position, without a cap: false (and nothing done) when a weight
+        // A page that the rows see whole, without a cap: false (and nothing done) when a weight
         // reaches 2 and the reference has to rise.
-        auto plain_half = [&](const float *ks, const float *vs, int half) -> bool {
+        auto plain_page = [&](const float *ks, const float *vs, int buf) -> bool {
             uint32_t s[2][32], p[2][16], any = 0;
-            tmem_ld_frag(tm + W::C_S + 64 * half, s[0]);
-            tmem_ld_frag(tm + (16u << 16) + W::C_S + 64 * half, s[1]);
+            tmem_ld_frag(tm + W::C_S + 64 * buf, s[0]);
+            tmem_ld_frag(tm + (16u << 16) + W::C_S + 64 * buf, s[1]);
             F2 q2[4], off[4], sum[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float2 kf = *(const float2 *)(ks + 64 * half + 8 * i + 2 * t), vf = *(const float2 *)(vs + 64 * half + 8 * i + 2 * t);
+                const float2 kf = *(const float2 *)(ks + 8 * i + 2 * t), vf = *(const float2 *)(vs + 8 * i + 2 * t);
                 const F2 k2 = f2(kf.x, kf.y), v2 = f2(vf.x, vf.y);
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
@@ -420,23 +420,23 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             if (__any_sync(0xffffffffu, (any & 0x40004000u) != 0)) return false;  // an exponent bit: 2 or more (or a NaN)
 #pragma unroll
             for (int k = 0; k < 4; k++) l[k] = add2(l[k], sum[k]);
-            hand_over(half, p);
+            hand_over(buf, p);
             return true;
         };
-        // The search for the rows' maxima over half a unit, and the references raised where they stand less than
+        // The search for the rows' maxima over a page, and the references raised where they stand less than
         // HEAD above.  MASKED: scores of positions that a row does not see do not count.
-        auto search = [&](int i, const float *ks, int half, auto masked) {
+        auto search = [&](int i, const float *ks, int buf, auto masked) {
             constexpr bool MASKED = decltype(masked)::value;
-            const int j0 = u0 * KVQ_PAGE + i * UN + 64 * half + 2 * t;
+            const int j0 = u0 * KVQ_PAGE + i * UN + 2 * t;
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 uint32_t s[32];
-                tmem_ld_frag(tm + ((uint32_t)(16 * h) << 16) + W::C_S + 64 * half, s);
+                tmem_ld_frag(tm + ((uint32_t)(16 * h) << 16) + W::C_S + 64 * buf, s);
                 tmem_ld_wait();
 #pragma unroll
                 for (int c = 0; c < 8; c++) {
-                    const float2 kf = *(const float2 *)(ks + 64 * half + 8 * c + 2 * t);
+                    const float2 kf = *(const float2 *)(ks + 8 * c + 2 * t);
                     const int j = j0 + 8 * c;
 #pragma unroll
                     for (int r = 0; r < 2; r++) {
@@ -469,29 +469,28 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                 }
                 l[k] = mul2(l[k], f2(f[k], f[k]));
             }
-            if ((i > 0 || half > 0) && __any_sync(0xffffffffu, moved)) {
+            if (i > 0 && __any_sync(0xffffffffu, moved)) {
                 float mine = 1.0f;  // of the row that is this lane
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const float x = __shfl_sync(0xffffffffu, f[k], (lane & 7) * 4);
                     if (lane >> 3 == k) mine = x;
                 }
-                // O holds the units before this one, and this one's first half once that is handed over
-                rescale_o(half > 0 ? i : i - 1, half > 0 ? half - 1 : UNP - 1, mine);
+                rescale_o(i - 1, mine);
             }
         };
-        // The weights of half a unit, with masks and cap.
-        auto masked_half = [&](int i, const float *ks, const float *vs, int half) {
-            const int j0 = u0 * KVQ_PAGE + i * UN + 64 * half + 2 * t;
+        // The weights of a page, with masks and cap.
+        auto masked_page = [&](int i, const float *ks, const float *vs, int buf) {
+            const int j0 = u0 * KVQ_PAGE + i * UN + 2 * t;
             uint32_t p[2][16];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 uint32_t s[32];
-                tmem_ld_frag(tm + ((uint32_t)(16 * h) << 16) + W::C_S + 64 * half, s);
+                tmem_ld_frag(tm + ((uint32_t)(16 * h) << 16) + W::C_S + 64 * buf, s);
                 tmem_ld_wait();
 #pragma unroll
                 for (int c = 0; c < 8; c++) {
-                    const float2 kf = *(const float2 *)(ks + 64 * half + 8 * c + 2 * t), vf = *(const float2 *)(vs + 64 * half + 8 * c + 2 * t);
+                    const float2 kf = *(const float2 *)(ks + 8 * c + 2 * t), vf = *(const float2 *)(vs + 8 * c + 2 * t);
 #pragma unroll
                     for (int r = 0; r < 2; r++) {
                         const int k = 2 * h + r, j = j0 + 8 * c;
@@ -509,39 +508,37 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                     }
                 }
             }
-            hand_over(half, p);
+            hand_over(buf, p);
         };
+        bool known = false;  // every row of the warp has seen a position
         for (int i = 0; i < n && ok; i++) {
-            const int st = i % STAGES;
-            ok = wait(W::B_S + tile, i & 1) && wait(W::B_FULL + st, (i / STAGES) & 1);
+            const int st = i % STAGES, buf = i & 1, p0 = u0 * KVQ_PAGE + i * UN;
+            ok = wait(W::B_S + tile * 2 + buf, (i >> 1) & 1) && wait(W::B_FULL + st, (i / STAGES) & 1);
             if (!(ok = __all_sync(0xffffffffu, ok))) break;
             fence_after();
-            const float *ks = (const float *)(smem + W::OFF_SC + st * W::SC_STAGE), *vs = ks + UN, *ex = vs + UN;
-            const int t0 = u0 * KVQ_PAGE + i * UN;
-            vpow = ex[1];
-            if (i > 0 && ex[0] != 1.0f) {  // the values' unit rose: O follows (every row alike)
-                rescale_o(i - 1, UNP - 1, ex[0]);
+            const float *ks = (const float *)(smem + W::OFF_SC + st * W::SC_STAGE), *vs = ks + UN;
+            const float4 ex = *(const float4 *)(vs + UN);
+            vpow = ex.y;
+            if (i > 0 && ex.x != 1.0f) {  // the values' unit rose: O follows (every row alike)
+                rescale_o(i - 1, ex.x);
                 if (!ok) break;
             }
-            const bool known = __all_sync(0xffffffffu, fminf(fminf(ref[0], ref[1]), fminf(ref[2], ref[3])) > -INFINITY);
-#pragma unroll 1
-            for (int half = 0; half < UNP && ok; half++) {
-                const int p0 = t0 + 64 * half;
-                if (ex[2 + half] != 0.0f || p0 > hi_end || p0 + KVQ_PAGE <= lo_min) {  // nothing for this warp's rows
-                    const uint32_t zero[2][16] = {};
-                    hand_over(half, zero);
-                } else if (!cap && p0 >= lo_max && p0 + KVQ_PAGE - 1 <= hi_min) {  // everything
-                    if ((known || half > 0) && plain_half(ks, vs, half)) continue;
-                    search(i, ks, half, std::false_type{});
-                    if (ok && !plain_half(ks, vs, half)) masked_half(i, ks, vs, half);  // (a NaN stays one)
-                } else {
-                    search(i, ks, half, std::true_type{});
-                    if (ok) masked_half(i, ks, vs, half);
-                }
+            if (ex.z != 0.0f || p0 > hi_end || p0 + KVQ_PAGE <= lo_min) {  // nothing for this warp's rows
+                const uint32_t zero[2][16] = {};
+                hand_over(buf, zero);
+            } else if (!cap && p0 >= lo_max && p0 + KVQ_PAGE - 1 <= hi_min) {  // everything
+                if (known && plain_page(ks, vs, buf)) continue;
+                search(i, ks, buf, std::false_type{});
+                known = true;
+                if (ok && !plain_page(ks, vs, buf)) masked_page(i, ks, vs, buf);  // (a NaN stays one)
+            } else {
+                search(i, ks, buf, std::true_type{});
+                if (ok) masked_page(i, ks, vs, buf);
+                known = __all_sync(0xffffffffu, fminf(fminf(ref[0], ref[1]), fminf(ref[2], ref[3])) > -INFINITY);
             }
         }
         if (ok && n > 0) {
-            ok = wait(W::B_O + tile * UNP + UNP - 1, (n - 1) & 1);
+            ok = wait(W::B_O + tile * 2 + ((n - 1) & 1), ((n - 1) >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
         }
         const int64_t RH = (int64_t)a.bt.rows * a.at.heads, slot = sg.pre ? sg.chunk : a.nsp + sg.chunk;
@@ -603,59 +600,49 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
 #pragma unroll
             for (int i = 0; i < T; i++) x.c[i] = ldg128(p + 2048 * i);
         };
-        // a unit's scales: warp 0 V's, warp 1 K's; lane: positions lane, lane + 32, ...
-        auto load_scales = [&](int page0, int page1, float (&c)[2 * UNP]) {
+        // a page's scales: warp 0 V's, warp 1 K's; lane: positions lane and lane + 32
+        auto load_scales = [&](int page, float (&c)[2]) {
             if (dw >= 2) return;
-#pragma unroll
-            for (int x = 0; x < UNP; x++) {
-                const int page = x ? page1 : page0;
-                const float *s = (dw == 0 ? a.pool.v_scale : a.pool.k_scale) + ((int64_t)page * Hk + sg.kvh) * KVQ_PAGE + lane;
-                c[2 * x] = none(page) ? 0.0f : __ldg(s);
-                c[2 * x + 1] = none(page) ? 0.0f : __ldg(s + 32);
-            }
+            const float *s = (dw == 0 ? a.pool.v_scale : a.pool.k_scale) + ((int64_t)page * Hk + sg.kvh) * KVQ_PAGE + lane;
+            c[0] = none(page) ? 0.0f : __ldg(s);
+            c[1] = none(page) ? 0.0f : __ldg(s + 32);
         };
         float vp = 0.0f;  // 2^E (warp 0)
         bool ok = true;
-        auto put_scales = [&](int i, int page0, int page1, const float (&c)[2 * UNP]) {
-            float *ks = (float *)(smem + W::OFF_SC + i % STAGES * W::SC_STAGE), *vs = ks + UN, *ex = vs + UN;
+        auto put_scales = [&](int i, int page, const float (&c)[2]) {
+            float *ks = (float *)(smem + W::OFF_SC + i % STAGES * W::SC_STAGE), *vs = ks + UN;
             if (dw == 0) {
                 const int t0 = u0 * KVQ_PAGE + i * UN + lane;
                 float top = 0.0f;  // of positions that exist; a NaN does not count
-#pragma unroll
-                for (int x = 0; x < 2 * UNP; x++)
-                    if (t0 + 32 * x < len) top = fmaxf(top, c[x] * code_unit<FMT>());
+                if (t0 < len) top = fmaxf(top, c[0] * code_unit<FMT>());
+                if (t0 + 32 < len) top = fmaxf(top, c[1] * code_unit<FMT>());
                 const float pw = scale_pow(warp_max(top));
                 float ve = 1.0f;
                 if (i == 0) {
                     vp = pw;
-                } else if (pw > vp * 8.0f) {  // weights stay below 2^8 * 2 * 8
+                } else if (pw > vp * 8.0f) {  // weights stay far below 2
                     ve = vp * pow_inverse(pw);
                     vp = pw;
                 }
                 const float inv = pow_inverse(vp);
-#pragma unroll
-                for (int x = 0; x < 2 * UNP; x++) vs[lane + 32 * x] = c[x] * code_unit<FMT>() * inv;
-                if (lane == 0) {
-                    ex[0] = ve;
-                    ex[1] = vp;
-                    ex[2] = none(page0) ? 1.0f : 0.0f;
-                    ex[3] = UNP > 1 && none(page1) ? 1.0f : 0.0f;
-                }
+                vs[lane] = c[0] * code_unit<FMT>() * inv;
+                vs[lane + 32] = c[1] * code_unit<FMT>() * inv;
+                if (lane == 0) *(float4 *)(vs + UN) = make_float4(ve, vp, none(page) ? 1.0f : 0.0f, 0.0f);
             } else if (dw == 1) {
-#pragma unroll
-                for (int x = 0; x < 2 * UNP; x++) ks[lane + 32 * x] = c[x];
+                ks[lane] = c[0];
+                ks[lane + 32] = c[1];
             }
         };
-        // K or V of page h of the segment's share: half h % UNP of unit h / UNP
-        auto convert = [&](int h, bool v, const Codes &x) {
-            const uint32_t d = base + h / UNP % STAGES * W::STAGE + h % UNP * KVQ_PAGE * W::ROW + (v ? W::K_BYTES : 0u);
+        // K or V of unit i
+        auto convert = [&](int i, bool v, const Codes &x) {
+            const uint32_t d = base + i % STAGES * W::STAGE + (v ? W::K_BYTES : 0u);
 #pragma unroll
-            for (int i = 0; i < T; i++) {
+            for (int k = 0; k < T; k++) {
                 // piece t: position r, codes 16 ch ..: two operand pieces of 8.  Lanes of the upper half of a
                 // 128-code row write them in the other order, so that eight lanes meet eight banks.
-                const int t = dt + 128 * i, ch = t % (D / 16), r = t / (D / 16), pc = (ch & 3) * 2, swap = (ch >> 2) & 1;
+                const int t = dt + 128 * k, ch = t % (D / 16), r = t / (D / 16), pc = (ch & 3) * 2, swap = (ch >> 2) & 1;
                 const uint32_t to = d + (ch >> 2) * W::K_BLK + r * W::ROW;
-                const uint4 c = x.c[i];
+                const uint4 c = x.c[k];
                 const uint32_t w[4] = {(swap ? c.z : c.x) ^ code_flip<FMT>(), (swap ? c.w : c.y) ^ code_flip<FMT>(),
                                        (swap ? c.x : c.z) ^ code_flip<FMT>(), (swap ? c.y : c.w) ^ code_flip<FMT>()};
                 sts128(to + ((pc + swap) ^ (r & 7)) * 16, codes2<FMT, 0, 1>(w[0]), codes2<FMT, 2, 3>(w[0]), codes2<FMT, 0, 1>(w[1]),
@@ -666,12 +653,12 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
         };
         // four sets of registers in turn, three loads ahead (a copy between sets would wait for them)
         Codes k0, v0, k1, v1;
-        float sc[2 * UNP];
+        float sc[2];
         int p0 = page_of(u0), p1 = page_of(u0 + 1), p2 = page_of(u0 + 2), p3 = page_of(u0 + 3);
         load(p0, false, k0);
         load(p0, true, v0);
         load(p1, false, k1);
-        load_scales(p0, p1, sc);
+        load_scales(p0, sc);
         __syncthreads();
         auto slot = [&](int i) {
             if (i < STAGES) return true;
@@ -682,28 +669,25 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // operands: generic writes -> tensor core
             bar_arrive(bars + 8 * (W::B_FULL + i % STAGES));
         };
-        for (int h = 0; h < n * UNP && ok; h += 2) {  // two pages a round: one unit, or two of one page
-            const int i = h / UNP, p4 = page_of(u0 + h + 4), p5 = page_of(u0 + h + 5);
+        for (int i = 0; i < n && ok; i += 2) {  // two pages a round
+            const int p4 = page_of(u0 + i + 4), p5 = page_of(u0 + i + 5);
             load(p1, true, v1);
             if (!slot(i)) break;
-            put_scales(i, p0, p1, sc);
-            if (UNP == 2) load_scales(p2, p3, sc);
-            else load_scales(p1, p1, sc);
-            convert(h, false, k0);
+            put_scales(i, p0, sc);
+            load_scales(p1, sc);
+            convert(i, false, k0);
             load(p2, false, k0);
-            convert(h, true, v0);
-            if (UNP == 1) {
-                done(i);
-                if (h + 1 >= n) break;
-                if (!slot(i + 1)) break;
-                put_scales(i + 1, p1, p1, sc);
-                load_scales(p2, p2, sc);
-            }
+            convert(i, true, v0);
+            done(i);
+            if (i + 1 >= n) break;
             load(p2, true, v0);
-            convert(h + 1, false, k1);
+            if (!slot(i + 1)) break;
+            put_scales(i + 1, p1, sc);
+            load_scales(p2, sc);
+            convert(i + 1, false, k1);
             load(p3, false, k1);
-            convert(h + 1, true, v1);
-            done(UNP == 1 ? i + 1 : i);
+            convert(i + 1, true, v1);
+            done(i + 1);
             p0 = p2;
             p1 = p3;
             p2 = p4;
@@ -717,41 +701,44 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             fence_after();
             // descriptors differ in their address field (units of 16 bytes): one addition each
             const uint64_t qd = sdesc(base + W::OFF_Q), kd = sdesc(base), vd = sdesc(base + W::K_BYTES, W::K_BLK);
-            auto qk = [&](int t, int st) {
-                const uint64_t q = qd + t * (W::Q_BYTES / 16), k = kd + st * (W::STAGE / 16);
-                const uint32_t d = tmem + t * W::TILE_COLS + W::C_S;
+            auto qk = [&](int t, int i) {
+                const uint64_t q = qd + t * (W::Q_BYTES / 16), k = kd + i % STAGES * (W::STAGE / 16);
+                const uint32_t d = tmem + t * W::TILE_COLS + W::C_S + 64 * (i & 1);
 #pragma unroll
                 for (int kk = 0; kk < D / 16; kk++)
                     umma_ss<UN>(d, q + (kk / 4 * W::Q_BLK + kk % 4 * 32) / 16, k + (kk / 4 * W::K_BLK + kk % 4 * 32) / 16, kk != 0);
-                umma_commit(bars + 8 * (W::B_S + t));
+                umma_commit(bars + 8 * (W::B_S + t * 2 + (i & 1)));
             };
-            bool ok = wait(W::B_FULL, 0);
-            fence_after();
-            for (int t = 0; t < nact && ok; t++) qk(t, 0);
+            bool ok = true;
+            for (int i = 0; i < 2 && i < n && ok; i++) {
+                if (!(ok = wait(W::B_FULL + i, 0))) break;
+                fence_after();
+                for (int t = 0; t < nact; t++) qk(t, i);
+            }
             for (int i = 0; i < n && ok; i++) {
-                const int st = i % STAGES, nx = (i + 1) % STAGES;
+                const uint64_t v = vd + i % STAGES * (W::STAGE / 16);
                 for (int t = 0; t < nact; t++) {
-                    const uint64_t v = vd + st * (W::STAGE / 16);
+                    if (!(ok = wait(W::B_P + t * 2 + (i & 1), (i >> 1) & 1))) break;
+                    fence_after();
                     const uint32_t tm = tmem + t * W::TILE_COLS;
 #pragma unroll
-                    for (int hf = 0; hf < UNP && ok; hf++) {
-                        if (!(ok = wait(W::B_P + t * UNP + hf, i & 1))) break;
-                        fence_after();
-#pragma unroll
-                        for (int kk = 0; kk < KVQ_PAGE / 16; kk++)
-                            umma_ts<D>(tm + W::C_O, tm + W::C_S + 32 * hf + 8 * kk,
-                                       v + (hf * 4 + kk) * 2 * W::GROUP / 16, i != 0 || hf != 0 || kk != 0);
-                        umma_commit(bars + 8 * (W::B_O + t * UNP + hf));
-                    }
-                    if (!ok) break;
-                    if (t == nact - 1) umma_commit(bars + 8 * (W::B_EMPTY + st));
-                    if (i + 1 < n) {
+                    for (int kk = 0; kk < UN / 16; kk++)
+                        umma_ts<D>(tm + W::C_O, tm + W::C_S + 64 * (i & 1) + 8 * kk, v + kk * 2 * W::GROUP / 16, i != 0 || kk != 0);
+                    umma_commit(bars + 8 * (W::B_O + t * 2 + (i & 1)));
+                    if (t == nact - 1) umma_commit(bars + 8 * (W::B_EMPTY + i % STAGES));
+                    if (i + 2 < n) {  // the scores that this page's weights leave room for
                         if (t == 0) {
-                            if (!(ok = wait(W::B_FULL + nx, ((i + 1) / STAGES) & 1))) break;
+                            // (with two stages the page after next is converted only once this one is read)
+                            if (STAGES > 2 && !(ok = wait(W::B_FULL + (i + 2) % STAGES, ((i + 2) / STAGES) & 1))) break;
                             fence_after();
                         }
-                        qk(t, nx);
+                        if (STAGES > 2) qk(t, i + 2);
                     }
+                }
+                if (STAGES == 2 && ok && i + 2 < n) {
+                    if (!(ok = wait(W::B_FULL + i % STAGES, ((i + 2) / STAGES) & 1))) break;
+                    fence_after();
+                    for (int t = 0; t < nact; t++) qk(t, i + 2);
                 }
             }
             // every product issued completes before the TMEM is released
