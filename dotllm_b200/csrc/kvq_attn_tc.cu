@@ -15,7 +15,7 @@
 //                             after the first positions is rare
 //   4 converting warps        codes from global memory (three K or V pages' loads in flight) to fp16 K
 //                             and V operands in shared memory, scales beside them
-//   1 warp                    one thread issues tcgen05.mma: S = Q K^T and O += P V with P and the
+//   1 warp per tile           one thread issues tcgen05.mma: S = Q K^T and O += P V with P and the
 //                             accumulators in TMEM.  S has two places per tile, so that the scores of the next
 //                             page are there when a page's weights are done.  (With one place of two pages the
 //                             products with N = 128 need half the time -- N = 64 takes as long, measured 62
@@ -42,7 +42,7 @@ template <int D> struct Wide {
     static constexpr int TILES = D == 256 ? 1 : 2;
     static constexpr int UN = KVQ_PAGE;               // positions of a unit
     static constexpr int STAGES = D == 256 ? 2 : 4;
-    static constexpr int THREADS = TILES * 128 + 256;  // rows, converters, products (one warp of four)
+    static constexpr int THREADS = TILES * 128 + 256;  // rows, converters, products (a warp per tile, of four)
     static constexpr uint32_t ROW = 128, GROUP = 8 * ROW;  // bytes of an operand's row, of eight
     static constexpr int KBLK = (D + 63) / 64;             // 64-wide blocks along the head dimension (Q, K)
     static constexpr uint32_t Q_BLK = 128 * ROW, K_BLK = UN * ROW;
@@ -54,7 +54,7 @@ template <int D> struct Wide {
     static constexpr uint32_t OFF_BAR = OFF_SC + STAGES * SC_STAGE;
     // barriers: a stage is converted, read; S, P and P V of a tile's two places; the drain
     static constexpr int B_FULL = 0, B_EMPTY = STAGES, B_S = 2 * STAGES, B_P = B_S + 2 * TILES, B_O = B_P + 2 * TILES,
-                         B_DRAIN = B_O + 2 * TILES, B_COUNT = B_DRAIN + 1;
+                         B_DRAIN = B_O + 2 * TILES, B_COUNT = B_DRAIN + TILES;
     static constexpr uint32_t SMEM = OFF_BAR + B_COUNT * 8 + 1024;  // and up to 1 KB to align the operands
     static constexpr int TILE_COLS = D + 2 * UN, C_O = 0, C_S = D;  // TMEM columns
     static_assert(TILES * TILE_COLS <= 512, "TMEM columns");
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
     constexpr int SOFT = W::TILES * 128;
     if (tid == SOFT) {
         for (int i = 0; i < W::B_COUNT; i++)
-            bar_init(bars + 8 * i, i < STAGES || (i >= W::B_P && i < W::B_O) ? 128u : 1u);
+            bar_init(bars + 8 * i, i < STAGES || (i >= W::B_P && i < W::B_O) ? 128u : i < 2 * STAGES ? (uint32_t)nact : 1u);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -697,54 +697,41 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
         // ------------------------------------------------------------ products
         if (W::TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         __syncthreads();
-        if (warp == SOFT / 32 + 4 && lane == 0 && n > 0) {
+        const int t = warp - (SOFT / 32 + 4);  // each tile's products are issued by a thread of its own
+        if (t < nact && lane == 0 && n > 0) {
             fence_after();
             // descriptors differ in their address field (units of 16 bytes): one addition each
-            const uint64_t qd = sdesc(base + W::OFF_Q), kd = sdesc(base), vd = sdesc(base + W::K_BYTES, W::K_BLK);
-            auto qk = [&](int t, int i) {
-                const uint64_t q = qd + t * (W::Q_BYTES / 16), k = kd + i % STAGES * (W::STAGE / 16);
-                const uint32_t d = tmem + t * W::TILE_COLS + W::C_S + 64 * (i & 1);
+            const uint64_t qd = sdesc(base + W::OFF_Q + t * W::Q_BYTES), kd = sdesc(base), vd = sdesc(base + W::K_BYTES, W::K_BLK);
+            const uint32_t tm = tmem + t * W::TILE_COLS, bs = bars + 8 * (W::B_S + t * 2), bo = bars + 8 * (W::B_O + t * 2);
+            bool ok = true;
+            auto qk = [&](int i) {
+                ok = wait(W::B_FULL + i % STAGES, (i / STAGES) & 1);
+                if (!ok) return;
+                fence_after();
+                const uint64_t k = kd + i % STAGES * (W::STAGE / 16);
 #pragma unroll
                 for (int kk = 0; kk < D / 16; kk++)
-                    umma_ss<UN>(d, q + (kk / 4 * W::Q_BLK + kk % 4 * 32) / 16, k + (kk / 4 * W::K_BLK + kk % 4 * 32) / 16, kk != 0);
-                umma_commit(bars + 8 * (W::B_S + t * 2 + (i & 1)));
+                    umma_ss<UN>(tm + W::C_S + 64 * (i & 1), qd + (kk / 4 * W::Q_BLK + kk % 4 * 32) / 16,
+                                k + (kk / 4 * W::K_BLK + kk % 4 * 32) / 16, kk != 0);
+                umma_commit(bs + 8 * (i & 1));
             };
-            bool ok = true;
-            for (int i = 0; i < 2 && i < n && ok; i++) {
-                if (!(ok = wait(W::B_FULL + i, 0))) break;
-                fence_after();
-                for (int t = 0; t < nact; t++) qk(t, i);
-            }
+            qk(0);
+            if (n > 1 && ok) qk(1);
             for (int i = 0; i < n && ok; i++) {
+                if (!(ok = wait(W::B_P + t * 2 + (i & 1), (i >> 1) & 1))) break;
+                fence_after();
                 const uint64_t v = vd + i % STAGES * (W::STAGE / 16);
-                for (int t = 0; t < nact; t++) {
-                    if (!(ok = wait(W::B_P + t * 2 + (i & 1), (i >> 1) & 1))) break;
-                    fence_after();
-                    const uint32_t tm = tmem + t * W::TILE_COLS;
 #pragma unroll
-                    for (int kk = 0; kk < UN / 16; kk++)
-                        umma_ts<D>(tm + W::C_O, tm + W::C_S + 64 * (i & 1) + 8 * kk, v + kk * 2 * W::GROUP / 16, i != 0 || kk != 0);
-                    umma_commit(bars + 8 * (W::B_O + t * 2 + (i & 1)));
-                    if (t == nact - 1) umma_commit(bars + 8 * (W::B_EMPTY + i % STAGES));
-                    if (i + 2 < n) {  // the scores that this page's weights leave room for
-                        if (t == 0) {
-                            // (with two stages the page after next is converted only once this one is read)
-                            if (STAGES > 2 && !(ok = wait(W::B_FULL + (i + 2) % STAGES, ((i + 2) / STAGES) & 1))) break;
-                            fence_after();
-                        }
-                        if (STAGES > 2) qk(t, i + 2);
-                    }
-                }
-                if (STAGES == 2 && ok && i + 2 < n) {
-                    if (!(ok = wait(W::B_FULL + i % STAGES, ((i + 2) / STAGES) & 1))) break;
-                    fence_after();
-                    for (int t = 0; t < nact; t++) qk(t, i + 2);
-                }
+                for (int kk = 0; kk < UN / 16; kk++)
+                    umma_ts<D>(tm + W::C_O, tm + W::C_S + 64 * (i & 1) + 8 * kk, v + kk * 2 * W::GROUP / 16, i != 0 || kk != 0);
+                umma_commit(bo + 8 * (i & 1));
+                umma_commit(bars + 8 * (W::B_EMPTY + i % STAGES));
+                if (i + 2 < n) qk(i + 2);  // the scores that this page's weights leave room for
             }
             // every product issued completes before the TMEM is released
-            umma_commit(bars + 8 * W::B_DRAIN);
+            umma_commit(bars + 8 * (W::B_DRAIN + t));
             const long long t0 = clock64();
-            while (!bar_try(bars + 8 * W::B_DRAIN, 0) && clock64() - t0 < WAIT_CLOCKS) {}
+            while (!bar_try(bars + 8 * (W::B_DRAIN + t), 0) && clock64() - t0 < WAIT_CLOCKS) {}
         }
         __syncwarp();
     }
