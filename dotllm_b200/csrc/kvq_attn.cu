@@ -152,25 +152,10 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
     }
     const int kvh = sg.kvh, chunk = sg.chunk, ch = sg.ch, len = sg.len, row_first = sg.tile * RT;
     const int32_t *pages = sg.pages;
-    // ---- rows: place, visible range [lo, hi] in the segment's positions, query as fp16
-    const SeqTable seqs = load_seqs(a, sg, (int32_t *)smem, NW * 32);  // (the slots' memory, not in use yet)
-    if (tid < RT) row_range(a, sg, seqs, row_first + tid, s_row[tid], s_lo[tid], s_hi[tid]);
-    __syncthreads();
-    // the tile's ranges (rows that do not exist see everything and are not written)
-    int lo_min = 0x7fffffff, lo_max = 0, hi_min = 0x7fffffff, hi_max = -1;
-#pragma unroll
-    for (int n = lane; n < (RT + 31) / 32 * 32; n += 32) {
-        const bool on = n < RT && s_row[n < RT ? n : 0] >= 0;
-        const int lo = on ? s_lo[n] : 0, hi = on ? s_hi[n] : 0;
-        lo_min = min(lo_min, __reduce_min_sync(0xffffffffu, on ? lo : 0x7fffffff));
-        lo_max = max(lo_max, __reduce_max_sync(0xffffffffu, on ? lo : 0));
-        hi_min = min(hi_min, __reduce_min_sync(0xffffffffu, on ? hi : 0x7fffffff));
-        hi_max = max(hi_max, __reduce_max_sync(0xffffffffu, on ? hi : -1));
-    }
-    // ---- pages [u0, u1) of the segment's list
-    const int u0 = max(chunk * ch, lo_min / KVQ_PAGE);
-    const int u1 = min((chunk + 1) * ch, hi_max < 0 ? 0 : hi_max / KVQ_PAGE + 1);
     const uint32_t smem_s = su32(smem);
+    // ---- pages [u0, u1) of the segment's list; those outside a window are left out once the rows' ranges are
+    // known, without one the first pages are on their way before that
+    int u0 = chunk * ch, u1 = min((chunk + 1) * ch, (max(len, 0) + KVQ_PAGE - 1) / KVQ_PAGE);
     auto place = [&](int u) -> int64_t {  // the page's first position in rows of one head, or -1
         const int page = u < u1 ? __ldg(pages + u) : -1;
         return (unsigned)page < (unsigned)a.pool.n_pages ? ((int64_t)page * Hk + kvh) * KVQ_PAGE : -1;
@@ -188,10 +173,36 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
         }
         cp_commit();
     };
-    int64_t at = place(u0), at1 = place(u0 + 1), at2 = place(u0 + 2);
-    fetch(at, 0, false);
-    fetch(at, 0, true);
-    fetch(at1, 1, false);
+    int64_t at = -1, at1 = -1, at2 = -1;
+    auto begin = [&]() {
+        at = place(u0);
+        at1 = place(u0 + 1);
+        at2 = place(u0 + 2);
+        fetch(at, 0, false);
+        fetch(at, 0, true);
+        fetch(at1, 1, false);
+    };
+    if (a.at.window == 0) begin();
+    // ---- rows: place, visible range [lo, hi] in the segment's positions, query as fp16
+    const SeqTable seqs = load_seqs(a, sg, (int32_t *)sq, NW * 32);  // (the queries' memory, not in use yet)
+    if (tid < RT) row_range(a, sg, seqs, row_first + tid, s_row[tid], s_lo[tid], s_hi[tid]);
+    __syncthreads();
+    // the tile's ranges (rows that do not exist see everything and are not written)
+    int lo_min = 0x7fffffff, lo_max = 0, hi_min = 0x7fffffff, hi_max = -1;
+#pragma unroll
+    for (int n = lane; n < (RT + 31) / 32 * 32; n += 32) {
+        const bool on = n < RT && s_row[n < RT ? n : 0] >= 0;
+        const int lo = on ? s_lo[n] : 0, hi = on ? s_hi[n] : 0;
+        lo_min = min(lo_min, __reduce_min_sync(0xffffffffu, on ? lo : 0x7fffffff));
+        lo_max = max(lo_max, __reduce_max_sync(0xffffffffu, on ? lo : 0));
+        hi_min = min(hi_min, __reduce_min_sync(0xffffffffu, on ? hi : 0x7fffffff));
+        hi_max = max(hi_max, __reduce_max_sync(0xffffffffu, on ? hi : -1));
+    }
+    if (a.at.window > 0) {
+        u0 = max(u0, lo_min / KVQ_PAGE);
+        u1 = min(u1, hi_max < 0 ? 0 : hi_max / KVQ_PAGE + 1);
+        begin();
+    }
 
     for (int n = warp; n < RT; n += NW) {
         const int row = s_row[n];
@@ -570,7 +581,7 @@ template <int D, int FMT, int NT, bool SPLIT> cudaError_t launch_tiles(const Att
 {
     using Sh = Shape<D>;
     constexpr int NQ = SPLIT ? 2 : 1, smem = Sh::OFF_Q + NQ * NT * 8 * (D + Sh::QPAD + 2 * PS) * 2;
-    static_assert(4 * Sh::SLOT >= (2 * SEQ_TABLE + 1) * 4, "the sequences' tables fit into the slots");
+    static_assert(smem - Sh::OFF_Q >= (2 * SEQ_TABLE + 1) * 4, "the sequences' tables fit into the queries' and weights' memory");
     static_assert(D != 64 || 4 * Sh::SLOT >= 2 * NT * 2 * 512, "two warps' outputs fit into the slots");
     static std::atomic<unsigned long long> done{0};
     cudaError_t e = smem_attr_once(done, kvq_attn_kernel<D, FMT, NT, SPLIT>, smem);
@@ -652,17 +663,19 @@ Plan make_plan(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const llmdot
     x.rtiles = (int)std::max<int64_t>(1, up(own_rows, x.wide_s ? wide : 8 * x.nt_s));
     // Chunks.  Narrow: about one CTA per place on the SMs for the prefix, two for the sequences' own pages
     // (max_pages is a bound: ragged sequences leave some without work), at most 32 pages, so that long
-    // and short sequences balance.  Wide: one CTA per SM, at least two pages.
+    // and short sequences balance.  Wide: one CTA per SM, at least two pages.  At most 256 chunks of either, which
+    // bounds the workspace and what the join reads.
     auto places = [&](int nt) {  // CTAs on the SMs: shared memory and registers (as built) of an instance
         const int d = p.head_dim, nq = a.type == T_F32 ? 2 : 1, bytes = 4 * 64 * d + 1024 + nq * nt * 8 * (d + 168) * 2 + 2048;
         const int regs = d == 256 ? (nt <= 2 ? 4 : nt == 3 ? 3 : 2) : nt == 1 ? 5 : nt <= 3 ? 4 : nt == 4 ? 3 : 2;
         return 148 * (int64_t)std::max(1, std::min(regs, 227 * 1024 / bytes));
     };
     auto chunk = [&](int64_t pages, int64_t ctas, int64_t least) { return std::min<int64_t>(32, std::max<int64_t>(least, up(pages, ctas))); };
+    auto bounded = [&](int64_t ch, int64_t pages) { return (int)std::max(ch, up(pages, 256)); };
     auto wide_ch = [&](int64_t ctas, int64_t pages) { return std::max<int64_t>(2, up(pages, std::max<int64_t>(1, 148 / std::max<int64_t>(1, ctas)))); };
-    x.ch_p = (int)(x.wide_p ? wide_ch(Hk * x.ptiles, npp) : chunk(Hk * x.ptiles * npp, places(x.nt_p), 1));
-    x.ch_s = (int)(x.wide_s ? wide_ch(Hk * x.rtiles * b.batch, b.max_pages)
-                            : chunk(Hk * b.batch * x.rtiles * b.max_pages, 2 * places(x.nt_s), 2));
+    x.ch_p = bounded(x.wide_p ? wide_ch(Hk * x.ptiles, npp) : chunk(Hk * x.ptiles * npp, places(x.nt_p), 1), npp);
+    x.ch_s = bounded(x.wide_s ? wide_ch(Hk * x.rtiles * b.batch, b.max_pages)
+                              : chunk(Hk * b.batch * x.rtiles * b.max_pages, 2 * places(x.nt_s), 2), b.max_pages);
     x.nsp = (int)up(npp, x.ch_p);
     x.nss = (int)std::max<int64_t>(1, up(b.max_pages, x.ch_s));
     x.direct = x.nsp == 0 && x.nss == 1 && !x.wide_s;

@@ -79,7 +79,7 @@ __device__ __forceinline__ bool segment_of(const AttnArgs &a, int rows, Segment 
 struct SeqTable {
     const int32_t *row_start, *seq_len;
 };
-constexpr int SEQ_TABLE = 512;  // sequences
+constexpr int SEQ_TABLE = 448;  // sequences
 // Called by all threads; `room`: 2 * SEQ_TABLE + 1 ints of shared memory.  The prefix's rows need it alone.
 __device__ __forceinline__ SeqTable load_seqs(const AttnArgs &a, const Segment &s, int32_t *room, int threads)
 {

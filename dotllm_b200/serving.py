@@ -132,7 +132,7 @@ def kvq_read(pool: KvqPool, batch: KvqBatch, rows: int, dtype: torch.dtype = tor
         _bad("kvq_read: dtype must be float32, float16 or bfloat16")
     if rows < 0 or batch.device != pool.device:
         _bad("kvq_read: negative rows, or pool and batch on different devices")
-    out = torch.empty((2, rows, pool.heads_kv, pool.head_dim), dtype=dtype, device=pool.k.device)
+    out = pool.k_scale.new_empty((2, rows, pool.heads_kv, pool.head_dim), dtype=dtype)
     ld = pool.heads_kv * pool.head_dim
     k, v = out.unbind(0)
     _call(lib().llmdot_cuda_kvq_read, pool.device, pool._c, batch._c(rows), k.data_ptr(), v.data_ptr(), _TYPES[dtype], ld, ld)
@@ -165,11 +165,11 @@ def kvq_attention(pool: KvqPool, batch: KvqBatch, q: torch.Tensor, prefix_pages:
                        prefix)
     need = C.c_size_t()
     check(L.llmdot_cuda_kvq_attention_workspace(p, b, a, need))
-    out = torch.empty((rows, heads, pool.head_dim), dtype=q.dtype, device=q.device)
-    lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    out = q.new_empty(q.shape)
+    lse = q.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
     work, size = None, need.value
     if size:
-        work = torch.empty(size, dtype=torch.uint8, device=q.device)
+        work = q.new_empty(size, dtype=torch.uint8)
     _call(L.llmdot_cuda_kvq_attention, device, p, b, a, q.data_ptr(), ld, out.data_ptr(), heads * pool.head_dim,
           lse.data_ptr() if return_lse else None, work.data_ptr() if size else None, size)
     return (out, lse) if return_lse else out
@@ -205,8 +205,7 @@ def verify_draft(p: torch.Tensor, q: Optional[torch.Tensor], draft: torch.Tensor
     ld_q = ld("q", q, k) if q is not None else 0
     if uniform.dtype is not torch.float32 or uniform.shape != (B, k1) or uniform.get_device() != device or not uniform.is_contiguous():
         _bad(f"verify_draft: uniform must be contiguous float32 [{B}, {k1}] on cuda:{device}")
-    tokens = torch.empty((B, k1), dtype=torch.int32, device=p.device)
-    accepted = torch.empty((B,), dtype=torch.int32, device=p.device)
+    tokens, accepted = p.new_empty((B, k1), dtype=torch.int32), p.new_empty((B,), dtype=torch.int32)
     _call(lib().llmdot_cuda_verify_draft, device,
           native.Verify(B, k, V, 0, p.data_ptr(), q.data_ptr() if q is not None else None, ld_p, ld_q,
                         _int32("draft", draft, (B, k), device), uniform.data_ptr(),
