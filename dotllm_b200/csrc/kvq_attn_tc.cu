@@ -314,17 +314,17 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                     sts128(piece(c), v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
                 }
             } else {
-                uint32_t top = 0;  // magnitudes order as integers, NaN above all
-#pragma unroll 4
+                __nv_bfloat162 top2 = __float2bfloat162_rn(0.0f);  // a NaN survives the maxima
+#pragma unroll 8
                 for (int c = 0; c < D / 8; c++) {
                     const uint4 v = lds128(piece(c));
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int k = 0; k < 4; k++) top = max(top, max((w[k] << 16) & 0x7fffffffu, w[k] & 0x7fff0000u));
+                    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&v);
+                    top2 = __hmax2_nan(top2, __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3]))));
                 }
-                e = row_exponent(__uint_as_float(top));
+                const float top = __bfloat162float(__hmax_nan(__low2bfloat16(top2), __high2bfloat16(top2)));
+                e = row_exponent(top);
                 const float up = pow2(e);
-#pragma unroll 4
+#pragma unroll 8
                 for (int c = 0; c < D / 8; c++) {
                     const uint4 v = lds128(piece(c));
                     const uint32_t w[4] = {v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip};
