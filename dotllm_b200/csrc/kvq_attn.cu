@@ -664,14 +664,17 @@ Plan make_plan(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const llmdot
     // Chunks.  Narrow: about one CTA per place on the SMs for the prefix, two for the sequences' own pages
     // (max_pages is a bound: ragged sequences leave some without work), at most 32 pages, so that long
     // and short sequences balance.  Wide: one CTA per SM, at least two pages.  At most 256 chunks of either, which
-    // bounds the workspace and what the join reads.
+    // bounds the workspace and what the join reads, and even ones.
     auto places = [&](int nt) {  // CTAs on the SMs: shared memory and registers (as built) of an instance
         const int d = p.head_dim, nq = a.type == T_F32 ? 2 : 1, bytes = 4 * 64 * d + 1024 + nq * nt * 8 * (d + 168) * 2 + 2048;
         const int regs = d == 256 ? (nt <= 2 ? 4 : nt == 3 ? 3 : 2) : nt == 1 ? 5 : nt <= 3 ? 4 : nt == 4 ? 3 : 2;
         return 148 * (int64_t)std::max(1, std::min(regs, 227 * 1024 / bytes));
     };
     auto chunk = [&](int64_t pages, int64_t ctas, int64_t least) { return std::min<int64_t>(32, std::max<int64_t>(least, up(pages, ctas))); };
-    auto bounded = [&](int64_t ch, int64_t pages) { return (int)std::max(ch, up(pages, 256)); };
+    auto bounded = [&](int64_t ch, int64_t pages) {
+        ch = std::max(ch, up(pages, 256));
+        return (int)std::max<int64_t>(1, up(pages, std::max<int64_t>(1, up(pages, ch))));
+    };
     auto wide_ch = [&](int64_t ctas, int64_t pages) { return std::max<int64_t>(2, up(pages, std::max<int64_t>(1, 148 / std::max<int64_t>(1, ctas)))); };
     x.ch_p = bounded(x.wide_p ? wide_ch(Hk * x.ptiles, npp) : chunk(Hk * x.ptiles * npp, places(x.nt_p), 1), npp);
     x.ch_s = bounded(x.wide_s ? wide_ch(Hk * x.rtiles * b.batch, b.max_pages)
