@@ -8,7 +8,8 @@
 // is a sum of exact products in fp32, and the key's scale multiplies the score.  The value's scale goes
 // into the weight: P_j = exp2(s_j - m) * (v_scale_j / 2^E), 2^E the largest power of two not above the
 // v_scales seen so far (raised with the running maximum, the sums rescaled by both), so that P stays in
-// fp16's normal range whatever the scales' size; P is rounded to fp16 once (fp32 queries: hi + lo).
+// fp16's normal range whatever the scales' size; P is hi + lo, or with bf16 queries, whose output has 8
+// bits, one fp16 (with fp16 outputs its rounding would add as much error again as the output's own).
 // The sum of exponentials, the maxima, both products' sums and the outputs are fp32.
 //
 // Work is cut into segments -- the prefix with every row of the batch, each sequence's own pages with
@@ -124,23 +125,24 @@ __device__ __forceinline__ void store4(void *p, int64_t i, uint32_t type, bool w
 // What a row's reference stands above its maximum when it is set (powers of two), and the test that a packed
 // weight has come too near fp16's limit.  One fp16 per weight: 2^6 above, weights of 2 and more (an exponent
 // bit).  hi + lo: 2^4 below, so that lo stays a normal number; 2^13 and more.
-template <bool SPLIT> constexpr float ref_head() { return SPLIT ? -4.0f : 6.0f; }
-template <bool SPLIT> __device__ __forceinline__ uint32_t too_large(uint32_t p)
+template <bool TWO> constexpr float ref_head() { return TWO ? -4.0f : 6.0f; }
+template <bool TWO> __device__ __forceinline__ uint32_t too_large(uint32_t p)
 {
-    return SPLIT ? ((p & 0x70007000u) + 0x10001000u) & 0x80008000u : p & 0x40004000u;
+    return TWO ? ((p & 0x70007000u) + 0x10001000u) & 0x80008000u : p & 0x40004000u;
 }
 
-template <int D, int FMT, int NT, bool SPLIT>
+// PREC 0 (bf16): one fp16 for query and weight; 1 (fp16): hi + lo weights; 2 (fp32): hi + lo queries too.
+template <int D, int FMT, int NT, int PREC>
 __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 ? 4 : 1) kvq_attn_kernel(const __grid_constant__ AttnArgs a)
 {
     using Sh = Shape<D>;
-    constexpr int RT = 8 * NT, QS = D + Sh::QPAD, NQ = SPLIT ? 2 : 1;
+    constexpr int RT = 8 * NT, QS = D + Sh::QPAD, NQ = PREC == 2 ? 2 : 1, NP = PREC > 0 ? 2 : 1;
     constexpr bool QREG = NT * NQ * D / 8 <= 32;  // the query's fragments stay in registers
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float s_qf[RT], s_max[NW][RT], s_l[NW][RT], s_vmax[NW];
     __shared__ int s_lo[RT], s_hi[RT], s_row[RT];
     __half *sq = (__half *)(smem + Sh::OFF_Q);  // [NQ][RT][QS]
-    __half *sp = sq + NQ * RT * QS;             // [2][NQ][RT][PS]
+    __half *sp = sq + NQ * RT * QS;             // [2][NP][RT][PS]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int G = a.group, Hk = a.pool.heads_kv;
 
@@ -220,7 +222,7 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
             const float y = x[i] * up;
             const __half h = __float2half_rn(y);
             sq[n * QS + i * 32 + lane] = h;
-            if (SPLIT) sq[(RT + n) * QS + i * 32 + lane] = __float2half_rn(y - __half2float(h));
+            if (NQ > 1) sq[(RT + n) * QS + i * 32 + lane] = __float2half_rn(y - __half2float(h));
         }
         // scores in base 2, or natural ones for the cap
         if (lane == 0)
@@ -279,7 +281,7 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
         at2 = place(u + 3);
         bool again = false;
         const int t0 = u * KVQ_PAGE + j16;
-        __half *pw = sp + sl * NQ * RT * PS;
+        __half *pw = sp + sl * NP * RT * PS;
         float s[NT][4], ln[NT][2], vf[2] = {0.0f, 0.0f};
         const bool whole = u * KVQ_PAGE >= lo_max && u * KVQ_PAGE + KVQ_PAGE - 1 <= hi_min;
         // the weights of this warp's positions into shared memory, relative to the references
@@ -298,19 +300,19 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
                     if (!whole && x == -INFINITY) y = p[e] = 0.0f;  // whatever the unseen position holds
                     ln[nt][e & 1] += y;
                 }
-                uint32_t b[NQ][2];
+                uint32_t b[NP][2];
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
                     const uint32_t hi = pack(p[2 * hf], p[2 * hf + 1]);
-                    any |= too_large<SPLIT>(hi);
+                    any |= too_large<(NP > 1)>(hi);
                     b[0][hf] = transpose8(hi);
-                    if (SPLIT) {
+                    if (NP > 1) {
                         const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-                        b[NQ - 1][hf] = transpose8(pack(p[2 * hf] - back.x, p[2 * hf + 1] - back.y));
+                        b[NP - 1][hf] = transpose8(pack(p[2 * hf] - back.x, p[2 * hf + 1] - back.y));
                     }
                 }
 #pragma unroll
-                for (int h = 0; h < NQ; h++)
+                for (int h = 0; h < NP; h++)
                     *(uint2 *)(pw + (h * RT + nt * 8 + g) * PS + warp * 16 + t * 4) = make_uint2(b[h][0], b[h][1]);
             }
             return any != 0;
@@ -352,7 +354,7 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     s[nt][e] *= kf[e >> 1] * qf[nt][e & 1];
-                    if (cap) s[nt][e] = capped<SPLIT>(s[nt][e], a.at.softcap, inv_cap2) * 1.4426950408889634f;
+                    if (cap) s[nt][e] = capped<PREC == 2>(s[nt][e], a.at.softcap, inv_cap2) * 1.4426950408889634f;
                 }
             if (!whole)
 #pragma unroll
@@ -393,7 +395,7 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     const int n = nt * 8 + 2 * t + c;
-                    const float top = fmaxf(fmaxf(s_max[0][n], s_max[1][n]), fmaxf(s_max[2][n], s_max[3][n])) + ref_head<SPLIT>();
+                    const float top = fmaxf(fmaxf(s_max[0][n], s_max[1][n]), fmaxf(s_max[2][n], s_max[3][n])) + ref_head<(NP > 1)>();
                     float f = 1.0f;
                     if (top > ref[nt][c]) {
                         f = ex2(ref[nt][c] - top);  // nothing seen before: exp2(-inf) = 0
@@ -423,9 +425,9 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
 #pragma unroll
             for (int m = 0; m < (D == 64 ? 2 : 4); m++) {
                 const int mt = mt0 + m;
-                uint2 pb[NQ][NT];
+                uint2 pb[NP][NT];
 #pragma unroll
-                for (int h = 0; h < NQ; h++)
+                for (int h = 0; h < NP; h++)
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) pb[h][nt] = *(const uint2 *)(pw + (h * RT + nt * 8 + g) * PS + mt * 16 + t * 4);
 #pragma unroll
@@ -443,7 +445,7 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                            for (int h = 0; h < NQ; h++) mma(o[q][hf][nt], fr, pb[h][nt].x, pb[h][nt].y);
+                            for (int h = 0; h < NP; h++) mma(o[q][hf][nt], fr, pb[h][nt].x, pb[h][nt].y);
                     }
                 }
             }
@@ -577,33 +579,37 @@ template <int D, int W> __global__ void __launch_bounds__(128) kvq_join_kernel(c
 }
 
 // ------------------------------------------------------------------ launch
-template <int D, int FMT, int NT, bool SPLIT> cudaError_t launch_tiles(const AttnArgs &a, int64_t grid, cudaStream_t st)
+template <int D, int FMT, int NT, int PREC> cudaError_t launch_tiles(const AttnArgs &a, int64_t grid, cudaStream_t st)
 {
     using Sh = Shape<D>;
-    constexpr int NQ = SPLIT ? 2 : 1, smem = Sh::OFF_Q + NQ * NT * 8 * (D + Sh::QPAD + 2 * PS) * 2;
+    constexpr int NQ = PREC == 2 ? 2 : 1, NP = PREC > 0 ? 2 : 1, smem = Sh::OFF_Q + NT * 8 * (NQ * (D + Sh::QPAD) + NP * 2 * PS) * 2;
     static_assert(smem - Sh::OFF_Q >= (2 * SEQ_TABLE + 1) * 4, "the sequences' tables fit into the queries' and weights' memory");
     static_assert(D != 64 || 4 * Sh::SLOT >= 2 * NT * 2 * 512, "two warps' outputs fit into the slots");
     static std::atomic<unsigned long long> done{0};
-    cudaError_t e = smem_attr_once(done, kvq_attn_kernel<D, FMT, NT, SPLIT>, smem);
+    cudaError_t e = smem_attr_once(done, kvq_attn_kernel<D, FMT, NT, PREC>, smem);
     if (e != cudaSuccess) return e;
-    return launch_kernel(a.chained != 0, kvq_attn_kernel<D, FMT, NT, SPLIT>, dim3((unsigned)grid), dim3(NW * 32), smem, st, a);
+    return launch_kernel(a.chained != 0, kvq_attn_kernel<D, FMT, NT, PREC>, dim3((unsigned)grid), dim3(NW * 32), smem, st, a);
 }
-template <int D, int FMT, bool SPLIT> cudaError_t launch_nt(int nt, const AttnArgs &a, int64_t grid, cudaStream_t st)
+template <int D, int FMT, int PREC> cudaError_t launch_nt(int nt, const AttnArgs &a, int64_t grid, cudaStream_t st)
 {
     switch (nt) {
-    case 1: return launch_tiles<D, FMT, 1, SPLIT>(a, grid, st);
-    case 2: return launch_tiles<D, FMT, 2, SPLIT>(a, grid, st);
-    case 3: return launch_tiles<D, FMT, 3, SPLIT>(a, grid, st);
-    case 4: return launch_tiles<D, FMT, 4, SPLIT>(a, grid, st);
-    default: return launch_tiles<D, FMT, Shape<D>::MAX_NT, SPLIT>(a, grid, st);
+    case 1: return launch_tiles<D, FMT, 1, PREC>(a, grid, st);
+    case 2: return launch_tiles<D, FMT, 2, PREC>(a, grid, st);
+    case 3: return launch_tiles<D, FMT, 3, PREC>(a, grid, st);
+    case 4: return launch_tiles<D, FMT, 4, PREC>(a, grid, st);
+    default: return launch_tiles<D, FMT, Shape<D>::MAX_NT, PREC>(a, grid, st);
     }
+}
+template <int D, int FMT> cudaError_t launch_prec(int nt, const AttnArgs &a, int64_t grid, cudaStream_t st)
+{
+    if (a.at.type == T_F32) return launch_nt<D, FMT, 2>(nt, a, grid, st);
+    if (a.at.type == T_F16) return launch_nt<D, FMT, 1>(nt, a, grid, st);
+    return launch_nt<D, FMT, 0>(nt, a, grid, st);
 }
 template <int D> cudaError_t launch_dim(int nt, const AttnArgs &a, int64_t grid, cudaStream_t st)
 {
-    const bool split = a.at.type == T_F32;
-    if (a.pool.format == LLMDOT_KVQ_I8)
-        return split ? launch_nt<D, LLMDOT_KVQ_I8, true>(nt, a, grid, st) : launch_nt<D, LLMDOT_KVQ_I8, false>(nt, a, grid, st);
-    return split ? launch_nt<D, LLMDOT_KVQ_E4M3, true>(nt, a, grid, st) : launch_nt<D, LLMDOT_KVQ_E4M3, false>(nt, a, grid, st);
+    if (a.pool.format == LLMDOT_KVQ_I8) return launch_prec<D, LLMDOT_KVQ_I8>(nt, a, grid, st);
+    return launch_prec<D, LLMDOT_KVQ_E4M3>(nt, a, grid, st);
 }
 cudaError_t launch_narrow(int nt, const AttnArgs &a, int64_t grid, cudaStream_t st)
 {
@@ -666,7 +672,8 @@ Plan make_plan(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const llmdot
     // and short sequences balance.  Wide: one CTA per SM, at least two pages.  At most 256 chunks of either, which
     // bounds the workspace and what the join reads, and even ones.
     auto places = [&](int nt) {  // CTAs on the SMs: shared memory and registers (as built) of an instance
-        const int d = p.head_dim, nq = a.type == T_F32 ? 2 : 1, bytes = 4 * 64 * d + 1024 + nq * nt * 8 * (d + 168) * 2 + 2048;
+        const int d = p.head_dim, nq = a.type == T_F32 ? 2 : 1, np = a.type == T_BF16 ? 1 : 2;
+        const int bytes = 4 * 64 * d + 1024 + nt * 8 * (nq * (d + 8) + np * 160) * 2 + 2048;
         const int regs = d == 256 ? (nt <= 2 ? 4 : nt == 3 ? 3 : 2) : nt == 1 ? 5 : nt <= 3 ? 4 : nt == 4 ? 3 : 2;
         return 148 * (int64_t)std::max(1, std::min(regs, 227 * 1024 / bytes));
     };
