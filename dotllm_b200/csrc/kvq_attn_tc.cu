@@ -9,9 +9,9 @@
 // and its roles overlap, 64 positions (a page) at a time:
 //   warps of a tile (4 each)  S from TMEM 64 columns at a time in fragments of 4 rows by 2 columns a lane
 //                             (a lane so needs a quarter of the columns' scales), weights as fp16 back
-//                             into TMEM over S.  The weights are taken relative to a row's reference, 2^6
-//                             above its maximum when it was set; only when a weight reaches 2 is
-//                             the maximum searched, the reference raised, and the sums and O rescaled, which
+//                             into TMEM over S.  The weights are taken relative to a row's reference,
+//                             set by its maximum; only when a weight comes near fp16's limit is the
+//                             maximum searched, the reference raised, and the sums and O rescaled, which
 //                             after the first positions is rare
 //   4 converting warps        codes from global memory (three K or V pages' loads in flight) to fp16 K
 //                             and V operands in shared memory, scales beside them
@@ -36,7 +36,13 @@ namespace llmdot {
 namespace {
 
 constexpr long long WAIT_CLOCKS = 4000000000ll;  // about two seconds
-constexpr float HEAD = 6.0f;  // a row's reference stands this power of two above its maximum
+// A row's reference stands this power of two above its maximum (hi + lo: below, so that lo stays a normal
+// number), and a packed weight that has come too near fp16's limit: 2 and more (an exponent bit), or 2^13.
+template <bool TWO> constexpr float head_room() { return TWO ? -4.0f : 6.0f; }
+template <bool TWO> __device__ __forceinline__ uint32_t too_large(uint32_t p)
+{
+    return TWO ? ((p & 0x70007000u) + 0x10001000u) & 0x80008000u : p & 0x40004000u;
+}
 
 template <int D> struct Wide {
     static constexpr int TILES = D == 256 ? 1 : 2;
@@ -195,7 +201,8 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c)
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
     return r;
 }
-template <int D, int FMT>
+// TWO: the weights as hi + lo (fp16 queries, whose outputs have 11 bits); one fp16 else.
+template <int D, int FMT, bool TWO>
 __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __grid_constant__ AttnArgs a, const int qwide)
 {
     using W = Wide<D>;
@@ -381,17 +388,30 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             }
             tmem_st_wait();
         };
-        auto hand_over = [&](int buf, const uint32_t (&p)[2][16]) {  // a page's weights, over scores that were read
-            tmem_st_frag(tm + W::C_S + 64 * buf, p[0]);
-            tmem_st_frag(tm + (16u << 16) + W::C_S + 64 * buf, p[1]);
+        // A page's weights, hi and lo in 32 columns each, over scores that were read.
+        constexpr int NP = TWO ? 2 : 1;
+        auto hand_over = [&](int buf, const uint32_t (&p)[NP][2][16]) {
+#pragma unroll
+            for (int x = 0; x < NP; x++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) tmem_st_frag(tm + ((uint32_t)(16 * h) << 16) + W::C_S + 64 * buf + 32 * x, p[x][h]);
             tmem_st_wait();
             fence_before();
             bar_arrive(bars + 8 * (W::B_P + tile * 2 + buf));
         };
-        // A page that the rows see whole, without a cap: false (and nothing done) when a weight
-        // reaches 2 and the reference has to rise.
+        auto split = [&](float y, float z, uint32_t (&p)[NP][2][16], int h, int at) {
+            const uint32_t hi = pack(y, z);
+            p[0][h][at] = hi;
+            if (TWO) {
+                const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+                p[NP - 1][h][at] = pack(y - b.x, z - b.y);
+            }
+            return hi;
+        };
+        // A page that the rows see whole, without a cap: false (and nothing done) when a weight comes too near
+        // the limit and the reference has to rise.
         auto plain_page = [&](const float *ks, const float *vs, int buf) -> bool {
-            uint32_t s[2][32], p[2][16], any = 0;
+            uint32_t s[2][32], p[NP][2][16], any = 0;
             tmem_ld_frag(tm + W::C_S + 64 * buf, s[0]);
             tmem_ld_frag(tm + (16u << 16) + W::C_S + 64 * buf, s[1]);
             F2 q2[4], off[4], sum[4];
@@ -414,17 +434,17 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                     const F2 e = f2(ex2(y), ex2(z));
                     sum[k] = add2(sum[k], e);
                     un2(mul2(e, v2), y, z);
-                    any |= p[k >> 1][2 * i + (k & 1)] = pack(y, z);
+                    const uint32_t hi = split(y, z, p, k >> 1, 2 * i + (k & 1));
+                    any |= TWO ? too_large<TWO>(hi) : hi;
                 }
             }
-            if (__any_sync(0xffffffffu, (any & 0x40004000u) != 0)) return false;  // an exponent bit: 2 or more (or a NaN)
+            if (__any_sync(0xffffffffu, (TWO ? any : too_large<TWO>(any)) != 0)) return false;  // (or a NaN)
 #pragma unroll
             for (int k = 0; k < 4; k++) l[k] = add2(l[k], sum[k]);
             hand_over(buf, p);
             return true;
         };
-        // The search for the rows' maxima over a page, and the references raised where they stand less than
-        // HEAD above.  MASKED: scores of positions that a row does not see do not count.
+        // The search for the rows' maxima over a page, and the references raised where they stand too low.  MASKED: scores of positions that a row does not see do not count.
         auto search = [&](int i, const float *ks, int buf, auto masked) {
             constexpr bool MASKED = decltype(masked)::value;
             const int j0 = u0 * KVQ_PAGE + i * UN + 2 * t;
@@ -458,7 +478,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                 if (top[k] != -INFINITY) {
                     float x = top[k] * fq[k];
                     if (cap) x = capped<false>(x, a.at.softcap, inv_cap2) * 1.4426950408889634f;  // monotonic
-                    x += HEAD;
+                    x += head_room<TWO>();
                     if (x > ref[k]) {
                         // by a power of two, which the factor then is
                         const float to = ref[k] == -INFINITY ? x : ref[k] + ceilf(x - ref[k]);
@@ -482,7 +502,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
         // The weights of a page, with masks and cap.
         auto masked_page = [&](int i, const float *ks, const float *vs, int buf) {
             const int j0 = u0 * KVQ_PAGE + i * UN + 2 * t;
-            uint32_t p[2][16];
+            uint32_t p[NP][2][16];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 uint32_t s[32];
@@ -504,7 +524,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                         y = ex2(y - off);
                         const bool gx = j < flo[k] || j > fhi[k], gy = j + 1 < flo[k] || j + 1 > fhi[k];
                         l[k] = add2(l[k], f2(gx ? 0.0f : x, gy ? 0.0f : y));
-                        p[h][2 * c + r] = pack(gx ? 0.0f : x * vf.x, gy ? 0.0f : y * vf.y);  // whatever an unseen position holds
+                        split(gx ? 0.0f : x * vf.x, gy ? 0.0f : y * vf.y, p, h, 2 * c + r);  // whatever an unseen position holds
                     }
                 }
             }
@@ -524,7 +544,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                 if (!ok) break;
             }
             if (ex.z != 0.0f || p0 > hi_end || p0 + KVQ_PAGE <= lo_min) {  // nothing for this warp's rows
-                const uint32_t zero[2][16] = {};
+                const uint32_t zero[NP][2][16] = {};
                 hand_over(buf, zero);
             } else if (!cap && p0 >= lo_max && p0 + KVQ_PAGE - 1 <= hi_min) {  // everything
                 if (known && plain_page(ks, vs, buf)) continue;
@@ -722,8 +742,8 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                 fence_after();
                 const uint64_t v = vd + i % STAGES * (W::STAGE / 16);
 #pragma unroll
-                for (int kk = 0; kk < UN / 16; kk++)
-                    umma_ts<D>(tm + W::C_O, tm + W::C_S + 64 * (i & 1) + 8 * kk, v + kk * 2 * W::GROUP / 16, i != 0 || kk != 0);
+                for (int kk = 0; kk < (TWO ? 2 : 1) * UN / 16; kk++)  // hi, then lo, on the same values
+                    umma_ts<D>(tm + W::C_O, tm + W::C_S + 64 * (i & 1) + 8 * kk, v + kk % (UN / 16) * 2 * W::GROUP / 16, i != 0 || kk != 0);
                 umma_commit(bo + 8 * (i & 1));
                 umma_commit(bars + 8 * (W::B_EMPTY + i % STAGES));
                 if (i + 2 < n) qk(i + 2);  // the scores that this page's weights leave room for
@@ -743,14 +763,18 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
     if (a.chained) pdl_wait();
 }
 
-template <int D, int FMT> cudaError_t launch(const AttnArgs &a, int64_t ctas, bool pdl, cudaStream_t st)
+template <int D, int FMT, bool TWO> cudaError_t launch_one(const AttnArgs &a, int64_t ctas, bool pdl, cudaStream_t st)
 {
     using W = Wide<D>;
     static std::atomic<unsigned long long> done{0};
-    cudaError_t e = smem_attr_once(done, kvq_wide_kernel<D, FMT>, W::SMEM);
+    cudaError_t e = smem_attr_once(done, kvq_wide_kernel<D, FMT, TWO>, W::SMEM);
     if (e != cudaSuccess) return e;
     const int qwide = ((uintptr_t)a.q & 15) == 0 && (a.bt.rows <= 1 || a.ldq * 2 % 16 == 0);
-    return launch_kernel(pdl, kvq_wide_kernel<D, FMT>, dim3((unsigned)ctas), dim3(W::THREADS), W::SMEM, st, a, qwide);
+    return launch_kernel(pdl, kvq_wide_kernel<D, FMT, TWO>, dim3((unsigned)ctas), dim3(W::THREADS), W::SMEM, st, a, qwide);
+}
+template <int D, int FMT> cudaError_t launch(const AttnArgs &a, int64_t ctas, bool pdl, cudaStream_t st)
+{
+    return a.at.type == T_F16 ? launch_one<D, FMT, true>(a, ctas, pdl, st) : launch_one<D, FMT, false>(a, ctas, pdl, st);
 }
 template <int FMT> cudaError_t by_dim(const AttnArgs &a, int64_t ctas, bool pdl, cudaStream_t st)
 {
