@@ -109,3 +109,28 @@ def test_long_sequences_few_rows(gpu, typ):
     run("i8", typ, 2, 4, 128, 0, [20000, 3, 7777], [1, 2, 5], k_ramp=4.0, v_ramp=6.0)
     run("e4m3", typ, 8, 1, 64, 5000, [6000] * 3, [1, 1, 1], k_ramp=4.0, scale=-0.2)
     run("i8", typ, 2, 2, 128, 300, [200] * 40, [1] * 40, scale=-0.1, window=333)
+
+
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+def test_many_rows_from_unaligned_queries(gpu, typ):
+    """Queries that start off every 16-byte boundary, and rows strided as slices of a wider product, give the bits
+    that dense ones give."""
+    import torch
+    from dotllm_b200 import serving
+    t = {"f16": torch.float16, "bf16": torch.bfloat16}[typ]
+    g = torch.Generator("cuda").manual_seed(3)
+    R, hk, heads, dim, P = 90, 2, 4, 128, 500
+    pool = serving.KvqPool.empty(8, hk, dim)
+    rows = torch.tensor([0, P], dtype=torch.int32, device="cuda")
+    pages = torch.arange(8, dtype=torch.int32, device="cuda")
+    serving.kvq_write(pool, serving.KvqBatch(rows, rows[1:].contiguous(), pages.view(1, -1), P),
+                      torch.randn(P, hk, dim, device="cuda", generator=g), torch.randn(P, hk, dim, device="cuda", generator=g))
+    batch = serving.KvqBatch(torch.arange(R + 1, dtype=torch.int32, device="cuda"), torch.zeros(R, dtype=torch.int32, device="cuda"),
+                             torch.full((R, 1), -1, dtype=torch.int32, device="cuda"), 1)
+    flat = torch.randn(R * 6 * dim + 1, device="cuda", generator=g).to(t)
+    for wide in (flat[1:].view(R, 6, dim), flat[:-1].view(R, 6, dim)):
+        q = wide[:, 1:5]
+        a = serving.kvq_attention(pool, batch, q, prefix_pages=pages, prefix_len=P)
+        b = serving.kvq_attention(pool, batch, q.contiguous(), prefix_pages=pages, prefix_len=P)
+        # a sequence of length 0 puts its row just before its own first position: it sees the whole prefix
+        assert torch.equal(a, b) and bool((a != 0).any())
