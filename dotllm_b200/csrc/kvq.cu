@@ -1,13 +1,19 @@
 // kvq.cu -- writing K/V rows into the 8-bit paged pool and reading them back.
 //
 // Per row and head: a = max |x|, scale = a / M, code = rne(x * (M * (1 / a))), M = 127 (int8) or 448
-// (e4m3), every operation rounded to fp32 by itself, so the codes are a function of the inputs alone.  Bound: HBM (each input value read once, one byte written for it) for long
-// prompts, launch latency for a decode step.  A (row, head) item is held by a group of D / 8 lanes
+// (e4m3), every operation rounded to fp32 by itself, so the codes are a function of the inputs alone.
+//
+// Bound: HBM (each input value read once, one byte written for it) for long prompts, launch latency for a
+// decode step.  A (row, head) item is held by a group of D / 8 lanes
 // (rounded up to a power of two), eight values per lane: one 16-byte load per lane for 16-bit
 // inputs, one 8-byte store of codes, the maximum by shuffles inside the group.  A group takes K and V
 // of one or two items, so a lane has up to four loads in flight while the rows' places are looked up.
 // Instructions come next to bytes: the maxima are taken on packed 16-bit pairs, and the two IEEE
 // divisions of an item are done by one lane per item.
+//
+// Measured on a B200 (copy bandwidth 6457 GB/s): writing 16381 rows of 8 x 128 bf16 values to e4m3 22.8 us,
+// 4460 GB/s (51 us with every lane dividing and 64-bit index divisions); reading 15988 such rows to fp32 31.6 us,
+// 5220 GB/s (43 us with eight neighbouring values per lane); a decode step of 8 rows of 8 x 64 4.2 us.
 #include "kvq.cuh"
 
 namespace llmdot {

@@ -29,6 +29,11 @@
 // bytes four positions of four consecutive dimensions, which byte permutes turn into fragments.
 // A row's weights are taken relative to a reference above its maximum at the time; while no weight comes
 // near fp16's limit no maximum is searched, and the barrier's vote tells all warps when one does.
+//
+// Measured on a B200, the own pages of 96 sequences with 3 to 5 drafted rows of 4 heads each, 64 to 2048
+// positions of 8 kv heads of 128: 94 us for 224 MB (2.4 TB/s; 0.54 instructions per clock and scheduler).
+// With a page per warp, maxima and O of all dimensions in each warp: 124 us.  Left out in turn (same sizes),
+// the scores' product saved 15 us, the output's 15, the loads 14, all of these 63.
 #include <algorithm>
 
 #include "kvq_attn.cuh"
