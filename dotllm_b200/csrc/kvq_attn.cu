@@ -656,8 +656,17 @@ int tiles_of(int dim, int64_t rows)  // 8-row tiles per CTA: 1, 2, 3, 4 or 8 (4 
     const int64_t n = std::max<int64_t>(1, (rows + 7) / 8);
     return (int)(n <= 4 ? n : dim == 256 ? 4 : 8);
 }
-// From this many rows (times heads) per kv head a segment is worth the wide kernel.
-constexpr int64_t WIDE_FROM = 48;
+// Whether `rows` rows (times heads) per kv head over `items` pages and heads in all go to the wide kernel.  It takes
+// the same time for 1 to 256 rows, the narrow one grows with every 8.  With work enough for all SMs the wide one
+// pays from 48 rows: 24 sequences of 1500 own positions, 8 heads of 128, bf16, in us, wide / narrow: 80.2 / 65.6 with
+// 24 rows, 81.8 / 97.0 with 40; 96 of 1000, fp16, heads of 64: 180 / 154 with 40.  With few items the latency of one
+// CTA's chunk counts, and it pays from 17 rows on own pages (4 of 3000: 26.8 / 39.0 with 20; 1 of 300: 16.4 / 18.5)
+// and with head_dim 256 (prefix of 2000, 24 rows: 22.6 / 30.8), from 25 on another prefix (of 2000: 26.8 / 24.7 with
+// 24, 26.8 / 32.4 with 32; of 12000: 36.0 / 51.6 with 32).
+bool wide_pays(const llmdot_kvq_pool &p, int64_t rows, int64_t items, bool own)
+{
+    return rows >= 48 || (items <= 2048 && rows >= (own || p.head_dim == 256 ? 17 : 25));
+}
 
 Plan make_plan(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const llmdot_kvq_attn &a)
 {
@@ -665,8 +674,8 @@ Plan make_plan(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const llmdot
     const int64_t G = a.heads / p.heads_kv, Hk = p.heads_kv, own_rows = (int64_t)b.max_rows * G, all_rows = (int64_t)b.rows * G;
     const int64_t npp = (a.prefix_len + KVQ_PAGE - 1) / KVQ_PAGE, wide = kvq_wide_rows(p.head_dim);
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
-    x.wide_p = a.type != T_F32 && npp > 0 && all_rows >= WIDE_FROM;
-    x.wide_s = a.type != T_F32 && own_rows >= WIDE_FROM;
+    x.wide_p = a.type != T_F32 && npp > 0 && wide_pays(p, all_rows, Hk * npp, false);
+    x.wide_s = a.type != T_F32 && wide_pays(p, own_rows, Hk * b.batch * b.max_pages, true);
     x.nt_p = tiles_of(p.head_dim, all_rows);
     x.nt_s = tiles_of(p.head_dim, own_rows);
     if (npp == 0) x.nt_p = x.nt_s;

@@ -134,3 +134,18 @@ def test_many_rows_from_unaligned_queries(gpu, typ):
         b = serving.kvq_attention(pool, batch, q.contiguous(), prefix_pages=pages, prefix_len=P)
         # a sequence of length 0 puts its row just before its own first position: it sees the whole prefix
         assert torch.equal(a, b) and bool((a != 0).any())
+
+
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+@pytest.mark.parametrize("dim,fmt", [(64, "i8"), (96, "e4m3"), (128, "i8"), (256, "e4m3")])
+@pytest.mark.parametrize("hk,prefix,lens,rows", [
+    (2, 1000, [333], [9]),               # 18 rows: prefix and own pages may go to different kernels
+    (2, 130, [700, 20], [12, 1]),        # 24 own rows, 26 on the prefix
+    (1, 0, [2900, 64, 65], [8, 9, 17]),  # 34 own rows at most, no prefix
+    (2, 6400, [8], [8]),                 # 16 rows
+    (32, 4500, [400, 1, 90], [10, 1, 3]),  # many heads: 28 rows on more pages
+])
+def test_middling_rows(gpu, typ, dim, fmt, hk, prefix, lens, rows):
+    """8 to 34 rows of a kv head (two query heads each), on either side of where the kernels change."""
+    run(fmt, typ, hk, 2, dim, prefix, lens, rows, window=0, q_scale=0.7)
+    run(fmt, typ, hk, 2, dim, prefix, lens, rows, window=150, softcap=20.0, k_ramp=3.0, v_ramp=3.0)
