@@ -12,8 +12,8 @@
 // divisions of an item are done by one lane per item.
 //
 // Measured on a B200 (copy bandwidth 6457 GB/s): writing 16381 rows of 8 x 128 bf16 values to e4m3 22.8 us,
-// 4460 GB/s (51 us with every lane dividing and 64-bit index divisions); reading 15988 such rows to fp32 31.6 us,
-// 5220 GB/s (43 us with eight neighbouring values per lane); a decode step of 8 rows of 8 x 64 4.2 us.
+// 4460 GB/s (51 us with every lane dividing and 64-bit index divisions); reading 15988 such rows to fp32 30.8 us,
+// 5360 GB/s (43 us with eight neighbouring values per lane); a decode step of 8 rows of 8 x 64 4.2 us.
 #include "kvq.cuh"
 
 namespace llmdot {
@@ -44,6 +44,10 @@ namespace {
 // Lanes per (row, head): D / 8, rounded up to a power of two (96 leaves 4 of 16 idle).
 template <int D> constexpr int kvq_lanes() { return D == 64 ? 8 : D == 256 ? 32 : 16; }
 constexpr int KVQ_THREADS = 256;
+// Items of a group where there are enough for four blocks per SM: two, so that more loads are in flight, but one for
+// fp32 heads of 128 and more, where a lane's own loads do.  Some 16000 rows of 8 heads, us with one / two:
+// reading bf16 128 22.6 / 18.7, fp32 64 17.2 / 16.5, fp32 128 30.9 / 32.3; writing bf16 256 42.7 / 39.1, fp32 128 29.9 / 30.8.
+template <typename T, int D> constexpr int kvq_each() { return sizeof(T) == 2 || D < 128 ? 2 : 1; }
 template <int D, int EACH> constexpr int kvq_items() { return KVQ_THREADS / kvq_lanes<D>() * EACH; }
 
 // Where a block's rows lie: for each row of the block's items the pool row of (page, head 0, slot), or -1
@@ -329,10 +333,10 @@ template <typename T, int D, int FMT> struct WriteOp {
                               int64_t ldv, int wide, cudaStream_t st)
     {
         const int64_t items = (int64_t)b.rows * p.heads_kv;
-        constexpr int N1 = kvq_items<D, 1>(), N2 = kvq_items<D, 2>();
+        constexpr int EACH = kvq_each<T, D>(), N1 = kvq_items<D, 1>(), N2 = kvq_items<D, EACH>();
         if (items >= 148 * 4 * N2)
-            kvq_write_kernel<T, D, FMT, 2><<<(unsigned)((items + N2 - 1) / N2), KVQ_THREADS, 0, st>>>(p, b, (const T *)k, (const T *)v,
-                                                                                                      ldk, ldv, wide);
+            kvq_write_kernel<T, D, FMT, EACH><<<(unsigned)((items + N2 - 1) / N2), KVQ_THREADS, 0, st>>>(p, b, (const T *)k, (const T *)v,
+                                                                                                         ldk, ldv, wide);
         else
             kvq_write_kernel<T, D, FMT, 1><<<(unsigned)((items + N1 - 1) / N1), KVQ_THREADS, 0, st>>>(p, b, (const T *)k, (const T *)v,
                                                                                                       ldk, ldv, wide);
@@ -344,9 +348,9 @@ template <typename T, int D, int FMT> struct ReadOp {
                               int wide, cudaStream_t st)
     {
         const int64_t items = (int64_t)b.rows * p.heads_kv;
-        constexpr int N1 = kvq_items<D, 1>(), N2 = kvq_items<D, 2>();
+        constexpr int EACH = kvq_each<T, D>(), N1 = kvq_items<D, 1>(), N2 = kvq_items<D, EACH>();
         if (items >= 148 * 4 * N2)
-            kvq_read_kernel<T, D, FMT, 2><<<(unsigned)((items + N2 - 1) / N2), KVQ_THREADS, 0, st>>>(p, b, (T *)k, (T *)v, ldk, ldv, wide);
+            kvq_read_kernel<T, D, FMT, EACH><<<(unsigned)((items + N2 - 1) / N2), KVQ_THREADS, 0, st>>>(p, b, (T *)k, (T *)v, ldk, ldv, wide);
         else
             kvq_read_kernel<T, D, FMT, 1><<<(unsigned)((items + N1 - 1) / N1), KVQ_THREADS, 0, st>>>(p, b, (T *)k, (T *)v, ldk, ldv, wide);
         return cudaGetLastError();
