@@ -27,7 +27,7 @@
 // CTAs per SM hide the latencies) and no joining of warps at the end.  The order of k inside a tile is free
 // as long as both operands agree; it is chosen so that a lane's K bytes are 16 consecutive ones, and its V
 // bytes four positions of four consecutive dimensions, which byte permutes turn into fragments.
-// A row's weights are taken relative to a reference above its maximum at the time; while no weight comes
+// A row's weights are taken relative to a reference below its maximum at the time; while no weight comes
 // near fp16's limit no maximum is searched, and the barrier's vote tells all warps when one does.
 //
 // Measured on a B200, the own pages of 96 sequences with 3 to 5 drafted rows of 4 heads each, 64 to 2048
@@ -125,15 +125,6 @@ __device__ __forceinline__ void store4(void *p, int64_t i, uint32_t type, bool w
 #pragma unroll
             for (int e = 0; e < 4; e++) o[e] = h[e];
     }
-}
-
-// What a row's reference stands above its maximum when it is set (powers of two), and the test that a packed
-// weight has come too near fp16's limit.  One fp16 per weight: 2^6 above, weights of 2 and more (an exponent
-// bit).  hi + lo: 2^4 below, so that lo stays a normal number; 2^13 and more.
-template <bool TWO> constexpr float ref_head() { return TWO ? -4.0f : 6.0f; }
-template <bool TWO> __device__ __forceinline__ uint32_t too_large(uint32_t p)
-{
-    return TWO ? ((p & 0x70007000u) + 0x10001000u) & 0x80008000u : p & 0x40004000u;
 }
 
 // PREC 0 (bf16): one fp16 for query and weight; 1 (fp16): hi + lo weights; 2 (fp32): hi + lo queries too.
@@ -309,7 +300,7 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
                     const uint32_t hi = pack(p[2 * hf], p[2 * hf + 1]);
-                    any |= too_large<(NP > 1)>(hi);
+                    any = __vmaxu2(any, hi);
                     b[0][hf] = transpose8(hi);
                     if (NP > 1) {
                         const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
@@ -320,7 +311,7 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
                 for (int h = 0; h < NP; h++)
                     *(uint2 *)(pw + (h * RT + nt * 8 + g) * PS + warp * 16 + t * 4) = make_uint2(b[h][0], b[h][1]);
             }
-            return any != 0;
+            return too_large(any);
         };
         if (now >= 0) {
             // ---- S^T = K Q^T: 16 positions
@@ -400,7 +391,7 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     const int n = nt * 8 + 2 * t + c;
-                    const float top = fmaxf(fmaxf(s_max[0][n], s_max[1][n]), fmaxf(s_max[2][n], s_max[3][n])) + ref_head<(NP > 1)>();
+                    const float top = fmaxf(fmaxf(s_max[0][n], s_max[1][n]), fmaxf(s_max[2][n], s_max[3][n])) - REF_HEAD;
                     float f = 1.0f;
                     if (top > ref[nt][c]) {
                         f = ex2(ref[nt][c] - top);  // nothing seen before: exp2(-inf) = 0

@@ -167,6 +167,12 @@ __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) <
 __device__ __forceinline__ float scale_pow(float vmax) { return __int_as_float(max(min(__float_as_int(vmax), 0x7e800000) & 0x7f800000, 0x00800000)); }
 __device__ __forceinline__ float pow_inverse(float p) { return __int_as_float(0x7f000000 - __float_as_int(p)); }
 
+// A row's weights are fp16.  Its reference is set 2^REF_HEAD below its maximum, so that weights of 2^-18 of the largest
+// are still normal numbers (the lo of a hi + lo pair, those of 2^-7), and set again when a packed weight reaches 2^13.
+constexpr float REF_HEAD = 4.0f;
+// Whether either half of a pair of weights (not negative) has; infinities and NaN have, too.
+__device__ __forceinline__ bool too_large(uint32_t p) { return ((p & 0x70007000u) + 0x10001000u) & 0x80008000u; }
+
 __device__ __forceinline__ float load_any(const void *p, int64_t i, uint32_t type)
 {
     if (type == T_F32) return __ldg((const float *)p + i);

@@ -42,14 +42,6 @@ namespace llmdot {
 namespace {
 
 constexpr long long WAIT_CLOCKS = 4000000000ll;  // about two seconds
-// A row's reference stands this power of two above its maximum (hi + lo: below, so that lo stays a normal
-// number), and a packed weight that has come too near fp16's limit: 2 and more (an exponent bit), or 2^13.
-template <bool TWO> constexpr float head_room() { return TWO ? -4.0f : 6.0f; }
-template <bool TWO> __device__ __forceinline__ uint32_t too_large(uint32_t p)
-{
-    return TWO ? ((p & 0x70007000u) + 0x10001000u) & 0x80008000u : p & 0x40004000u;
-}
-
 template <int D> struct Wide {
     static constexpr int TILES = D == 256 ? 1 : 2;
     static constexpr int UN = KVQ_PAGE;               // positions of a unit
@@ -441,10 +433,10 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                     sum[k] = add2(sum[k], e);
                     un2(mul2(e, v2), y, z);
                     const uint32_t hi = split(y, z, p, k >> 1, 2 * i + (k & 1));
-                    any |= TWO ? too_large<TWO>(hi) : hi;
+                    any = __vmaxu2(any, hi);
                 }
             }
-            if (__any_sync(0xffffffffu, (TWO ? any : too_large<TWO>(any)) != 0)) return false;  // (or a NaN)
+            if (__any_sync(0xffffffffu, too_large(any))) return false;  // (or a NaN)
 #pragma unroll
             for (int k = 0; k < 4; k++) l[k] = add2(l[k], sum[k]);
             hand_over(buf, p);
@@ -484,7 +476,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                 if (top[k] != -INFINITY) {
                     float x = top[k] * fq[k];
                     if (cap) x = capped<false>(x, a.at.softcap, inv_cap2) * 1.4426950408889634f;  // monotonic
-                    x += head_room<TWO>();
+                    x -= REF_HEAD;
                     if (x > ref[k]) {
                         // by a power of two, which the factor then is
                         const float to = ref[k] == -INFINITY ? x : ref[k] + ceilf(x - ref[k]);
@@ -646,7 +638,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                 float ve = 1.0f;
                 if (i == 0) {
                     vp = pw;
-                } else if (pw > vp * 8.0f) {  // weights stay far below 2
+                } else if (pw > vp * 8.0f) {  // weights stay far below the limit
                     ve = vp * pow_inverse(pw);
                     vp = pw;
                 }
