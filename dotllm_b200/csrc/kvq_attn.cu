@@ -6,10 +6,12 @@
 // Mathematics.  A code is an integer of at most 7 bits and sign, or an e4m3 value: exact in fp16.  The
 // query row is scaled by a power of two into fp16 (fp32 queries: as hi + lo, two products), so q . code
 // is a sum of exact products in fp32, and the key's scale multiplies the score.  The value's scale goes
-// into the weight: P_j = exp2(s_j - m) * (v_scale_j / 2^E), 2^E the largest power of two not above the
-// v_scales seen so far (raised with the running maximum, the sums rescaled by both), so that P stays in
-// fp16's normal range whatever the scales' size; P is hi + lo, or with bf16 queries, whose output has 8
-// bits, one fp16 (with fp16 outputs its rounding would add as much error again as the output's own).
+// into the weight: P_j = exp2(s_j - ref) * v_scale_j / 2^E.  ref and E are a row's own, from the positions that it
+// sees: ref was its maximum when it was set, E brought its largest exp2(s_j - ref) * v_scale_j into fp16's upper
+// range, and both rise (the sums rescaled by powers of two) when a later product of the row nears fp16's limit.
+// So neither a value that a row does not see nor one that it gives no weight costs it bits, whatever
+// the scales' size.  P is hi + lo, or with bf16 queries, whose output has 8 bits, one fp16 (with fp16 outputs its
+// rounding would add as much error again as the output's own).
 // The sum of exponentials, the maxima, both products' sums and the outputs are fp32.
 //
 // Work is cut into segments -- the prefix with every row of the batch, each sequence's own pages with
@@ -27,8 +29,8 @@
 // CTAs per SM hide the latencies) and no joining of warps at the end.  The order of k inside a tile is free
 // as long as both operands agree; it is chosen so that a lane's K bytes are 16 consecutive ones, and its V
 // bytes four positions of four consecutive dimensions, which byte permutes turn into fragments.
-// A row's weights are taken relative to a reference below its maximum at the time; while no weight comes
-// near fp16's limit no maximum is searched, and the barrier's vote tells all warps when one does.
+// While no weight comes near fp16's limit no maximum is searched, and the barrier's vote tells all warps when one
+// does; then only the rows that need it take new references, so that a row's result does not depend on its neighbours.
 //
 // Measured on a B200, the own pages of 96 sequences with 3 to 5 drafted rows of 4 heads each, 64 to 2048
 // positions of 8 kv heads of 128: 94 us for 224 MB (2.4 TB/s; 0.54 instructions per clock and scheduler).
@@ -135,7 +137,7 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
     constexpr int RT = 8 * NT, QS = D + Sh::QPAD, NQ = PREC == 2 ? 2 : 1, NP = PREC > 0 ? 2 : 1;
     constexpr bool QREG = NT * NQ * D / 8 <= 32;  // the query's fragments stay in registers
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float s_qf[RT], s_max[NW][RT], s_l[NW][RT], s_vmax[NW];
+    __shared__ float s_qf[RT], s_max[NW][RT], s_l[NW][RT];  // s_l: at the end; before, maxima with the values' scales
     __shared__ int s_lo[RT], s_hi[RT], s_row[RT];
     __half *sq = (__half *)(smem + Sh::OFF_Q);  // [NQ][RT][QS]
     __half *sp = sq + NQ * RT * QS;             // [2][NP][RT][PS]
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
     cp_wait<0>();
     __syncthreads();
     // this lane's rows are nt * 8 + 2 t and the next
-    float qf[NT][2], ref[NT][2], l[NT][2], o[Sh::GPW][2][NT][4];
+    float qf[NT][2], ref[NT][2], unit[NT][2], l[NT][2], o[Sh::GPW][2][NT][4];  // unit: 2^-E
     int clo[NT][2], chi[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -238,6 +240,7 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
             clo[nt][c] = s_lo[n];
             chi[nt][c] = s_hi[n];
             ref[nt][c] = -INFINITY;
+            unit[nt][c] = 1.0f;
             l[nt][c] = 0.0f;
         }
 #pragma unroll
@@ -245,7 +248,6 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
 #pragma unroll
             for (int e = 0; e < 4; e++) o[q][0][nt][e] = o[q][1][nt][e] = 0.0f;
     }
-    float vpow = 1.17549435e-38f;  // 2^E: O is in units of it
     const bool cap = a.at.softcap > 0.0f;
     const float inv_cap2 = cap ? 2.0f * 1.4426950408889634f / a.at.softcap : 0.0f;
     auto query = [&](int c, uint32_t (&qb)[NQ][NT][Sh::KB / 2]) {  // B fragments of piece c
@@ -282,8 +284,8 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
         const bool whole = u * KVQ_PAGE >= lo_max && u * KVQ_PAGE + KVQ_PAGE - 1 <= hi_min;
         // the weights of this warp's positions into shared memory, relative to the references
         auto weights = [&]() {
-            const float inv = pow_inverse(vpow);
             uint32_t any = 0;
+            bool over = false;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 float p[4];
@@ -292,15 +294,16 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
                 for (int e = 0; e < 4; e++) {
                     const float x = s[nt][e];
                     float y = ex2(x - ref[nt][e & 1]);
-                    p[e] = y * (vf[e >> 1] * inv);
+                    p[e] = y * vf[e >> 1] * unit[nt][e & 1];
                     if (!whole && x == -INFINITY) y = p[e] = 0.0f;  // whatever the unseen position holds
                     ln[nt][e & 1] += y;
                 }
+                over |= !(fmaxf(ln[nt][0], ln[nt][1]) < SUM_LIMIT);  // (not set yet: infinite)
                 uint32_t b[NP][2];
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
                     const uint32_t hi = pack(p[2 * hf], p[2 * hf + 1]);
-                    any = __vmaxu2(any, hi);
+                    any = hadd2(any, hi);
                     b[0][hf] = transpose8(hi);
                     if (NP > 1) {
                         const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
@@ -311,7 +314,7 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
                 for (int h = 0; h < NP; h++)
                     *(uint2 *)(pw + (h * RT + nt * 8 + g) * PS + warp * 16 + t * 4) = make_uint2(b[h][0], b[h][1]);
             }
-            return too_large(any);
+            return over || too_large(any);
         };
         if (now >= 0) {
             // ---- S^T = K Q^T: 16 positions
@@ -368,43 +371,41 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
         fetch(at1, sl, false);
         if (now < 0) continue;
         if (again) {
-            // ---- some weight is near the limit (or a reference is not set): search the page's maxima, raise
-            float vmax = t0 < len ? fmaxf(vf[0], 0.0f) : 0.0f;  // of positions that exist; a NaN does not count
-            if (t0 + 8 < len) vmax = fmaxf(vmax, vf[1]);
-            vmax = warp_max(vmax);
-            if (lane == 0) s_vmax[warp] = vmax;
+            // ---- some weight is near the limit (or a reference is not set): search the rows' maxima over the page, of
+            // the scores and with the values' scales, and raise the references of the rows that need it
+            const float lv[2] = {log2_abs(vf[0]), log2_abs(vf[1])};
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    float mx = fmaxf(s[nt][c], s[nt][c + 2]);
+                for (int c = 0; c < 2; c++) {  // (a NaN does not count)
+                    float mx = fmaxf(s[nt][c], s[nt][c + 2]), mv = fmaxf(s[nt][c] + lv[0], s[nt][c + 2] + lv[1]);
 #pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                    if (g == 0) s_max[warp][nt * 8 + 2 * t + c] = mx;
+                    for (int d = 4; d < 32; d <<= 1) {
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                        mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, d));
+                    }
+                    if (g == 0) {
+                        s_max[warp][nt * 8 + 2 * t + c] = mx;
+                        s_l[warp][nt * 8 + 2 * t + c] = mv;
+                    }
                 }
             __syncthreads();
-            const float vp = fmaxf(vpow, scale_pow(fmaxf(fmaxf(s_vmax[0], s_vmax[1]), fmaxf(s_vmax[2], s_vmax[3]))));
-            const float ve = vpow * pow_inverse(vp);
-            vpow = vp;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     const int n = nt * 8 + 2 * t + c;
-                    const float top = fmaxf(fmaxf(s_max[0][n], s_max[1][n]), fmaxf(s_max[2][n], s_max[3][n])) - REF_HEAD;
-                    float f = 1.0f;
-                    if (top > ref[nt][c]) {
-                        f = ex2(ref[nt][c] - top);  // nothing seen before: exp2(-inf) = 0
-                        ref[nt][c] = top;
-                        l[nt][c] *= f;
-                    }
-                    f *= ve;
+                    const float top = fmaxf(fmaxf(s_max[0][n], s_max[1][n]), fmaxf(s_max[2][n], s_max[3][n]));
+                    const float topv = fmaxf(fmaxf(s_l[0][n], s_l[1][n]), fmaxf(s_l[2][n], s_l[3][n]));
+                    float fl, fo;
+                    if (!raise_refs(top, topv, ref[nt][c], unit[nt][c], fl, fo)) continue;
+                    l[nt][c] *= fl;
 #pragma unroll
                     for (int q = 0; q < Sh::GPW; q++)
 #pragma unroll
                         for (int j = 0; j < 2; j++) {
-                            o[q][j][nt][c] *= f;
-                            o[q][j][nt][c + 2] *= f;
+                            o[q][j][nt][c] *= fo;
+                            o[q][j][nt][c + 2] *= fo;
                         }
                 }
             weights();
@@ -490,9 +491,9 @@ __global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 
                         x[3] += v.w;
                     }
                     const int d = (grp + 4 * q) * 32 + g * 4;
-                    const float f = a.direct ? (L == 0.0f ? 0.0f : vpow / L) : vpow;
+                    const float f = a.direct ? 1.0f / L : 1.0f, u = pow_inverse(unit[nt][c]);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[e] = a.direct && L == 0.0f ? 0.0f : x[e] * f;
+                    for (int e = 0; e < 4; e++) x[e] = a.direct && L == 0.0f ? 0.0f : x[e] * f * u;
                     if (a.direct) store4(a.out, row * a.ldo + (int64_t)head * D + d, a.at.type, a.wide != 0, x);
                     else *(float4 *)(a.part_o + (slot * RH + rh) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
                 }

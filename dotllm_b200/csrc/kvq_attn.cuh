@@ -137,6 +137,12 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi)
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
+__device__ __forceinline__ uint32_t hadd2(uint32_t a, uint32_t b)
+{
+    uint32_t d;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
 __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b)
 {
     uint32_t d;
@@ -163,15 +169,42 @@ __device__ __forceinline__ int row_exponent(float top)
     return b > 0 && b < 0x7f800000 ? min(14 + 127 - (b >> 23), 126) : 0;
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
-// The power of two (normal, at most 2^126) not above a value scale; its inverse is exact.
-__device__ __forceinline__ float scale_pow(float vmax) { return __int_as_float(max(min(__float_as_int(vmax), 0x7e800000) & 0x7f800000, 0x00800000)); }
-__device__ __forceinline__ float pow_inverse(float p) { return __int_as_float(0x7f000000 - __float_as_int(p)); }
+__device__ __forceinline__ float pow_inverse(float p) { return __int_as_float(0x7f000000 - __float_as_int(p)); }  // p a power of two
+__device__ __forceinline__ int pow_exponent(float p) { return (__float_as_int(p) >> 23) - 127; }
+__device__ __forceinline__ float log2_abs(float x)  // -infinity for 0 and subnormal numbers
+{
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fabsf(x)));
+    return y;
+}
 
-// A row's weights are fp16.  Its reference is set 2^REF_HEAD below its maximum, so that weights of 2^-18 of the largest
-// are still normal numbers (the lo of a hi + lo pair, those of 2^-7), and set again when a packed weight reaches 2^13.
-constexpr float REF_HEAD = 4.0f;
-// Whether either half of a pair of weights (not negative) has; infinities and NaN have, too.
-__device__ __forceinline__ bool too_large(uint32_t p) { return ((p & 0x70007000u) + 0x10001000u) & 0x80008000u; }
+// A row's two references.  Its exponentials are exp2(s - ref); its weights those times the values' scales times `unit`,
+// a power of two, as fp16.  When they are set, `ref` is the row's maximum and `unit` brings its largest weight into
+// (2^3, 2^4], so that weights of 2^-17 of the largest are still normal numbers (the lo of a hi + lo pair, those of 2^-6).
+// They are set again where a weight has reached 2^8, which a lane notices when its at most 32 packed weights sum to 2^13
+// (an addition of two halves costs less than a test, and an infinity or NaN stays one), or when the exponentials grow
+// without their values (scales of nearly 0) and their sum reaches SUM_LIMIT.
+constexpr float REF_HEAD = 4.0f, REF_LIMIT = 8.0f;
+constexpr float SUM_LIMIT = 18446744073709551616.0f, SUM_LIMIT_LOG = 64.0f;
+// Whether either half of such a sum is 2^13 or more, infinite or NaN, or negative (by a negative scale).
+__device__ __forceinline__ bool too_large(uint32_t p) { return (((p & 0x70007000u) + 0x10001000u) | p) & 0x80008000u; }
+// top: the largest score (base 2) that the row sees in a page; topv: with the logs of the values' scales.  False where the
+// references hold for them; else they rise, and fl and fo are the (exact) factors for what was summed before: the
+// exponentials, and the products.  The margins keep the logs' rounding from leaving a weight past the limit unanswered.
+__device__ __forceinline__ bool raise_refs(float top, float topv, float &ref, float &unit, float &fl, float &fo)
+{
+    if (top == -INFINITY) return false;
+    const bool first = ref == -INFINITY;
+    const float E = -pow_exponent(unit);
+    if (!first && topv - ref - E < REF_LIMIT - 0.01f && top - ref < SUM_LIMIT_LOG - 7.0f) return false;
+    const float d = first ? 0.0f : ceilf(fmaxf(top - ref, 0.0f)), to = first ? top : ref + d;
+    const float least = fminf(fmaxf(ceilf(topv - to) - REF_HEAD, -126.0f), 126.0f), Eo = first ? least : fmaxf(E - d, least);
+    fl = ex2(-d);
+    fo = ex2(E - d - Eo);
+    ref = to;
+    unit = __int_as_float((127 - (int)Eo) << 23);
+    return true;
+}
 
 __device__ __forceinline__ float load_any(const void *p, int64_t i, uint32_t type)
 {

@@ -9,10 +9,11 @@
 // and its roles overlap, 64 positions (a page) at a time:
 //   warps of a tile (4 each)  S from TMEM 64 columns at a time in fragments of 4 rows by 2 columns a lane
 //                             (a lane so needs a quarter of the columns' scales), weights as fp16 back
-//                             into TMEM over S.  The weights are taken relative to a row's reference,
-//                             set by its maximum; only when a weight comes near fp16's limit is the
-//                             maximum searched, the reference raised, and the sums and O rescaled, which
-//                             after the first positions is rare
+//                             into TMEM over S.  The weights are taken relative to a row's two references,
+//                             one for the exponentials and one with the values' scales (raise_refs); only when a
+//                             weight comes near fp16's limit are the maxima searched, the references of the
+//                             rows that need it raised, and their sums and O rescaled, which after the first
+//                             positions is rare
 //   4 converting warps        codes from global memory (three K or V pages' loads in flight) to fp16 K
 //                             and V operands in shared memory, scales beside them
 //   1 warp per tile           one thread issues tcgen05.mma: S = Q K^T and O += P V with P and the
@@ -42,6 +43,7 @@ namespace llmdot {
 namespace {
 
 constexpr long long WAIT_CLOCKS = 4000000000ll;  // about two seconds
+
 template <int D> struct Wide {
     static constexpr int TILES = D == 256 ? 1 : 2;
     static constexpr int UN = KVQ_PAGE;               // positions of a unit
@@ -53,7 +55,7 @@ template <int D> struct Wide {
     static constexpr uint32_t Q_BYTES = KBLK * Q_BLK, K_BYTES = KBLK * K_BLK;
     static constexpr uint32_t STAGE = 2 * K_BYTES;  // K, then V alike
     static constexpr uint32_t OFF_Q = STAGES * STAGE;
-    static constexpr uint32_t OFF_SC = OFF_Q + TILES * Q_BYTES;  // per stage: K scales, V scales, {rescale, 2^E, no page, -}
+    static constexpr uint32_t OFF_SC = OFF_Q + TILES * Q_BYTES;  // per stage: K scales, V scales, 1 where there is no page
     static constexpr uint32_t SC_STAGE = 2 * UN * 4 + 16;
     static constexpr uint32_t OFF_BAR = OFF_SC + STAGES * SC_STAGE;
     // barriers: a stage is converted, read; S, P and P V of a tile's two places; the drain
@@ -352,7 +354,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
         // ---- fragments: this lane's four rows (of the warp's 32) are g + 8 k, its columns 8 i + 2 t and the next
         const int g = lane >> 2, t = lane & 3;
         int flo[4], fhi[4];
-        float fq[4], ref[4], vpow = 0.0f;  // ref: base 2; -infinity until the row has seen a position
+        float fq[4], ref[4], unit[4];  // ref: base 2; -infinity until the row has seen a position
         F2 l[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -360,9 +362,10 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             fhi[k] = __shfl_sync(0xffffffffu, hi, g + 8 * k);
             fq[k] = __shfl_sync(0xffffffffu, qf, g + 8 * k);
             ref[k] = -INFINITY;
+            unit[k] = 1.0f;
             l[k] = f2(0.0f, 0.0f);
         }
-        bool ok = tile < nact;
+        bool ok = tile < nact, wild = false;  // wild: some row's unit is too large or small to go through an exponential
         // O times f (lane = row), once the products that add to it (through unit i) are complete.
         auto rescale_o = [&](int i, float f) {
             ok = wait(W::B_O + tile * 2 + (i & 1), (i >> 1) & 1);
@@ -406,8 +409,20 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             }
             return hi;
         };
+        // Whether a page's sums or weights have passed the limits for a row of the warp (or are NaN).
+        auto passed = [&](const F2 (&sum)[4], uint32_t any) {
+            bool over = too_large(any);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                float x, y;
+                un2(sum[k], x, y);
+                over |= !(x + y < SUM_LIMIT);
+            }
+            return __any_sync(0xffffffffu, over) != 0;
+        };
         // A page that the rows see whole, without a cap: false (and nothing done) when a weight comes too near
-        // the limit and the reference has to rise.
+        // the limit and the references have to rise.  `unit` goes into the exponent (so not where a row is `wild`), and
+        // comes out of the page's sums.
         auto plain_page = [&](const float *ks, const float *vs, int buf) -> bool {
             uint32_t s[2][32], p[NP][2][16], any = 0;
             tmem_ld_frag(tm + W::C_S + 64 * buf, s[0]);
@@ -416,7 +431,8 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 q2[k] = f2(fq[k], fq[k]);
-                off[k] = f2(-ref[k], -ref[k]);
+                const float at = pow_exponent(unit[k]) - ref[k];
+                off[k] = f2(at, at);
                 sum[k] = f2(0.0f, 0.0f);
             }
             tmem_ld_wait();
@@ -433,20 +449,23 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                     sum[k] = add2(sum[k], e);
                     un2(mul2(e, v2), y, z);
                     const uint32_t hi = split(y, z, p, k >> 1, 2 * i + (k & 1));
-                    any = __vmaxu2(any, hi);
+                    any = hadd2(any, hi);
                 }
             }
-            if (__any_sync(0xffffffffu, too_large(any))) return false;  // (or a NaN)
+#pragma unroll
+            for (int k = 0; k < 4; k++) sum[k] = mul2(sum[k], f2(pow_inverse(unit[k]), pow_inverse(unit[k])));
+            if (passed(sum, any)) return false;
 #pragma unroll
             for (int k = 0; k < 4; k++) l[k] = add2(l[k], sum[k]);
             hand_over(buf, p);
             return true;
         };
-        // The search for the rows' maxima over a page, and the references raised where they stand too low.  MASKED: scores of positions that a row does not see do not count.
-        auto search = [&](int i, const float *ks, int buf, auto masked) {
+        // The search for the rows' maxima over a page, of the scores and with the values' scales, and the references raised
+        // where they stand too low.  MASKED: scores of positions that a row does not see do not count.
+        auto search = [&](int i, const float *ks, const float *vs, int buf, auto masked) {
             constexpr bool MASKED = decltype(masked)::value;
             const int j0 = u0 * KVQ_PAGE + i * UN + 2 * t;
-            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, topv[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 uint32_t s[32];
@@ -454,15 +473,21 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                 tmem_ld_wait();
 #pragma unroll
                 for (int c = 0; c < 8; c++) {
-                    const float2 kf = *(const float2 *)(ks + 8 * c + 2 * t);
+                    const float2 kf = *(const float2 *)(ks + 8 * c + 2 * t), vf = *(const float2 *)(vs + 8 * c + 2 * t);
+                    const float lx = log2_abs(vf.x), ly = log2_abs(vf.y);
                     const int j = j0 + 8 * c;
 #pragma unroll
                     for (int r = 0; r < 2; r++) {
                         const int k = 2 * h + r;
-                        float x = __uint_as_float(s[4 * c + 2 * r]) * kf.x, y = __uint_as_float(s[4 * c + 2 * r + 1]) * kf.y;
+                        float x = __uint_as_float(s[4 * c + 2 * r]) * kf.x * fq[k], y = __uint_as_float(s[4 * c + 2 * r + 1]) * kf.y * fq[k];
+                        if (cap) {
+                            x = capped<false>(x, a.at.softcap, inv_cap2) * 1.4426950408889634f;
+                            y = capped<false>(y, a.at.softcap, inv_cap2) * 1.4426950408889634f;
+                        }
                         if (MASKED && (j < flo[k] || j > fhi[k])) x = -INFINITY;
                         if (MASKED && (j + 1 < flo[k] || j + 1 > fhi[k])) y = -INFINITY;
-                        top[k] = fmaxf(top[k], fmaxf(x, y));
+                        top[k] = fmaxf(top[k], fmaxf(x, y));  // (a NaN does not count)
+                        topv[k] = fmaxf(topv[k], fmaxf(x + lx, y + ly));
                     }
                 }
             }
@@ -470,23 +495,18 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             bool moved = false;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
-                top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
-                f[k] = 1.0f;
-                if (top[k] != -INFINITY) {
-                    float x = top[k] * fq[k];
-                    if (cap) x = capped<false>(x, a.at.softcap, inv_cap2) * 1.4426950408889634f;  // monotonic
-                    x -= REF_HEAD;
-                    if (x > ref[k]) {
-                        // by a power of two, which the factor then is
-                        const float to = ref[k] == -INFINITY ? x : ref[k] + ceilf(x - ref[k]);
-                        f[k] = ex2(ref[k] - to);
-                        ref[k] = to;
-                        moved = true;
-                    }
+#pragma unroll
+                for (int d = 1; d < 4; d <<= 1) {
+                    top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], d));
+                    topv[k] = fmaxf(topv[k], __shfl_xor_sync(0xffffffffu, topv[k], d));
                 }
-                l[k] = mul2(l[k], f2(f[k], f[k]));
+                float fl = 1.0f;
+                f[k] = 1.0f;
+                if (raise_refs(top[k], topv[k], ref[k], unit[k], fl, f[k])) moved = true;
+                l[k] = mul2(l[k], f2(fl, fl));
             }
+            wild = __any_sync(0xffffffffu, max(max(abs(pow_exponent(unit[0])), abs(pow_exponent(unit[1]))),
+                                               max(abs(pow_exponent(unit[2])), abs(pow_exponent(unit[3])))) > 60);
             if (i > 0 && __any_sync(0xffffffffu, moved)) {
                 float mine = 1.0f;  // of the row that is this lane
 #pragma unroll
@@ -497,10 +517,13 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                 rescale_o(i - 1, mine);
             }
         };
-        // The weights of a page, with masks and cap.
-        auto masked_page = [&](int i, const float *ks, const float *vs, int buf) {
+        // The weights of a page, with masks and cap: false (and nothing done) as above, unless `last`.
+        auto masked_page = [&](int i, const float *ks, const float *vs, int buf, bool last) -> bool {
             const int j0 = u0 * KVQ_PAGE + i * UN + 2 * t;
-            uint32_t p[NP][2][16];
+            uint32_t p[NP][2][16], any = 0;
+            F2 sum[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) sum[k] = f2(0.0f, 0.0f);
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 uint32_t s[32];
@@ -521,12 +544,18 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                         x = ex2(x - off);
                         y = ex2(y - off);
                         const bool gx = j < flo[k] || j > fhi[k], gy = j + 1 < flo[k] || j + 1 > fhi[k];
-                        l[k] = add2(l[k], f2(gx ? 0.0f : x, gy ? 0.0f : y));
-                        split(gx ? 0.0f : x * vf.x, gy ? 0.0f : y * vf.y, p, h, 2 * c + r);  // whatever an unseen position holds
+                        sum[k] = add2(sum[k], f2(gx ? 0.0f : x, gy ? 0.0f : y));
+                        // whatever an unseen position holds
+                        const uint32_t hi = split(gx ? 0.0f : x * vf.x * unit[k], gy ? 0.0f : y * vf.y * unit[k], p, h, 2 * c + r);
+                        any = hadd2(any, hi);
                     }
                 }
             }
+            if (passed(sum, any) && !last) return false;
+#pragma unroll
+            for (int k = 0; k < 4; k++) l[k] = add2(l[k], sum[k]);
             hand_over(buf, p);
+            return true;
         };
         bool known = false;  // every row of the warp has seen a position
         for (int i = 0; i < n && ok; i++) {
@@ -535,23 +564,18 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             if (!(ok = __all_sync(0xffffffffu, ok))) break;
             fence_after();
             const float *ks = (const float *)(smem + W::OFF_SC + st * W::SC_STAGE), *vs = ks + UN;
-            const float4 ex = *(const float4 *)(vs + UN);
-            vpow = ex.y;
-            if (i > 0 && ex.x != 1.0f) {  // the values' unit rose: O follows (every row alike)
-                rescale_o(i - 1, ex.x);
-                if (!ok) break;
-            }
-            if (ex.z != 0.0f || p0 > hi_end || p0 + KVQ_PAGE <= lo_min) {  // nothing for this warp's rows
+            if (vs[UN] != 0.0f || p0 > hi_end || p0 + KVQ_PAGE <= lo_min) {  // nothing for this warp's rows
                 const uint32_t zero[NP][2][16] = {};
                 hand_over(buf, zero);
-            } else if (!cap && p0 >= lo_max && p0 + KVQ_PAGE - 1 <= hi_min) {  // everything
+            } else if (!cap && !wild && p0 >= lo_max && p0 + KVQ_PAGE - 1 <= hi_min) {  // everything
                 if (known && plain_page(ks, vs, buf)) continue;
-                search(i, ks, buf, std::false_type{});
+                search(i, ks, vs, buf, std::false_type{});
                 known = true;
-                if (ok && !plain_page(ks, vs, buf)) masked_page(i, ks, vs, buf);  // (a NaN stays one)
+                if (ok && (wild || !plain_page(ks, vs, buf))) masked_page(i, ks, vs, buf, true);  // (a NaN stays one)
             } else {
-                search(i, ks, buf, std::true_type{});
-                if (ok) masked_page(i, ks, vs, buf);
+                if (known && masked_page(i, ks, vs, buf, false)) continue;
+                search(i, ks, vs, buf, std::true_type{});
+                if (ok) masked_page(i, ks, vs, buf, true);
                 known = __all_sync(0xffffffffu, fminf(fminf(ref[0], ref[1]), fminf(ref[2], ref[3])) > -INFINITY);
             }
         }
@@ -576,7 +600,9 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
         }
         if (ok && n > 0) {  // O: four lanes write 32 consecutive bytes of a row
             fence_after();
-            const F2 vp2 = f2(vpow, vpow);
+            F2 u2[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) u2[k] = f2(pow_inverse(unit[k]), pow_inverse(unit[k]));
 #pragma unroll 1
             for (int c = 0; c < (D + 63) / 64; c++) {
 #pragma unroll
@@ -591,7 +617,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             float x, y;
-                            un2(mul2(f2(__uint_as_float(v[4 * i + 2 * r]), __uint_as_float(v[4 * i + 2 * r + 1])), vp2), x, y);
+                            un2(mul2(f2(__uint_as_float(v[4 * i + 2 * r]), __uint_as_float(v[4 * i + 2 * r + 1])), u2[k]), x, y);
                             if (to[k] >= 0 && 64 * c + 8 * i < D) o[4 * i] = make_float2(x, y);
                         }
                     }
@@ -625,27 +651,13 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
             c[0] = none(page) ? 0.0f : __ldg(s);
             c[1] = none(page) ? 0.0f : __ldg(s + 32);
         };
-        float vp = 0.0f;  // 2^E (warp 0)
         bool ok = true;
         auto put_scales = [&](int i, int page, const float (&c)[2]) {
             float *ks = (float *)(smem + W::OFF_SC + i % STAGES * W::SC_STAGE), *vs = ks + UN;
             if (dw == 0) {
-                const int t0 = u0 * KVQ_PAGE + i * UN + lane;
-                float top = 0.0f;  // of positions that exist; a NaN does not count
-                if (t0 < len) top = fmaxf(top, c[0] * code_unit<FMT>());
-                if (t0 + 32 < len) top = fmaxf(top, c[1] * code_unit<FMT>());
-                const float pw = scale_pow(warp_max(top));
-                float ve = 1.0f;
-                if (i == 0) {
-                    vp = pw;
-                } else if (pw > vp * 8.0f) {  // weights stay far below the limit
-                    ve = vp * pow_inverse(pw);
-                    vp = pw;
-                }
-                const float inv = pow_inverse(vp);
-                vs[lane] = c[0] * code_unit<FMT>() * inv;
-                vs[lane + 32] = c[1] * code_unit<FMT>() * inv;
-                if (lane == 0) *(float4 *)(vs + UN) = make_float4(ve, vp, none(page) ? 1.0f : 0.0f, 0.0f);
+                vs[lane] = c[0] * code_unit<FMT>();
+                vs[lane + 32] = c[1] * code_unit<FMT>();
+                if (lane == 0) vs[UN] = none(page) ? 1.0f : 0.0f;
             } else if (dw == 1) {
                 ks[lane] = c[0];
                 ks[lane + 32] = c[1];

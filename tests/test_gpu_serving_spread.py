@@ -138,6 +138,122 @@ def queries(seed, typ, *shape, scale=1.0):
 def random_parts(seed, hk, dim, *lens):
     return [(noise(seed + 2 * i, n, hk, dim), noise(seed + 2 * i + 1, n, hk, dim)) for i, n in enumerate(lens)]
 
+
+# group 2: few rows per kv head; group 20: 60 and more, the many-row kernel (for 16-bit queries)
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("dim,fmt", [(64, "i8"), (96, "e4m3"), (128, "i8"), (256, "e4m3")])
+@pytest.mark.parametrize("group", [2, 20])
+def test_large_value_of_a_later_row(gpu, typ, dim, fmt, group):
+    """The last drafted row's own value is 2^k times the others': the earlier rows, which do not see it, keep their precision."""
+    for k in (8, 12, 16, 20, 40):
+        parts = random_parts(k, 2, dim, 70, 60, 9)
+        parts[1][1][-1] *= 2.0 ** k
+        c = Held(fmt, parts, [3, 2])
+        q = queries(1, typ, 5, 2 * group, dim)
+        c.check(q, typ, c.attend(q), only=(0, 1) if typ == "f16" else None)  # (2^40 is beyond fp16)
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("dim,fmt", [(64, "e4m3"), (96, "i8"), (128, "e4m3"), (256, "i8")])
+@pytest.mark.parametrize("group", [2, 20])
+def test_large_value_outside_the_window(gpu, typ, dim, fmt, group):
+    """The same at positions that the window hides, before (in the prefix's page that is still read) and in own pages."""
+    for k in (8, 12, 16, 20, 40):
+        parts = random_parts(k, 2, dim, 150, 100)
+        parts[0][1][:120] *= 2.0 ** k
+        parts[0][1][120:] *= 2.0 ** -3
+        c = Held(fmt, parts, [3])
+        q = queries(2, typ, 3, 2 * group, dim)
+        c.check(q, typ, c.attend(q, window=125), window=125)  # the first row sees from position 123 on
+        parts = random_parts(k, 2, dim, 0, 130)
+        parts[1][1][:70] *= 2.0 ** k
+        c = Held(fmt, parts, [3])
+        c.check(q, typ, c.attend(q, window=50), window=50)  # from position 78 on
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("dim,fmt", [(64, "i8"), (96, "e4m3"), (128, "i8"), (256, "e4m3")])
+@pytest.mark.parametrize("group", [2, 20])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+def test_large_value_with_next_to_no_weight(gpu, typ, dim, fmt, group, softcap):
+    """A position that every row sees with a weight of 2^-50 or less, its value 2^20 times the others': what it adds is
+    far below the others' rounding, first or last in the order of pages, and they keep theirs."""
+    for at in (0, 199):
+        parts = random_parts(at, 2, dim, 200, 40)
+        for part in parts:
+            part[0][..., 0] = 0.0
+        parts[0][0][at] = 0.0
+        parts[0][0][at, :, 0] = -40.0 * dim ** 0.5 / 4.0  # a score of -40, -30 tanh(4 / 3) under the cap
+        parts[0][1][at] *= 2.0 ** 12 if softcap else 2.0 ** 20
+        c = Held(fmt, parts, [4])
+        q = queries(3, typ, 4, 2 * group, dim)
+        q[..., 0] = 4.0
+        c.check(q, typ, c.attend(q, softcap=softcap), softcap=softcap)
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("dim,fmt", [(64, "i8"), (96, "e4m3"), (128, "i8"), (256, "e4m3")])
+@pytest.mark.parametrize("group", [2, 20])
+def test_value_scales_of_every_size(gpu, typ, dim, fmt, group):
+    """All values tiny, all huge, and orders that change from page to page, up and down."""
+    sizes = [0, -8, 3] if typ == "f16" else [0, -90, 100]
+    for k in sizes:
+        parts = random_parts(k + 100, 2, dim, 130, 70)
+        for _, v in parts:
+            v *= 2.0 ** k
+        c = Held(fmt, parts, [3])
+        q = queries(4, typ, 3, 2 * group, dim)
+        c.check(q, typ, c.attend(q))
+    steps = [5, -6, 0, -9] if typ == "f16" else [40, -40, 0, -60]
+    for order in (steps, steps[::-1]):
+        parts = random_parts(7, 2, dim, 256, 70)
+        for i, k in enumerate(order):
+            parts[0][1][64 * i:64 * (i + 1)] *= 2.0 ** k
+        c = Held(fmt, parts, [3])
+        q = queries(5, typ, 3, 2 * group, dim)
+        c.check(q, typ, c.attend(q))
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("group", [2, 20])
+def test_values_of_zero_under_a_large_score(gpu, typ, group):
+    """A position that takes nearly all the weight and whose value is zero, by scores of up to 100: what is left of the
+    others is still right to a row's own precision."""
+    import torch
+    for score in (10.0, 40.0, 80.0):
+        parts = random_parts(11, 2, 128, 300, 30)
+        for part in parts:
+            part[0][..., 0] = 0.0
+        parts[0][0][100] = 0.0
+        parts[0][0][100, :, 0] = score * 128 ** 0.5 / 4.0
+        parts[0][1][100] = 0.0
+        c = Held("i8", parts, [3])
+        q = queries(6, typ, 3, 2 * group, 128)
+        q[..., 0] = 4.0
+        out, lse = c.attend(q)
+        c.check(q, typ, (out, lse))
+        if typ != "f16":
+            assert bool((out != 0).any()) and bool(torch.isfinite(lse).all())
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("dim,fmt", [(64, "i8"), (128, "e4m3"), (256, "i8")])
+@pytest.mark.parametrize("group", [2, 20])
+def test_attention_sink(gpu, typ, dim, fmt, group):
+    """The first position takes most of the weight and has a small value, as a model's first token often does: the output
+    is made of the many small weights."""
+    for gap in (8.0, 10.0, 11.0, 13.0):
+        parts = random_parts(12, 2, dim, 4096, 70)
+        for part in parts:
+            part[0][..., 0] = 0.0
+        parts[0][0][0] = 0.0
+        parts[0][0][0, :, 0] = gap * dim ** 0.5 / 4.0
+        parts[0][1][0] *= 0.01
+        c = Held(fmt, parts, [3])
+        q = queries(7, typ, 3, 2 * group, dim, scale=0.3)
+        q[..., 0] = 4.0
+        c.check(q, typ, c.attend(q))
+
 @pytest.mark.parametrize("typ", ["f16", "bf16"])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_long_tail_of_small_weights(gpu, typ, dim):
@@ -153,3 +269,17 @@ def test_long_tail_of_small_weights(gpu, typ, dim):
     q = queries(8, typ, 64, 32 * 16, dim, scale=0.3)
     q[..., 0] = 4.0
     c.check(q, typ, c.attend(q), chain=32768)
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("group", [2, 20])
+def test_negative_scales(gpu, typ, group):
+    """A code stands for code * scale whatever the scale's sign."""
+    parts = random_parts(16, 2, 128, 300, 70)
+    c = Held("i8", parts, [3])
+    for which, scales in ((0, c.pool.k_scale), (1, c.pool.v_scale)):
+        scales[:, :, 1::3] *= -1.0
+        for n, held in enumerate(c.values[which]):
+            held[[j for j in range(held.shape[0]) if j % PAGE % 3 == 1]] *= -1.0
+    q = queries(9, typ, 3, 2 * group, 128)
+    c.check(q, typ, c.attend(q))
