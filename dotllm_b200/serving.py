@@ -191,11 +191,13 @@ def verify_draft(p: torch.Tensor, q: Optional[torch.Tensor], draft: torch.Tensor
         _bad("verify_draft: p holds no row")
 
     def ld(name, t, n):
+        """From one of the B * n rows to the next: the sequences' stride where each has one row."""
         s0, s1, s2 = t.stride()
+        row = s1 if n > 1 else s0
         if t.dtype is not torch.float32 or t.shape != (B, n, V) or t.get_device() != device or (s2 != 1 and V > 1) \
-                or (s0 != n * s1 and n > 0 and B > 1) or (s1 < V and n > 1):
-            _bad(f"verify_draft: {name} must be float32 [{B}, {n}, {V}] on cuda:{device} with evenly strided rows")
-        return max(s1, V)
+                or (s0 != n * s1 and n > 1 and B > 1) or (row < V and B * n > 1):
+            _bad(f"verify_draft: {name} must be float32 [{B}, {n}, {V}] on cuda:{device} with evenly strided rows that do not overlap")
+        return row if B * n > 1 else V
 
     ld_p = ld("p", p, k1)
     if q is not None and k == 0:

@@ -125,3 +125,102 @@ def test_serving_refuses_host_tensors():
         serving.KvqBatch(torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32), 1)
     with pytest.raises(ValueError):
         serving.verify_draft(torch.zeros(1, 1, 8), None, torch.zeros(1, 0, dtype=torch.int32), torch.zeros(1, 1))
+
+
+class OnDevice:
+    """A host tensor that says it is on device 0: what a call would hand to the library, without a device."""
+    is_cuda = True
+
+    def __init__(self, t):
+        self.t, self.shape, self.dtype = t, t.shape, t.dtype
+
+    def dim(self):
+        return self.t.dim()
+
+    def stride(self):
+        return self.t.stride()
+
+    def is_contiguous(self):
+        return self.t.is_contiguous()
+
+    def get_device(self):
+        return 0
+
+    def data_ptr(self):
+        return self.t.data_ptr()
+
+    def new_empty(self, *a, **kw):
+        return OnDevice(self.t.new_empty(*a, **kw))
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The arguments of the library calls that would have been made."""
+    from dotllm_b200 import serving
+    made = []
+    monkeypatch.setattr(serving, "lib", lambda: type("L", (), {"llmdot_cuda_verify_draft": None})())
+    monkeypatch.setattr(serving, "_call", lambda fn, device, *args: made.append(args))
+    return made
+
+
+def rows_end(start, rows, ld, vocab):
+    """Address behind the last row that the kernel may read."""
+    return start + 4 * ((rows - 1) * ld + vocab)
+
+
+def test_verify_reads_stay_inside_their_tensors(launches):
+    """Whatever strides are accepted, row b * n + i of the call is row (b, i) of the tensor, and the last ends inside it."""
+    import torch
+
+    from dotllm_b200 import serving
+    B, V = 5, 12
+    flat = torch.rand(B * 4 * (V + 3))
+
+    def views(n):
+        yield flat[:B * n * V].view(B, n, V)                                     # dense
+        yield flat.view(B, 4, V + 3)[:, :n, :V] if n in (1, 4) else flat[:B * n * (V + 3)].view(B, n, V + 3)[..., :V]  # wide rows
+        yield flat.view(B, 4, V + 3)[:, :n, 1:V + 1]                             # some of each sequence's rows
+        yield flat[:V].expand(B, n, V)                                           # one row for all
+        yield flat[-V:].expand(B, n + 1, V)[:, :n]                               # the same, every stride between rows 0
+        yield flat[:B * V].view(B, 1, V).expand(B, n, V)                         # one row per sequence
+        yield flat[:n * V].view(1, n, V).expand(B, n, V)                         # the same rows for all sequences
+        yield flat[:B * n * V].view(n, B, V).transpose(0, 1)
+
+    for k in (0, 1, 3):
+        draft, u = OnDevice(torch.zeros(B, k, dtype=torch.int32)), OnDevice(torch.rand(B, k + 1))
+        for p in views(k + 1):
+            for q in [None] if k == 0 else [None, *views(k)]:
+                launches.clear()
+                try:
+                    serving.verify_draft(OnDevice(p), None if q is None else OnDevice(q), draft, u)
+                except ValueError:
+                    continue
+                a = launches[0][0]
+                for t, start, ld, n in [(p, a.p, a.ld_p, k + 1)] + ([] if q is None else [(q, a.q, a.ld_q, k)]):
+                    assert rows_end(start, B * n, ld, V) <= t.untyped_storage().data_ptr() + t.untyped_storage().nbytes(), (t.shape, t.stride())
+                    for b in range(B):
+                        for i in range(n):
+                            assert start + 4 * (b * n + i) * ld == t[b, i].data_ptr(), (t.shape, t.stride())
+
+
+def test_verify_takes_evenly_strided_rows_and_refuses_shared_ones(launches):
+    import torch
+
+    from dotllm_b200 import serving
+    B, V = 5, 12
+
+    def call(p, q):
+        k = p.shape[1] - 1
+        serving.verify_draft(OnDevice(p), None if q is None else OnDevice(q), OnDevice(torch.zeros(B, k, dtype=torch.int32)),
+                             OnDevice(torch.rand(B, k + 1)))
+
+    call(torch.rand(B, 4, V)[:, :1], None)   # one row of several
+    call(torch.rand(B, 4, V)[:, -1:], None)
+    call(torch.rand(B, 2, V), torch.rand(B, 3, V)[:, 1:2])
+    call(torch.rand(B, 2, V + 4)[..., :V], torch.rand(B, V).unsqueeze(1))
+    for p, q in [(torch.rand(V).expand(B, 1, V), None), (torch.rand(V).expand(B, 2, V)[:, :1], None),
+                 (torch.rand(B, 2, V), torch.rand(V).expand(B, 2, V)[:, 1:]), (torch.rand(B, 2, V), torch.rand(V).expand(B, 1, V)),
+                 (torch.rand(B, 2, V), torch.rand(1, 1, V).expand(B, 1, V)), (torch.rand(1, 2, V).expand(B, 2, V), None),
+                 (torch.rand(B, 4, V)[:, :2], None)]:
+        with pytest.raises(ValueError):
+            call(p, q)
