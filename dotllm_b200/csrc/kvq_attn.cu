@@ -660,14 +660,22 @@ bool wide_pays(const llmdot_kvq_pool &p, int64_t rows, int64_t items, bool own)
     return rows >= 48 || (items <= 2048 && rows >= (own || p.head_dim == 256 ? 17 : 25));
 }
 
+// Product of counts, at most 2^60: batch, max_pages and heads may each be large without any being too large.
+int64_t times(int64_t a, int64_t b)
+{
+    const int64_t most = (int64_t)1 << 60;
+    return b > 0 && a > most / b ? most : std::min(a * b, most);
+}
+
 Plan make_plan(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const llmdot_kvq_attn &a)
 {
     Plan x = {};
-    const int64_t G = a.heads / p.heads_kv, Hk = p.heads_kv, own_rows = (int64_t)b.max_rows * G, all_rows = (int64_t)b.rows * G;
+    // max_rows is a bound: no sequence has more rows than the call
+    const int64_t G = a.heads / p.heads_kv, Hk = p.heads_kv, own_rows = std::min(b.max_rows, b.rows) * G, all_rows = (int64_t)b.rows * G;
     const int64_t npp = (a.prefix_len + KVQ_PAGE - 1) / KVQ_PAGE, wide = kvq_wide_rows(p.head_dim);
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
     x.wide_p = a.type != T_F32 && npp > 0 && wide_pays(p, all_rows, Hk * npp, false);
-    x.wide_s = a.type != T_F32 && wide_pays(p, own_rows, Hk * b.batch * b.max_pages, true);
+    x.wide_s = a.type != T_F32 && wide_pays(p, own_rows, times(Hk * b.batch, b.max_pages), true);
     x.nt_p = tiles_of(p.head_dim, all_rows);
     x.nt_s = tiles_of(p.head_dim, own_rows);
     if (npp == 0) x.nt_p = x.nt_s;
@@ -690,13 +698,13 @@ Plan make_plan(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const llmdot
     };
     auto wide_ch = [&](int64_t ctas, int64_t pages) { return std::max<int64_t>(2, up(pages, std::max<int64_t>(1, 148 / std::max<int64_t>(1, ctas)))); };
     x.ch_p = bounded(x.wide_p ? wide_ch(Hk * x.ptiles, npp) : chunk(Hk * x.ptiles * npp, places(x.nt_p), 1), npp);
-    x.ch_s = bounded(x.wide_s ? wide_ch(Hk * x.rtiles * b.batch, b.max_pages)
-                              : chunk(Hk * b.batch * x.rtiles * b.max_pages, 2 * places(x.nt_s), 2), b.max_pages);
+    x.ch_s = bounded(x.wide_s ? wide_ch(times(Hk * x.rtiles, b.batch), b.max_pages)
+                              : chunk(times(times(Hk * x.rtiles, b.batch), b.max_pages), 2 * places(x.nt_s), 2), b.max_pages);
     x.nsp = (int)up(npp, x.ch_p);
     x.nss = (int)std::max<int64_t>(1, up(b.max_pages, x.ch_s));
     x.direct = x.nsp == 0 && x.nss == 1 && !x.wide_s;
     x.ctas_p = Hk * x.ptiles * x.nsp;
-    x.ctas_s = Hk * x.rtiles * x.nss * b.batch;
+    x.ctas_s = times(times(Hk * x.rtiles, x.nss), b.batch);
     if (!x.direct) {
         const size_t rh = (size_t)b.rows * a.heads * (x.nsp + x.nss);
         x.o_bytes = rh * p.head_dim * 4;

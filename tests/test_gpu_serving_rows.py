@@ -30,3 +30,22 @@ def test_verify_refuses_one_row_for_all_sequences(gpu):
         with pytest.raises(ValueError):
             serving.verify_draft(p, q, draft, u)
         serving.verify_draft(p, q.contiguous(), draft, u)
+
+
+@pytest.mark.parametrize("typ", ["float32", "bfloat16"])
+@pytest.mark.parametrize("heads", [4, 48])
+def test_a_loose_max_rows_gives_the_same_bits(gpu, typ, heads):
+    import torch
+    from dotllm_b200 import serving
+    g = torch.Generator("cuda").manual_seed(5)
+    pool = serving.KvqPool.empty(8, 2, 64)
+    pages = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4)
+    lens = torch.tensor([200, 130], dtype=torch.int32, device="cuda")
+    all_rows = torch.tensor([0, 200, 330], dtype=torch.int32, device="cuda")
+    serving.kvq_write(pool, serving.KvqBatch(all_rows, lens, pages, 200),
+                      *(torch.randn(330, 2, 64, device="cuda", generator=g) for _ in range(2)))
+    row_start = torch.tensor([0, 3, 5], dtype=torch.int32, device="cuda")
+    q = torch.randn(5, heads, 64, device="cuda", generator=g).to(getattr(torch, typ))
+    want = serving.kvq_attention(pool, serving.KvqBatch(row_start, lens, pages, 5), q)
+    for loose in (6, 1000, 2 ** 31 - 1):
+        assert torch.equal(serving.kvq_attention(pool, serving.KvqBatch(row_start, lens, pages, loose), q), want)

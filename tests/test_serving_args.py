@@ -224,3 +224,31 @@ def test_verify_takes_evenly_strided_rows_and_refuses_shared_ones(launches):
                  (torch.rand(B, 4, V)[:, :2], None)]:
         with pytest.raises(ValueError):
             call(p, q)
+
+
+def workspace(batch_kw, attn_kw, pool_kw=()):
+    need = C.c_size_t()
+    status = native.lib().llmdot_cuda_kvq_attention_workspace(pool(**dict(pool_kw)), batch(**batch_kw), attn(**attn_kw), need)
+    return status, need.value
+
+
+def test_a_loose_max_rows_changes_nothing():
+    """max_rows is a bound: no sequence has more rows than the call, so one above that is the same bound."""
+    for heads, hk, typ in ((32, 8, 25), (8, 1, 0), (65536, 1, 0), (4, 4, 1)):
+        for rows, prefix in ((4, 0), (3, 500), (64, 70)):
+            kw = dict(rows=rows, max_pages=300)
+            a = dict(heads=heads, type=typ, prefix_len=prefix, prefix_pages=P)
+            tight = workspace(dict(kw, max_rows=rows), a, dict(heads_kv=hk))
+            assert tight[0] == 0 and tight[1] > 0
+            for loose in (rows + 1, 1000, 1 << 20, 2 ** 31 - 1):
+                assert workspace(dict(kw, max_rows=loose), a, dict(heads_kv=hk)) == tight, (heads, rows, loose)
+
+
+def test_too_many_blocks_are_refused():
+    """The largest counts that the checks let through, together: more blocks than a launch has, refused before one."""
+    L = native.lib()
+    p, a = pool(heads_kv=4096, n_pages=1), attn(heads=4096, type=0)
+    for n, m in ((2 ** 31 - 1, 1 << 24), (1 << 30, 1 << 18), (1 << 20, 1 << 24)):
+        b = batch(batch=n, rows=2, max_rows=2 ** 31 - 1, max_pages=m)
+        assert L.llmdot_cuda_kvq_attention(p, b, a, P, 4096 * 64, P, 4096 * 64, None, P, 1 << 60, None) == INVALID, (n, m)
+        assert "too many" in message()
