@@ -667,6 +667,8 @@ int64_t times(int64_t a, int64_t b)
     return b > 0 && a > most / b ? most : std::min(a * b, most);
 }
 
+constexpr int64_t PART_BYTES = 128 << 20;  // of the prefix's partials, and of the own pages'
+
 Plan make_plan(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const llmdot_kvq_attn &a)
 {
     Plan x = {};
@@ -683,8 +685,12 @@ Plan make_plan(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const llmdot
     x.rtiles = (int)std::max<int64_t>(1, up(own_rows, x.wide_s ? wide : 8 * x.nt_s));
     // Chunks.  Narrow: about one CTA per place on the SMs for the prefix, two for the sequences' own pages
     // (max_pages is a bound: ragged sequences leave some without work), at most 32 pages, so that long
-    // and short sequences balance.  Wide: one CTA per SM, at least two pages.  At most 256 chunks of either, which
-    // bounds the workspace and what the join reads, and even ones.
+    // and short sequences balance.  Wide: one CTA per SM, at least two pages.  At most 256 chunks of either, even ones,
+    // and no more than PART_BYTES of partials unless one chunk takes them: with rows enough for that a chunk has
+    // CTAs enough for all SMs, and the partials of a table much longer than the sequences, or of a long prompt
+    // chunk of fp32 rows (2 GB with 2048 rows of 32 heads and 2048 pages), stay in L2.
+    const int64_t part = std::max<int64_t>(1, (int64_t)b.rows * a.heads * (p.head_dim * 4 + 8));  // bytes of one chunk's
+    const int64_t most = std::min<int64_t>(256, std::max<int64_t>(1, PART_BYTES / part));
     auto places = [&](int nt) {  // CTAs on the SMs: shared memory and registers (as built) of an instance
         const int d = p.head_dim, nq = a.type == T_F32 ? 2 : 1, np = a.type == T_BF16 ? 1 : 2;
         const int bytes = 4 * 64 * d + 1024 + nt * 8 * (nq * (d + 8) + np * 160) * 2 + 2048;
@@ -693,7 +699,7 @@ Plan make_plan(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const llmdot
     };
     auto chunk = [&](int64_t pages, int64_t ctas, int64_t least) { return std::min<int64_t>(32, std::max<int64_t>(least, up(pages, ctas))); };
     auto bounded = [&](int64_t ch, int64_t pages) {
-        ch = std::max(ch, up(pages, 256));
+        ch = std::max(ch, up(pages, most));
         return (int)std::max<int64_t>(1, up(pages, std::max<int64_t>(1, up(pages, ch))));
     };
     auto wide_ch = [&](int64_t ctas, int64_t pages) { return std::max<int64_t>(2, up(pages, std::max<int64_t>(1, 148 / std::max<int64_t>(1, ctas)))); };

@@ -252,3 +252,18 @@ def test_too_many_blocks_are_refused():
         b = batch(batch=n, rows=2, max_rows=2 ** 31 - 1, max_pages=m)
         assert L.llmdot_cuda_kvq_attention(p, b, a, P, 4096 * 64, P, 4096 * 64, None, P, 1 << 60, None) == INVALID, (n, m)
         assert "too many" in message()
+
+
+@pytest.mark.parametrize("typ", [0, 1, 25])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("prefix", [0, 5000, 500000])
+def test_scratch_is_bounded(typ, dim, prefix):
+    """Prefix and own pages leave at most 128 MB of partial results each, or those of one chunk where a call has so many
+    rows that one takes more, whatever the table's length and the types."""
+    for heads, hk in ((32, 8), (32, 32), (8, 1)):
+        for n, rows in ((1, 1), (1, 200), (1, 2048), (1, 8192), (96, 480), (64, 64)):
+            for pages in (1, 32, 256, 2048, 1 << 16):
+                chunk = rows * heads * (4 * dim + 8)
+                status, size = workspace(dict(batch=n, rows=rows, max_rows=-(-rows // n), max_pages=pages),
+                                         dict(heads=heads, type=typ, prefix_len=prefix, prefix_pages=P), dict(heads_kv=hk, head_dim=dim))
+                assert status == 0 and size <= 2 * max(chunk, 128 << 20), (heads, hk, rows, pages, size)
