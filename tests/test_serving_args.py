@@ -239,7 +239,7 @@ def test_a_loose_max_rows_changes_nothing():
             kw = dict(rows=rows, max_pages=300)
             a = dict(heads=heads, type=typ, prefix_len=prefix, prefix_pages=P)
             tight = workspace(dict(kw, max_rows=rows), a, dict(heads_kv=hk))
-            assert tight[0] == 0 and tight[1] > 0
+            assert tight[0] == 0
             for loose in (rows + 1, 1000, 1 << 20, 2 ** 31 - 1):
                 assert workspace(dict(kw, max_rows=loose), a, dict(heads_kv=hk)) == tight, (heads, rows, loose)
 
