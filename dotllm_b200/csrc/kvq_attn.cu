@@ -79,6 +79,16 @@ template <int D> struct Shape {
     static constexpr int OFF_SC = 4 * SLOT, OFF_Q = OFF_SC + 4 * KVQ_PAGE * 4;  // K 0, K 1, V 0, V 1, scales, queries, weights
 };
 constexpr int PS = 80;  // halves from one row's weights to the next (64 and 16 against bank conflicts)
+// An instance's resources, for its launch, its compilation and the plan alike.  CTAs per SM that its registers are
+// limited to leave room for: what its accumulators and query fragments take with few spills.
+constexpr int narrow_regs_ctas(int d, int nt) { return d == 256 ? (nt <= 2 ? 3 : 2) : nt == 1 ? 5 : nt <= 3 ? 4 : 2; }
+// Bytes of dynamic shared memory with nq terms per query and np per weight; 48 bytes per row and 1 KB of the system's beside it.
+constexpr int narrow_smem(int d, int nt, int nq, int np) { return 4 * KVQ_PAGE * d + 1024 + nt * 8 * (nq * (d + (d == 96 ? 0 : 8)) + np * 2 * PS) * 2; }
+constexpr int narrow_ctas(int d, int nt, int nq, int np)
+{
+    const int room = 228 * 1024 / (narrow_smem(d, nt, nq, np) + nt * 8 * 48 + 1024), regs = narrow_regs_ctas(d, nt);
+    return room < 1 ? 1 : room < regs ? room : regs;
+}
 // Where 16-byte piece c of position r lies in its slot: chosen so that the lanes of one shared-memory
 // access (K: 8 or 16 lanes on positions a, a + 4, ...; V: on positions 4 i .. 4 i + 3) meet distinct banks.
 template <int D> __device__ __forceinline__ int k_piece(int r, int c)
@@ -131,7 +141,7 @@ __device__ __forceinline__ void store4(void *p, int64_t i, uint32_t type, bool w
 
 // PREC 0 (bf16): one fp16 for query and weight; 1 (fp16): hi + lo weights; 2 (fp32): hi + lo queries too.
 template <int D, int FMT, int NT, int PREC>
-__global__ void __launch_bounds__(NW * 32, D == 256 ? 1 : NT == 1 ? 5 : NT <= 3 ? 4 : 1) kvq_attn_kernel(const __grid_constant__ AttnArgs a)
+__global__ void __launch_bounds__(NW * 32, narrow_regs_ctas(D, NT)) kvq_attn_kernel(const __grid_constant__ AttnArgs a)
 {
     using Sh = Shape<D>;
     constexpr int RT = 8 * NT, QS = D + Sh::QPAD, NQ = PREC == 2 ? 2 : 1, NP = PREC > 0 ? 2 : 1;
@@ -579,7 +589,8 @@ template <int D, int W> __global__ void __launch_bounds__(128) kvq_join_kernel(c
 template <int D, int FMT, int NT, int PREC> cudaError_t launch_tiles(const AttnArgs &a, int64_t grid, cudaStream_t st)
 {
     using Sh = Shape<D>;
-    constexpr int NQ = PREC == 2 ? 2 : 1, NP = PREC > 0 ? 2 : 1, smem = Sh::OFF_Q + NT * 8 * (NQ * (D + Sh::QPAD) + NP * 2 * PS) * 2;
+    constexpr int NQ = PREC == 2 ? 2 : 1, NP = PREC > 0 ? 2 : 1, smem = narrow_smem(D, NT, NQ, NP);
+    static_assert(smem == Sh::OFF_Q + NT * 8 * (NQ * (D + Sh::QPAD) + NP * 2 * PS) * 2, "the kernel's layout");
     static_assert(smem - Sh::OFF_Q >= (2 * SEQ_TABLE + 1) * 4, "the sequences' tables fit into the queries' and weights' memory");
     static_assert(D != 64 || 4 * Sh::SLOT >= 2 * NT * 2 * 512, "two warps' outputs fit into the slots");
     static std::atomic<unsigned long long> done{0};
@@ -691,11 +702,8 @@ Plan make_plan(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const llmdot
     // chunk of fp32 rows (2 GB with 2048 rows of 32 heads and 2048 pages), stay in L2.
     const int64_t part = std::max<int64_t>(1, (int64_t)b.rows * a.heads * (p.head_dim * 4 + 8));  // bytes of one chunk's
     const int64_t most = std::min<int64_t>(256, std::max<int64_t>(1, PART_BYTES / part));
-    auto places = [&](int nt) {  // CTAs on the SMs: shared memory and registers (as built) of an instance
-        const int d = p.head_dim, nq = a.type == T_F32 ? 2 : 1, np = a.type == T_BF16 ? 1 : 2;
-        const int bytes = 4 * 64 * d + 1024 + nt * 8 * (nq * (d + 8) + np * 160) * 2 + 2048;
-        const int regs = d == 256 ? (nt <= 2 ? 4 : nt == 3 ? 3 : 2) : nt == 1 ? 5 : nt <= 3 ? 4 : nt == 4 ? 3 : 2;
-        return 148 * (int64_t)std::max(1, std::min(regs, 227 * 1024 / bytes));
+    auto places = [&](int nt) {  // CTAs on the SMs
+        return (int64_t)148 * narrow_ctas(p.head_dim, nt, a.type == T_F32 ? 2 : 1, a.type == T_BF16 ? 1 : 2);
     };
     auto chunk = [&](int64_t pages, int64_t ctas, int64_t least) { return std::min<int64_t>(32, std::max<int64_t>(least, up(pages, ctas))); };
     auto bounded = [&](int64_t ch, int64_t pages) {
