@@ -267,3 +267,32 @@ def test_scratch_is_bounded(typ, dim, prefix):
                 status, size = workspace(dict(batch=n, rows=rows, max_rows=-(-rows // n), max_pages=pages),
                                          dict(heads=heads, type=typ, prefix_len=prefix, prefix_pages=P), dict(heads_kv=hk, head_dim=dim))
                 assert status == 0 and size <= 2 * max(chunk, 128 << 20), (heads, hk, rows, pages, size)
+
+
+def test_counts_beyond_32_bits_are_not_cut(monkeypatch):
+    """The library's counts are 32-bit: a larger one reaches it as the largest, never as what its low bits happen to be."""
+    import torch
+
+    from dotllm_b200 import serving
+    made = []
+    monkeypatch.setattr(serving, "_call", lambda fn, device, *args: made.append(args))
+    codes = OnDevice(torch.zeros(2, 2, 64, 64, dtype=torch.int8))
+    scales = OnDevice(torch.zeros(2, 2, 64))
+    p = serving.KvqPool(codes, codes, scales, scales)
+
+    def ints(*shape):
+        return OnDevice(torch.zeros(*shape, dtype=torch.int32))
+
+    q = OnDevice(torch.zeros(3, 4, 64))
+    for big in (2 ** 31, 2 ** 32, 2 ** 32 + 10, 2 ** 40 + 1):
+        b = serving.KvqBatch(ints(2), ints(1), ints(1, 2), big)
+        serving.kvq_attention(p, b, q, window=big)
+        assert made[-1][1].max_rows == 2 ** 31 - 1 and made[-1][2].window == 2 ** 31 - 1
+        b = serving.KvqBatch(ints(2), ints(1), ints(1, 2), 3)
+        for kw in (dict(window=-big), dict(prefix_len=-big)):
+            with pytest.raises(native.CudaBackendError):
+                serving.kvq_attention(p, b, q, **kw)
+    wide = OnDevice(torch.zeros(1).expand(1, 1, 2 ** 32 + 5))  # (refused by its stride otherwise)
+    monkeypatch.setattr(OnDevice, "stride", lambda self: (2 ** 32 + 5, 2 ** 32 + 5, 1) if self is wide else self.t.stride())
+    serving.verify_draft(wide, None, ints(1, 0), OnDevice(torch.zeros(1, 1)))
+    assert made[-1][0].vocab == 2 ** 31 - 1
