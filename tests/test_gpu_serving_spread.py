@@ -283,3 +283,68 @@ def test_negative_scales(gpu, typ, group):
             held[[j for j in range(held.shape[0]) if j % PAGE % 3 == 1]] *= -1.0
     q = queries(9, typ, 3, 2 * group, 128)
     c.check(q, typ, c.attend(q))
+
+
+# 3 rows a sequence: 6, 18 and 60 per kv head on own pages, twice that on the prefix -- either side of where the kernels change
+GROUPS = [2, 6, 20]
+DIMS = [(64, "e4m3"), (96, "i8"), (128, "e4m3"), (256, "i8")]
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("dim,fmt", DIMS)
+@pytest.mark.parametrize("group", GROUPS)
+def test_pages_outside_the_pool(gpu, typ, dim, fmt, group):
+    """Ids outside the pool, in a sequence's list or the prefix's, first, in the middle and last: never followed, not seen."""
+    c = Held(fmt, random_parts(17, 2, dim, 300, 330, 200), [3, 3])
+    q = queries(10, typ, 6, 2 * group, dim)
+    for bad in (-1, c.pool.n_pages, 2 ** 31 - 1):
+        for own, pre in ((1, None), (None, 2), (0, 0), (5, 4), (None, 0)):
+            table, prefix_pages = c.table.clone(), c.prefix_pages.clone()
+            gone = []
+            if pre is not None:
+                prefix_pages[pre] = bad
+                gone += list(range(64 * pre, min(300, 64 * pre + 64)))
+            if own is not None:
+                table[0, own] = bad
+            mine = [] if own is None else list(range(300 + 64 * own, 300 + min(330, 64 * own + 64)))
+            got = c.attend(q, table=table, prefix_pages=prefix_pages)
+            c.check(q, typ, got, hidden=lambda b: gone + (mine if b == 0 else []))
+    table[:], prefix_pages[:] = -1, -1  # nothing at all
+    out, lse = c.attend(q, table=table, prefix_pages=prefix_pages)
+    assert bool((out == 0).all()) and bool((lse == float("-inf")).all())
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("dim,fmt", DIMS)
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+def test_nan_scales_reach_the_rows_that_see_them(gpu, typ, dim, fmt, group, softcap):
+    """A NaN scale of K or V makes the rows NaN that see it, of its kv head; the others are what they are without it.  At the
+    last drafted position, one before, and in the prefix where the window shows it to the first row alone."""
+    import torch
+    for which in ("k_scale", "v_scale"):
+        for at, seen, window in ((329, (2,), 0), (328, (1, 2), 0), (-40, (0,), 368)):
+            c = Held(fmt, random_parts(18, 2, dim, 300, 330, 200), [3, 3])
+            q = queries(11, typ, 6, 2 * group, dim)
+            pages, j = (c.lists[1], at) if at >= 0 else (c.lists[0], 300 + at)
+            getattr(c.pool, which)[int(pages[j // PAGE]), 1, j % PAGE] = float("nan")
+            held = c.values[0 if which == "k_scale" else 1][1 if at >= 0 else 0]
+            held[j, 1] = float("nan")
+            if at < 0:  # (both sequences have the prefix: the second's rows see it in the window, too)
+                seen_by = {0: seen, 1: (0, 1, 2)}
+            else:
+                seen_by = {0: seen, 1: ()}
+            out, lse = c.attend(q, window=window, softcap=softcap)
+            clear = torch.ones(6, dtype=torch.bool)
+            for b in (0, 1):
+                for i in seen_by[b]:
+                    clear[3 * b + i] = False
+                    assert bool(torch.isnan(out[3 * b + i, group:]).all())
+            held[j, 1] = 0.0
+            assert bool(torch.isfinite(out[:, :group]).all()) and bool(torch.isfinite(out[clear.cuda()]).all())
+            if at >= 0:
+                c.check(q, typ, (out, lse), window=window, softcap=softcap, only=[i for i in range(3) if i not in seen])
+            else:
+                c.rows, keep = [3], c.rows
+                c.check(q[:3], typ, (out[:3], lse[:3]), window=window, softcap=softcap, only=(1, 2))
+                c.rows = keep
