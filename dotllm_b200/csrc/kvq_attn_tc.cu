@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
 #pragma unroll
                     for (int r = 0; r < 2; r++) {
                         const int k = 2 * h + r;
-                        float x = __uint_as_float(s[4 * c + 2 * r]) * kf.x * fq[k], y = __uint_as_float(s[4 * c + 2 * r + 1]) * kf.y * fq[k];
+                        float x = __uint_as_float(s[4 * c + 2 * r]) * (kf.x * fq[k]), y = __uint_as_float(s[4 * c + 2 * r + 1]) * (kf.y * fq[k]);
                         if (cap) {
                             x = capped<false>(x, a.at.softcap, inv_cap2) * 1.4426950408889634f;
                             y = capped<false>(y, a.at.softcap, inv_cap2) * 1.4426950408889634f;
@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 1) kvq_wide_kernel(const __g
                     for (int r = 0; r < 2; r++) {
                         const int k = 2 * h + r, j = j0 + 8 * c;
                         const float off = ref[k] == -INFINITY ? 0.0f : ref[k];
-                        float x = __uint_as_float(s[4 * c + 2 * r]) * kf.x * fq[k], y = __uint_as_float(s[4 * c + 2 * r + 1]) * kf.y * fq[k];
+                        float x = __uint_as_float(s[4 * c + 2 * r]) * (kf.x * fq[k]), y = __uint_as_float(s[4 * c + 2 * r + 1]) * (kf.y * fq[k]);
                         if (cap) {
                             x = capped<false>(x, a.at.softcap, inv_cap2) * 1.4426950408889634f;
                             y = capped<false>(y, a.at.softcap, inv_cap2) * 1.4426950408889634f;

@@ -348,3 +348,18 @@ def test_nan_scales_reach_the_rows_that_see_them(gpu, typ, dim, fmt, group, soft
                 c.rows, keep = [3], c.rows
                 c.check(q[:3], typ, (out[:3], lse[:3]), window=window, softcap=softcap, only=(1, 2))
                 c.rows = keep
+
+
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("dim,fmt", DIMS)
+@pytest.mark.parametrize("group", [2, 20])
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+def test_key_scales_of_every_size(gpu, typ, dim, fmt, group, softcap):
+    """Keys tiny or huge and queries the inverse: the scores are ordinary, whatever the order of their factors."""
+    for k in (-90, 110):
+        parts = random_parts(k + 200, 2, dim, 130, 70)
+        for key, _ in parts:
+            key *= 2.0 ** k
+        c = Held(fmt, parts, [3])
+        q = queries(12, typ, 3, 2 * group, dim, scale=2.0 ** -k)
+        c.check(q, typ, c.attend(q, softcap=softcap), softcap=softcap)
