@@ -363,3 +363,16 @@ def test_key_scales_of_every_size(gpu, typ, dim, fmt, group, softcap):
         c = Held(fmt, parts, [3])
         q = queries(12, typ, 3, 2 * group, dim, scale=2.0 ** -k)
         c.check(q, typ, c.attend(q, softcap=softcap), softcap=softcap)
+
+
+@pytest.mark.parametrize("dim,fmt", DIMS)
+@pytest.mark.parametrize("group", [2, 20])
+def test_subnormal_fp16_queries(gpu, dim, fmt, group):
+    """fp16 queries below the smallest normal number, over keys that make ordinary scores of them."""
+    parts = random_parts(19, 2, dim, 130, 70)
+    for key, _ in parts:
+        key *= 2.0 ** 17
+    c = Held(fmt, parts, [3])
+    q = queries(13, "f16", 3, 2 * group, dim, scale=2.0 ** -17)
+    c.check(q, "f16", c.attend(q))
+    c.check(q, "f16", c.attend(q, window=90), window=90)
