@@ -59,7 +59,7 @@ template <int N> __device__ __forceinline__ void kvq_find(const llmdot_kvq_pool 
     const int r = row0 + threadIdx.x;
     if (threadIdx.x < N && r < bt.rows) {
         const int b = kvq_seq_of(bt.row_start, bt.batch, r);
-        place[threadIdx.x] = b < 0 ? -2 : kvq_place(pool, bt, b, bt.seq_len[b] - bt.row_start[b + 1] + r, 0);
+        place[threadIdx.x] = b < 0 ? -2 : kvq_place(pool, bt, b, bt.seq_len[b] - bt.row_start[b + 1] + r);
     }
 }
 

@@ -38,39 +38,22 @@ __device__ __forceinline__ int kvq_seq_of(const int32_t *__restrict__ row_start,
     return lo < batch && row_start[lo] <= r ? lo : -1;
 }
 
-// Index of (page, kv head, slot) of sequence b's position pos in units of one head's row, or -1.
-__device__ __forceinline__ int64_t kvq_place(const llmdot_kvq_pool &pool, const llmdot_kvq_batch &bt, int b, int pos, int head)
+// Index of (page, kv head 0, slot) of sequence b's position pos in units of one head's row, or -1.
+__device__ __forceinline__ int64_t kvq_place(const llmdot_kvq_pool &pool, const llmdot_kvq_batch &bt, int b, int pos)
 {
     const int pi = pos / KVQ_PAGE;
     if (pos < 0 || pi >= bt.max_pages) return -1;
     const int page = bt.pages[(int64_t)b * bt.max_pages + pi];
     if ((unsigned)page >= (unsigned)pool.n_pages) return -1;
-    return ((int64_t)page * pool.heads_kv + head) * KVQ_PAGE + pos % KVQ_PAGE;
+    return (int64_t)page * pool.heads_kv * KVQ_PAGE + pos % KVQ_PAGE;
 }
 
-template <typename T> __device__ __forceinline__ float to_f32(T x);
-template <> __device__ __forceinline__ float to_f32<float>(float x) { return x; }
-template <> __device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
-template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <typename T> __device__ __forceinline__ T from_f32(float x);
 template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
 template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
 // Eight consecutive values; `wide`: the address is a multiple of 16 bytes.
-template <typename T> __device__ __forceinline__ void load8(const T *__restrict__ p, bool wide, float (&x)[8])
-{
-    if (wide) {
-        __align__(16) T t[8];
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; i++) ((uint4 *)t)[i] = __ldg((const uint4 *)p + i);
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = to_f32<T>(t[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = to_f32<T>(p[i]);
-    }
-}
 template <typename T> __device__ __forceinline__ void store8(T *__restrict__ p, bool wide, const float (&x)[8])
 {
     __align__(16) T t[8];

@@ -107,7 +107,6 @@ template <int D> __device__ __forceinline__ int v_piece(int r, int c)
 __device__ __forceinline__ int row_position(int r) { return ((r & 7) >> 1) + 4 * (r & 1) + (r & 8); }
 
 template <int N> struct Bytes;
-template <> struct Bytes<4> { using T = uint32_t; };
 template <> struct Bytes<8> { using T = uint2; };
 template <> struct Bytes<16> { using T = uint4; };
 template <int N> __device__ __forceinline__ void lds(const uint8_t *p, uint32_t (&w)[N / 4])
