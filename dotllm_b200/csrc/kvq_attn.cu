@@ -74,7 +74,6 @@ template <int D> struct Shape {
     static constexpr int SLOT = KVQ_PAGE * D;                  // bytes of a page's K or V
     static constexpr int KB = D == 96 ? 8 : 16, KC = D / (4 * KB);  // K bytes a lane takes at once; such pieces
     static constexpr int GPW = D == 256 ? 2 : 1;               // 32-dimension groups of O per warp (64: two warps share one, 96: three have one)
-    static constexpr int MAX_NT = D == 256 ? 4 : 8;
     static constexpr int QPAD = D == 96 ? 0 : 8;               // halves between query rows against bank conflicts
     static constexpr int OFF_SC = 4 * SLOT, OFF_Q = OFF_SC + 4 * KVQ_PAGE * 4;  // K 0, K 1, V 0, V 1, scales, queries, weights
 };
@@ -603,8 +602,9 @@ template <int D, int FMT, int PREC> cudaError_t launch_nt(int nt, const AttnArgs
     case 1: return launch_tiles<D, FMT, 1, PREC>(a, grid, st);
     case 2: return launch_tiles<D, FMT, 2, PREC>(a, grid, st);
     case 3: return launch_tiles<D, FMT, 3, PREC>(a, grid, st);
-    case 4: return launch_tiles<D, FMT, 4, PREC>(a, grid, st);
-    default: return launch_tiles<D, FMT, Shape<D>::MAX_NT, PREC>(a, grid, st);
+    case 8:
+        if constexpr (PREC == 2 && D != 256) return launch_tiles<D, FMT, 8, PREC>(a, grid, st);  // others: 32 rows at most (wide_pays)
+    default: return launch_tiles<D, FMT, 4, PREC>(a, grid, st);
     }
 }
 template <int D, int FMT> cudaError_t launch_prec(int nt, const AttnArgs &a, int64_t grid, cudaStream_t st)
@@ -653,21 +653,23 @@ struct Plan {
     int64_t ctas_p, ctas_s;
     size_t o_bytes, ml_bytes;
 };
-int tiles_of(int dim, int64_t rows)  // 8-row tiles per CTA: 1, 2, 3, 4 or 8 (4 with head_dim 256)
+int tiles_of(int dim, int64_t rows)  // 8-row tiles per CTA: 1, 2, 3, 4 or (fp32 queries) 8, 4 with head_dim 256
 {
     const int64_t n = std::max<int64_t>(1, (rows + 7) / 8);
     return (int)(n <= 4 ? n : dim == 256 ? 4 : 8);
 }
 // Whether `rows` rows (times heads) per kv head over `items` pages and heads in all go to the wide kernel.  It takes
-// the same time for 1 to 256 rows, the narrow one grows with every 8.  With work enough for all SMs the wide one
-// pays from 48 rows: 24 sequences of 1500 own positions, 8 heads of 128, bf16, in us, wide / narrow: 80.2 / 65.6 with
-// 24 rows, 81.8 / 97.0 with 40; 96 of 1000, fp16, heads of 64: 180 / 154 with 40.  With few items the latency of one
-// CTA's chunk counts, and it pays from 17 rows on own pages (4 of 3000: 26.8 / 39.0 with 20; 1 of 300: 16.4 / 18.5)
-// and with head_dim 256 (prefix of 2000, 24 rows: 22.6 / 30.8), from 25 on another prefix (of 2000: 26.8 / 24.7 with
-// 24, 26.8 / 32.4 with 32; of 12000: 36.0 / 51.6 with 32).
+// the same time for 1 to 256 rows, the narrow one grows with every 8 up to 32 rows and then takes 64.  Some thousand
+// positions, 8 kv heads (or as said), bf16, heads of 64 / 96 / 128 / 256, us, wide : narrow.
+//   Work enough for all SMs, so that only throughput counts, own pages of 24 sequences, 4608 items: 32 rows 62 : 46 / 68 : 64 /
+//   72 : 72 / 128 : 115, 40 rows 62 : 68 / 68 : 92 / 72 : 103 / 128 : 161; 96 sequences, fp16, heads of 64: 40 rows 165 : 160.
+//   2048 items or fewer, where the latency of one CTA's chunk counts.  Own pages, 2048 items: 16 rows 28 : 27 / 31 : 33 / 31 : 35 /
+//   52 : 54, 20 rows 29 : 35 / 31 : 39 / 32 : 42 / 52 : 66; 188 items, 20 rows 19 : 18 / 21 : 21 / 21 : 21 / 24 : 27.
+//   A prefix, 2048 items: 24 rows 29 : 30 / 34 : 37 / 34 : 37 / 58 : 56, with 32 kv heads 33 : 27 / 38 : 33 / 39 : 35 / 62 : 73, and with
+//   32 rows 33 : 39 / 39 : 46 / 39 : 51 / 64 : 86; 256 items, 20 rows of 256 27 : 35.  3000 items: 24 rows 37 : 33 / 43 : 41 / 44 : 43 / 79 : 64.
 bool wide_pays(const llmdot_kvq_pool &p, int64_t rows, int64_t items, bool own)
 {
-    return rows >= 48 || (items <= 2048 && rows >= (own || p.head_dim == 256 ? 17 : 25));
+    return rows >= 33 || (items <= 2048 && rows >= (own || p.head_dim == 256 ? 17 : 25));
 }
 
 // Product of counts, at most 2^60: batch, max_pages and heads may each be large without any being too large.
