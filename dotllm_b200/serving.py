@@ -29,7 +29,8 @@ def _bad(text: str):
 
 
 def _count(n: int) -> int:
-    """n for a 32-bit count of the library, which refuses (or bounds) what does not fit; ctypes would keep its low bits."""
+    """n for a 32-bit count of the library, which refuses (or bounds) what does not fit; ctypes would keep its low bits.
+    (Rows, heads and pages of tensors that fit a device stay below.)"""
     return max(-(1 << 31), min(n, (1 << 31) - 1))
 
 
@@ -60,7 +61,7 @@ class KvqPool:
         if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
             _bad("KvqPool: tensors must be contiguous")
         self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, device
-        self._c = native.KvqPool(fmt, _count(self.head_dim), _count(self.heads_kv), _count(self.n_pages), k.data_ptr(), v.data_ptr(),
+        self._c = native.KvqPool(fmt, self.head_dim, self.heads_kv, self.n_pages, k.data_ptr(), v.data_ptr(),
                                  k_scale.data_ptr(), v_scale.data_ptr())
 
     @classmethod
@@ -89,12 +90,14 @@ class KvqBatch:
         if max_rows < 0:
             _bad("KvqBatch: max_rows is negative")
         self.row_start, self.seq_len, self.pages, self.device, self.max_rows = row_start, seq_len, pages, device, max_rows
-        self._sizes = _count(shape[0]), _count(shape[1])
+        self._sizes = shape[0], max_rows, shape[1]
+        if max(self._sizes) >= 1 << 31:
+            self._sizes = tuple(map(_count, self._sizes))
         self._ptrs = (_int32("row_start", row_start, (shape[0] + 1,), device), _int32("seq_len", seq_len, (shape[0],), device),
                       _int32("pages", pages, shape, device))
 
     def _c(self, rows: int) -> native.KvqBatch:
-        return native.KvqBatch(self._sizes[0], _count(rows), _count(self.max_rows), self._sizes[1], *self._ptrs)
+        return native.KvqBatch(self._sizes[0], rows, self._sizes[1], self._sizes[2], *self._ptrs)
 
 
 def _rows(name: str, t: torch.Tensor, heads: int, dim: int, device: int) -> int:
@@ -165,8 +168,10 @@ def kvq_attention(pool: KvqPool, batch: KvqBatch, q: torch.Tensor, prefix_pages:
         if prefix_pages.dim() != 1 or prefix_pages.shape[0] * PAGE < prefix_len:
             _bad("kvq_attention: prefix_pages holds fewer than prefix_len positions")
         prefix = _int32("prefix_pages", prefix_pages, prefix_pages.shape, device)
+    if not (-1 < window < 1 << 31 and -1 < prefix_len < 1 << 31):
+        window, prefix_len = _count(window), _count(prefix_len)
     L, p, b = lib(), pool._c, batch._c(rows)
-    a = native.KvqAttn(_count(heads), _TYPES[q.dtype], _count(prefix_len), _count(window), pool.head_dim ** -0.5 if scale is None else scale, softcap,
+    a = native.KvqAttn(heads, _TYPES[q.dtype], prefix_len, window, pool.head_dim ** -0.5 if scale is None else scale, softcap,
                        prefix)
     need = C.c_size_t()
     check(L.llmdot_cuda_kvq_attention_workspace(p, b, a, need))
@@ -212,10 +217,12 @@ def verify_draft(p: torch.Tensor, q: Optional[torch.Tensor], draft: torch.Tensor
     ld_q = ld("q", q, k) if q is not None else 0
     if uniform.dtype is not torch.float32 or uniform.shape != (B, k1) or uniform.get_device() != device or not uniform.is_contiguous():
         _bad(f"verify_draft: uniform must be contiguous float32 [{B}, {k1}] on cuda:{device}")
+    if p.shape.numel() >= 1 << 31:
+        k, V = _count(k), _count(V)
     tokens, accepted = p.new_empty((B, k1), dtype=torch.int32), p.new_empty((B,), dtype=torch.int32)
     _call(lib().llmdot_cuda_verify_draft, device,
-          native.Verify(_count(B), _count(k), _count(V), 0, p.data_ptr(), q.data_ptr() if q is not None else None, ld_p, ld_q,
-                        _int32("draft", draft, (B, k), device), uniform.data_ptr(),
+          native.Verify(B, k, V, 0, p.data_ptr(), q.data_ptr() if q is not None else None, ld_p, ld_q,
+                        _int32("draft", draft, (B, k1 - 1), device), uniform.data_ptr(),
                         _int32("n_draft", n_draft, (B,), device) if n_draft is not None else None, tokens.data_ptr(),
                         accepted.data_ptr()))
     return tokens, accepted
