@@ -33,7 +33,7 @@
 // does; then only the rows that need it take new references, so that a row's result does not depend on its neighbours.
 //
 // Measured on a B200, the own pages of 96 sequences with 3 to 5 drafted rows of 4 heads each, 64 to 2048
-// positions of 8 kv heads of 128: 94 us for 224 MB (2.4 TB/s; 0.54 instructions per clock and scheduler).
+// positions of 8 kv heads of 128: 94 us for 224 MB (2.4 TB/s; 0.58 instructions per clock and scheduler).
 // With a page per warp, maxima and O of all dimensions in each warp: 124 us.  Left out in turn (same sizes),
 // the scores' product saved 15 us, the output's 15, the loads 14, all of these 63.
 #include <algorithm>

@@ -14,7 +14,7 @@ struct AttnArgs {
     int64_t ldq, ldo;
     float *lse;
     float *part_o;     // [slots][rows * heads][D]
-    float2 *part_ml;   // [slots][rows * heads]: maximum (base 2), sum
+    float2 *part_ml;   // [slots][rows * heads]: reference (base 2), sum of the exponentials
     int group;         // query heads per kv head
     int ch_p, ch_s;    // pages per chunk: prefix, own pages
     int nsp, nss;      // chunks of the prefix; most chunks of a sequence

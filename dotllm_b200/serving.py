@@ -76,7 +76,8 @@ class KvqPool:
 class KvqBatch:
     """Sequences over a pool: ``pages[b, i]`` holds positions 64 i .. 64 i + 63 of sequence b,
     ``seq_len[b]`` is its length, and rows ``row_start[b] .. row_start[b + 1]`` of a call are its last
-    positions.  ``max_rows`` bounds the rows of any one sequence."""
+    positions.  ``max_rows`` bounds the rows of any one sequence; rows beyond it, and rows of no sequence, leave
+    their part of a call's (new) outputs undefined."""
 
     __slots__ = ("row_start", "seq_len", "pages", "device", "max_rows", "_sizes", "_ptrs")
 

@@ -412,7 +412,10 @@ typedef struct llmdot_kvq_pool {
  * (max_pages entries each); seq_len[b] is its number of positions.  The call's rows are packed:
  * rows row_start[b] .. row_start[b + 1] - 1 are the LAST positions of sequence b, in order (a row
  * that would fall before position 0 is no position).  max_rows bounds the rows of any sequence;
- * rows beyond it are not computed. */
+ * rows beyond it are not attended, and those from row_start[batch] on belong to no sequence: what a
+ * call would write for them is left as it is.  max_pages and max_rows size the attention's launch and
+ * scratch and choose its kernels, whatever the lengths on the device: a table with eight times the pages in
+ * use costs 10 to 40 us an attention call. */
 typedef struct llmdot_kvq_batch {
     int32_t batch;
     int32_t rows; /* row_start[batch] */
@@ -440,8 +443,9 @@ LLMDOT_API int llmdot_cuda_kvq_read(const llmdot_kvq_pool *pool, const llmdot_kv
  * position j of sequence b is prefix_len + j of the whole.  A row at whole position p sees positions
  * <= p, and with window > 0 only those > p - window.  Query head h reads kv head h / (heads /
  * heads_kv).  s = scale * q . k, then softcap * tanh(s / softcap) when softcap > 0; the output is
- * sum softmax(s) v, in `type`; sums and softmax in fp32.  A row that sees nothing gives zeros and a
- * log-sum of -infinity. */
+ * sum softmax(s) v, in `type`.  Scores, exponentials and sums are fp32; products take fp32 queries to 22 bits and
+ * the weights to 22 bits, or to 11 for bf16 queries (an eighth of the output's own rounding).  What a row does
+ * not see does not change it, whatever the scales there.  A row that sees nothing gives zeros and a log-sum of -infinity. */
 typedef struct llmdot_kvq_attn {
     int32_t heads; /* a multiple of heads_kv */
     uint32_t type; /* of q and the output: LLMDOT_F32, LLMDOT_F16 or LLMDOT_BF16 */
