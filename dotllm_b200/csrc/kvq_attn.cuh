@@ -199,8 +199,8 @@ __device__ __forceinline__ bool raise_refs(float top, float topv, float &ref, fl
     if (!first && topv - ref - E < REF_LIMIT - 0.01f && top - ref < SUM_LIMIT_LOG - 7.0f) return false;
     const float d = first ? 0.0f : ceilf(fmaxf(top - ref, 0.0f)), to = first ? top : ref + d;
     const float least = fminf(fmaxf(ceilf(topv - to) - REF_HEAD, -126.0f), 126.0f), Eo = first ? least : fmaxf(E - d, least);
-    fl = ex2(-d);
-    fo = ex2(E - d - Eo);
+    fl = d > 126.0f ? 0.0f : pow2(-(int)d);  // (both 1 for a row that has summed nothing)
+    fo = first || Eo - E + d > 126.0f ? (float)first : pow2((int)(E - d - Eo));
     ref = to;
     unit = __int_as_float((127 - (int)Eo) << 23);
     return true;

@@ -395,7 +395,8 @@ LLMDOT_API int llmdot_cuda_argmax_noalloc(const float *d_logits, int n, int rows
 /* Pool of KV pages held in 8 bits: LLMDOT_KV_PAGE positions of one kv head are one contiguous run
  * of codes, [n_pages][heads_kv][64][head_dim], with one fp32 scale per position and head,
  * [n_pages][heads_kv][64].  A code stands for code * scale.  head_dim is 64, 96, 128 or 256.  The
- * code arrays are 16-byte aligned. */
+ * code arrays are 16-byte aligned.  (e4m3's two NaN codes are never written; the attention takes them as +-480, so a
+ * NaN is held by the scale.) */
 #define LLMDOT_KV_PAGE 64
 #define LLMDOT_KVQ_I8 0   /* signed 8-bit integers, -127..127 */
 #define LLMDOT_KVQ_E4M3 1 /* 8-bit floating point, 4 exponent bits, 3 mantissa bits, largest 448 */
