@@ -35,6 +35,7 @@ int kvq_check(const char *who, const llmdot_kvq_pool *p, const llmdot_kvq_batch 
     if (b->max_pages > (1 << 24)) return bad("max_pages exceeds 2^24 (positions are 32-bit)");
     if (b->batch > 0 && (!b->row_start || !b->seq_len)) return bad("null row_start or seq_len");
     if (b->batch > 0 && b->max_pages > 0 && !b->pages) return bad("null pages");
+    if (((uintptr_t)b->row_start | (uintptr_t)b->seq_len | (uintptr_t)b->pages) & 3) return bad("row_start, seq_len and pages must be 4-byte aligned");
     if (b->rows > 0 && b->batch == 0) return bad("rows without a sequence");
     return LLMDOT_OK;
 }

@@ -754,6 +754,7 @@ int check_attn(const char *who, const llmdot_kvq_pool *p, const llmdot_kvq_batch
     if (a->heads <= 0 || a->heads % p->heads_kv || a->heads > (1 << 16)) return bad("heads must be a multiple of heads_kv, at most 65536");
     if (a->prefix_len < 0 || a->prefix_len > (1 << 30) || a->window < 0) return bad("bad prefix_len or window");
     if (a->prefix_len > 0 && !a->prefix_pages) return bad("null prefix_pages");
+    if ((uintptr_t)a->prefix_pages & 3) return bad("prefix_pages must be 4-byte aligned");
     if (!(a->softcap >= 0.0f) || !(a->softcap < INFINITY) || !(fabsf(a->scale) < INFINITY)) return bad("bad scale or softcap");
     if ((int64_t)b->rows * a->heads > (int64_t)1 << 30) return bad("rows * heads exceeds 2^30");
     return LLMDOT_OK;
@@ -789,6 +790,7 @@ extern "C" int llmdot_cuda_kvq_attention(const llmdot_kvq_pool *pool, const llmd
         if (batch->rows > 1 && (ld_q < row || ld_out < row)) return bad("row stride below heads * head_dim");
         const int es = kvq_type_size(attn->type);
         if (((uintptr_t)d_q | (uintptr_t)d_out) % es) return bad("q or output is not aligned to its type");
+        if ((uintptr_t)d_lse & 3) return bad("lse must be 4-byte aligned");
         const Plan x = make_plan(*pool, *batch, *attn);
         if (x.o_bytes + x.ml_bytes > 0 && (!d_work || work_bytes < x.o_bytes + x.ml_bytes || ((uintptr_t)d_work & 15)))
             return bad("workspace is null, too small or not 16-byte aligned");

@@ -193,6 +193,8 @@ extern "C" int llmdot_cuda_verify_draft(const llmdot_verify *a, void *stream)
         if (!a->p || !a->uniform || !a->tokens || !a->accepted) return bad("null device pointer");
         if (a->drafts > 0 && !a->draft) return bad("null drafts");
         if (((uintptr_t)a->p | (uintptr_t)a->q) & 3) return bad("probabilities must be 4-byte aligned");
+        if (((uintptr_t)a->draft | (uintptr_t)a->uniform | (uintptr_t)a->n_draft | (uintptr_t)a->tokens | (uintptr_t)a->accepted) & 3)
+            return bad("drafts, uniform numbers, counts and results must be 4-byte aligned");
         if (a->ld_p < a->vocab || (a->q && a->ld_q < a->vocab)) return bad("row stride below the vocabulary");
         // CTAs per sequence: as many as still give each warp a block, until the SMs hold two each
         const int blocks = (a->vocab + VBLOCK - 1) / VBLOCK;

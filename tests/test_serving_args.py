@@ -296,3 +296,22 @@ def test_counts_beyond_32_bits_are_not_cut(monkeypatch):
     monkeypatch.setattr(OnDevice, "stride", lambda self: (2 ** 32 + 5, 2 ** 32 + 5, 1) if self is wide else self.t.stride())
     serving.verify_draft(wide, None, ints(1, 0), OnDevice(torch.zeros(1, 1)))
     assert made[-1][0].vocab == 2 ** 31 - 1
+
+
+def test_misaligned_pointers_are_refused():
+    """Lengths, lists, numbers and results off their type's boundary never reach the device."""
+    L = native.lib()
+    need = C.c_size_t()
+    for kw in (dict(row_start=P + 1), dict(seq_len=P + 2), dict(pages=P + 3)):
+        b = batch(**kw)
+        assert L.llmdot_cuda_kvq_write(pool(), b, P, P, 1, 128, 128, None) == INVALID, kw
+        assert L.llmdot_cuda_kvq_read(pool(), b, P, P, 1, 128, 128, None) == INVALID, kw
+        assert L.llmdot_cuda_kvq_attention_workspace(pool(), b, attn(), need) == INVALID, kw
+    a = attn(prefix_len=64, prefix_pages=P + 2)
+    assert L.llmdot_cuda_kvq_attention_workspace(pool(), batch(), a, need) == INVALID
+    assert L.llmdot_cuda_kvq_attention(pool(), batch(), attn(), P, 256, P, 256, P + 2, P, 1 << 30, None) == INVALID
+    assert "aligned" in message()
+    ok = dict(batch=1, drafts=2, vocab=100, p=P, q=P, ld_p=100, ld_q=100, draft=P, uniform=P, n_draft=None, tokens=P, accepted=P)
+    for name in ("p", "q", "draft", "uniform", "n_draft", "tokens", "accepted"):
+        assert L.llmdot_cuda_verify_draft(native.Verify(**dict(ok, **{name: P + 2})), None) == INVALID, name
+        assert "aligned" in message()
