@@ -12,7 +12,11 @@
 // So neither a value that a row does not see nor one that it gives no weight costs it bits, whatever
 // the scales' size.  P is hi + lo, or with bf16 queries, whose output has 8 bits, one fp16 (with fp16 outputs its
 // rounding would add as much error again as the output's own).
-// The sum of exponentials, the maxima, both products' sums and the outputs are fp32.
+// The sum of exponentials, the maxima, both products' sums and the outputs are fp32.  The tensor core truncates what it
+// adds into its accumulators, half a unit of the sum lost per addition, so with fp32 queries a chain of such additions
+// ends after a K piece (64 dimensions or fewer) and after a page, and its sum is added with rounding: 60 drawn
+// cases against 64 bits, 0.73 of the error of 32-bit torch operations in the geometric mean, 4.5e-7 at most (1.23 and 2.9e-6
+// with one chain).
 //
 // Work is cut into segments -- the prefix with every row of the batch, each sequence's own pages with
 // its rows -- times kv heads, row tiles and chunks of pages.  The prefix is read once per row tile of
@@ -144,6 +148,7 @@ __global__ void __launch_bounds__(NW * 32, narrow_regs_ctas(D, NT)) kvq_attn_ker
     using Sh = Shape<D>;
     constexpr int RT = 8 * NT, QS = D + Sh::QPAD, NQ = PREC == 2 ? 2 : 1, NP = PREC > 0 ? 2 : 1;
     constexpr bool QREG = NT * NQ * D / 8 <= 32;  // the query's fragments stay in registers
+    constexpr bool ROUNDED = PREC == 2;           // short chains of tensor-core additions
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float s_qf[RT], s_max[NW][RT], s_l[NW][RT];  // s_l: at the end; before, maxima with the values' scales
     __shared__ int s_lo[RT], s_hi[RT], s_row[RT];
@@ -340,6 +345,8 @@ __global__ void __launch_bounds__(NW * 32, narrow_regs_ctas(D, NT)) kvq_attn_ker
                 uint32_t ql[NQ][NT][Sh::KB / 2];
                 if (!QREG) query(c, ql);
                 const uint32_t (&qb)[NQ][NT][Sh::KB / 2] = QREG ? qr[QREG ? c : 0] : ql;
+                float piece[NT][4] = {};
+                float (&acc)[NT][4] = ROUNDED && Sh::KC > 1 ? piece : s;
                 uint32_t w[2][Sh::KB / 4];
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
@@ -353,8 +360,13 @@ __global__ void __launch_bounds__(NW * 32, narrow_regs_ctas(D, NT)) kvq_attn_ker
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int h = 0; h < NQ; h++) mma(s[nt], f, qb[h][nt][2 * k], qb[h][nt][2 * k + 1]);
+                        for (int h = 0; h < NQ; h++) mma(acc[nt], f, qb[h][nt][2 * k], qb[h][nt][2 * k + 1]);
                 }
+                if (ROUNDED && Sh::KC > 1)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s[nt][e] += piece[nt][e];
             }
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
@@ -427,6 +439,8 @@ __global__ void __launch_bounds__(NW * 32, narrow_regs_ctas(D, NT)) kvq_attn_ker
         // ---- O^T += V^T P^T: 32 dimensions
         if (D != 96 || warp < 3) {
             const uint8_t *vslot = smem + (2 + sl) * Sh::SLOT;
+            float page[Sh::GPW][2][NT][4] = {};
+            float (&acc)[Sh::GPW][2][NT][4] = ROUNDED ? page : o;
 #pragma unroll
             for (int m = 0; m < (D == 64 ? 2 : 4); m++) {
                 const int mt = mt0 + m;
@@ -450,10 +464,19 @@ __global__ void __launch_bounds__(NW * 32, narrow_regs_ctas(D, NT)) kvq_attn_ker
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                            for (int h = 0; h < NP; h++) mma(o[q][hf][nt], fr, pb[h][nt].x, pb[h][nt].y);
+                            for (int h = 0; h < NP; h++) mma(acc[q][hf][nt], fr, pb[h][nt].x, pb[h][nt].y);
                     }
                 }
             }
+            if (ROUNDED)
+#pragma unroll
+                for (int q = 0; q < Sh::GPW; q++)
+#pragma unroll
+                    for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[q][hf][nt][e] += page[q][hf][nt][e];
         }
     }
     cp_wait<0>();
@@ -602,9 +625,7 @@ template <int D, int FMT, int PREC> cudaError_t launch_nt(int nt, const AttnArgs
     case 1: return launch_tiles<D, FMT, 1, PREC>(a, grid, st);
     case 2: return launch_tiles<D, FMT, 2, PREC>(a, grid, st);
     case 3: return launch_tiles<D, FMT, 3, PREC>(a, grid, st);
-    case 8:
-        if constexpr (PREC == 2 && D != 256) return launch_tiles<D, FMT, 8, PREC>(a, grid, st);  // others: 32 rows at most (wide_pays)
-    default: return launch_tiles<D, FMT, 4, PREC>(a, grid, st);
+    default: return launch_tiles<D, FMT, D == 256 && PREC == 2 ? 3 : 4, PREC>(a, grid, st);
     }
 }
 template <int D, int FMT> cudaError_t launch_prec(int nt, const AttnArgs &a, int64_t grid, cudaStream_t st)
@@ -653,10 +674,14 @@ struct Plan {
     int64_t ctas_p, ctas_s;
     size_t o_bytes, ml_bytes;
 };
-int tiles_of(int dim, int64_t rows)  // 8-row tiles per CTA: 1, 2, 3, 4 or (fp32 queries) 8, 4 with head_dim 256
+// 8-row tiles per CTA, 1 to 4.  16-bit queries of more than 32 rows go to the wide kernel; fp32 ones take several CTAs: a tile of
+// 64 rows leaves two CTAs per SM and spills (512 rows, heads of 64 / 96 / 128: 263 / 424 / 447 us; 32: 221 / 286 / 310).  fp32 and
+// head_dim 256, where 32 rows fill an SM's shared memory: 16 up to 32 rows, else 24 (4 x 4 rows on a prefix of 6144: 16 28.9, 24
+// 33.5, 32 39.0; 80 rows on 3000: 39.1, 31.6, 53.0; 512 rows: 634, 522, 669).
+int tiles_of(int dim, int64_t rows, uint32_t type)
 {
     const int64_t n = std::max<int64_t>(1, (rows + 7) / 8);
-    return (int)(n <= 4 ? n : dim == 256 ? 4 : 8);
+    return (int)std::min<int64_t>(n, type != T_F32 || dim != 256 ? 4 : n <= 4 ? 2 : 3);
 }
 // Whether `rows` rows (times heads) per kv head over `items` pages and heads in all go to the wide kernel.  It takes
 // the same time for 1 to 256 rows, the narrow one grows with every 8 up to 32 rows and then takes 64.  Some thousand
@@ -690,8 +715,8 @@ Plan make_plan(const llmdot_kvq_pool &p, const llmdot_kvq_batch &b, const llmdot
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
     x.wide_p = a.type != T_F32 && npp > 0 && wide_pays(p, all_rows, Hk * npp, false);
     x.wide_s = a.type != T_F32 && wide_pays(p, own_rows, times(Hk * b.batch, b.max_pages), true);
-    x.nt_p = tiles_of(p.head_dim, all_rows);
-    x.nt_s = tiles_of(p.head_dim, own_rows);
+    x.nt_p = tiles_of(p.head_dim, all_rows, a.type);
+    x.nt_s = tiles_of(p.head_dim, own_rows, a.type);
     if (npp == 0) x.nt_p = x.nt_s;
     x.ptiles = (int)up(all_rows, x.wide_p ? wide : 8 * x.nt_p);
     x.rtiles = (int)std::max<int64_t>(1, up(own_rows, x.wide_s ? wide : 8 * x.nt_s));

@@ -376,3 +376,38 @@ def test_subnormal_fp16_queries(gpu, dim, fmt, group):
     q = queries(13, "f16", 3, 2 * group, dim, scale=2.0 ** -17)
     c.check(q, "f16", c.attend(q))
     c.check(q, "f16", c.attend(q, window=90), window=90)
+
+
+@pytest.mark.parametrize("dim,fmt", [(64, "i8"), (96, "e4m3"), (128, "i8"), (256, "e4m3")])
+@pytest.mark.parametrize("group,rows,prefix,own", [(2, [7] * 25, 2148, 17), (4, [100], 4000, 300), (1, [1], 0, 1900), (8, [1] * 3, 6239, 121)])
+def test_fp32_sums_keep_32_bits(gpu, dim, fmt, group, rows, prefix, own):
+    """fp32 queries: no further from 64 bits, in the norm of all rows, than torch operations in 32 bits are, but for 2^-20.  That is 2^-21
+    for sums that the tensor core truncates (half a unit, 2^-24, an addition, eight additions before one that rounds), 2^-22 for
+    the exponential and 2^-22 for queries and weights of 22 bits."""
+    import torch
+    hk = 4
+    parts = random_parts(20, hk, dim, prefix, *[own] * len(rows))
+    c = Held(fmt, parts, rows)
+    q = queries(14, "f32", sum(rows), hk * group, dim)
+    out = c.attend(q)[0]
+    far, plain, size, r = 0.0, 0.0, 0.0, 0
+    for b, n in enumerate(rows):
+        T = prefix + own
+        p = T - n + torch.arange(n, device="cuda").repeat_interleave(group)[:, None]
+        gone = torch.arange(T, device="cuda")[None] > p
+
+        def rows_of(x):
+            return x[r:r + n].reshape(n, hk, group, dim).permute(1, 0, 2, 3).reshape(hk, n * group, dim)
+
+        def attend(t):
+            k, v = (torch.cat([x[0], x[1 + b]]).transpose(0, 1).to(t) for x in c.values)
+            s = (rows_of(q).to(t) @ k.transpose(1, 2) * dim ** -0.5).masked_fill(gone, float("-inf"))
+            w = torch.exp(s - s.amax(-1, keepdim=True))
+            return (w @ v / w.sum(-1, keepdim=True)).double()
+
+        want = attend(torch.float64)
+        far += float((rows_of(out).double() - want).square().sum())
+        plain += float((attend(torch.float32) - want).square().sum())
+        size += float(want.square().sum())
+        r += n
+    assert (far / size) ** 0.5 <= (plain / size) ** 0.5 + 2.0 ** -20, ((far / size) ** 0.5, (plain / size) ** 0.5)
