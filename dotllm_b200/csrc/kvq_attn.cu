@@ -684,7 +684,7 @@ int tiles_of(int dim, int64_t rows, uint32_t type)
     return (int)std::min<int64_t>(n, type != T_F32 || dim != 256 ? 4 : n <= 4 ? 2 : 3);
 }
 // Whether `rows` rows (times heads) per kv head over `items` pages and heads in all go to the wide kernel.  It takes
-// the same time for 1 to 256 rows, the narrow one grows with every 8 up to 32 rows and then takes 64.  Some thousand
+// the same time for 1 to 256 rows, the narrow one grows with every 8 (above 32 rows measured with a tile of 64).  Some thousand
 // positions, 8 kv heads (or as said), bf16, heads of 64 / 96 / 128 / 256, us, wide : narrow.
 //   Work enough for all SMs, so that only throughput counts, own pages of 24 sequences, 4608 items: 32 rows 62 : 46 / 68 : 64 /
 //   72 : 72 / 128 : 115, 40 rows 62 : 68 / 68 : 92 / 72 : 103 / 128 : 161; 96 sequences, fp16, heads of 64: 40 rows 165 : 160.
